@@ -7,7 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import POINTER, Structure, c_float, c_int, c_longlong, c_void_p
+from ctypes import POINTER, Structure, c_double, c_float, c_int, c_longlong, c_void_p
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libglmasr_fp4.so")
@@ -28,7 +28,15 @@ class LayerWeights(Structure):
                 ("hidden", c_int), ("ffn", c_int)]
 
 
+class Kv8Cache(Structure):
+    """``glmasr_kv8_cache`` of include/glmasr_fp4.h."""
+
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p),
+                ("num_blocks", c_int), ("block_size", c_int), ("kv_heads", c_int), ("head_dim", c_int)]
+
+
 P = c_void_p
+L = c_longlong
 #: symbol -> (restype, argtypes); must list every function include/glmasr_fp4.h declares
 SIGNATURES = {
     "fp4_dequant_to_bf16": (None, [P, P, P, c_float, c_int, c_int]),
@@ -84,6 +92,10 @@ SIGNATURES = {
     "glmasr_fp4_layer_proj": (c_int, [c_int, P, P, POINTER(LayerWeights), c_int]),
     "glmasr_fp4_layer_proj_host": (c_int, [c_int, P, P, POINTER(LayerWeights), c_int]),
     "glmasr_nvfp4_linear_noalloc": (c_int, [P, P, P, P, c_float, c_float, c_int, c_int, c_int]),
+    "glmasr_kv8_append": (c_int, [POINTER(Kv8Cache), P, L, P, L, P, L, P, L, c_int, P, c_int, P, P, c_int, c_int, c_double]),
+    "glmasr_kv8_attention_workspace": (L, [c_int]),
+    "glmasr_kv8_attention": (c_int, [P, L, P, L, POINTER(Kv8Cache), P, c_int, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
+                                     c_float, P, L]),
     "glmasr_fp4_status": (c_int, []),
     "glmasr_last_gemm_route": (c_int, []),
     "glmasr_launch_count": (c_longlong, []),

@@ -1,0 +1,92 @@
+// C entry points of the 8-bit paged cache: argument checks, then the launches (kv8_append.cu, kv8_attention.cu).
+#include <math.h>
+
+#include "../../include/glmasr_fp4.h"
+#include "kv8_attention.cuh"
+#include "runtime.cuh"
+
+using namespace glmasr;
+
+namespace {
+
+bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
+
+// The shape of cache and batch; what a kernel could not index safely is refused here.
+bool make_batch(Kv8Batch &b, const glmasr_kv8_cache *c, const int *block_tables, int max_blocks, const int *seq_lens, const int *cu_new,
+                int num_seqs, int total_new, int q_heads) {
+    if (c == nullptr || c->k == nullptr || c->v == nullptr || c->k_scale == nullptr || c->v_scale == nullptr) return false;
+    if (!aligned16(c->k) || !aligned16(c->v) || ((uintptr_t)c->k_scale & 3) != 0 || ((uintptr_t)c->v_scale & 3) != 0) return false;
+    if (c->head_dim != kKv8Dim || c->kv_heads <= 0 || c->num_blocks <= 0 || c->block_size <= 0 || c->block_size % kKv8Group != 0) return false;
+    if (num_seqs < 0 || total_new < 0 || max_blocks <= 0 || q_heads < 0) return false;
+    if ((num_seqs > 0 && total_new > 0) && (block_tables == nullptr || seq_lens == nullptr || cu_new == nullptr)) return false;
+    if ((((uintptr_t)block_tables | (uintptr_t)seq_lens | (uintptr_t)cu_new) & 3) != 0) return false;
+    b.block_tables = block_tables;
+    b.seq_lens = seq_lens;
+    b.cu_new = cu_new;
+    b.num_seqs = num_seqs;
+    b.max_blocks = max_blocks;
+    b.num_blocks = c->num_blocks;
+    b.block_size = c->block_size;
+    b.kv_heads = c->kv_heads;
+    b.q_heads = q_heads;
+    b.total_new = total_new;
+    return true;
+}
+
+// rows of `heads` heads of 128 at a pitch of ld elements, read and written 16 bytes at a time
+bool rows_ok(const void *p, long long ld, int heads, int rows) {
+    return p != nullptr && aligned16(p) && ld % 8 == 0 && (rows <= 1 || ld >= (long long)heads * kKv8Dim);
+}
+
+}  // namespace
+
+extern "C" int glmasr_kv8_append(const glmasr_kv8_cache *cache, const uint16_t *key, long long ldk, const uint16_t *value, long long ldv,
+                                 const uint16_t *query, long long ldq, uint16_t *query_out, long long ldqo, int q_heads,
+                                 const int *block_tables, int max_blocks, const int *seq_lens, const int *cu_new, int num_seqs,
+                                 int total_new, double theta) {
+    Kv8Batch b;
+    if (!make_batch(b, cache, block_tables, max_blocks, seq_lens, cu_new, num_seqs, total_new, query != nullptr ? q_heads : 0)) return -1;
+    if (!isfinite(theta) || theta < 0.0 || (query != nullptr && q_heads <= 0) || (query == nullptr) != (query_out == nullptr)) return -1;
+    if (num_seqs == 0 || total_new == 0) return 0;
+    if (!rows_ok(key, ldk, b.kv_heads, total_new) || !rows_ok(value, ldv, b.kv_heads, total_new)) return -1;
+    if (query != nullptr && (!rows_ok(query, ldq, q_heads, total_new) || !rows_ok(query_out, ldqo, q_heads, total_new))) return -1;
+    if (!kv8_append_launch(cache->k, cache->v, cache->k_scale, cache->v_scale, (const __nv_bfloat16 *)key, ldk, (const __nv_bfloat16 *)value, ldv,
+                           (const __nv_bfloat16 *)query, ldq, (__nv_bfloat16 *)query_out, ldqo, b, theta, current_stream())) {
+        (void)cudaGetLastError();
+        return -1;
+    }
+    note_launches(1);
+    return 0;
+}
+
+extern "C" long long glmasr_kv8_attention_workspace(int num_seqs) {
+    return num_seqs < 0 ? -1 : (long long)kv8_attention_workspace_bytes(num_seqs);
+}
+
+extern "C" int glmasr_kv8_attention(uint16_t *out, long long ldo, const uint16_t *query, long long ldq, const glmasr_kv8_cache *cache,
+                                    const int *block_tables, int max_blocks, const int *seq_lens, const int *cu_new, int num_seqs,
+                                    int total_new, int q_heads, int max_new, int max_len, int window, int sinks, float scale,
+                                    void *workspace, long long workspace_bytes) {
+    Kv8Attend a;
+    if (!make_batch(a.b, cache, block_tables, max_blocks, seq_lens, cu_new, num_seqs, total_new, q_heads)) return -1;
+    if (q_heads <= 0 || q_heads % a.b.kv_heads != 0 || window < 0 || sinks < 0 || max_new < 0 || max_len < 0 || !isfinite(scale)) return -1;
+    if (num_seqs == 0 || total_new == 0) return 0;
+    if (!rows_ok(query, ldq, q_heads, total_new) || !rows_ok(out, ldo, q_heads, total_new)) return -1;
+    if (workspace == nullptr || !aligned16(workspace) || workspace_bytes < glmasr_kv8_attention_workspace(num_seqs)) return -1;
+    a.k_cache = cache->k, a.v_cache = cache->v;
+    a.k_scale = cache->k_scale, a.v_scale = cache->v_scale;
+    a.query = (const __nv_bfloat16 *)query;
+    a.out = (__nv_bfloat16 *)out;
+    a.ldq = ldq, a.ldo = ldo;
+    a.group = q_heads / a.b.kv_heads;
+    a.window = window;
+    a.sinks = sinks;
+    a.scale_log2 = scale * 1.4426950408889634f;
+    int launches = 0;
+    if (!kv8_attention_launch(a, max_new, max_len, workspace, current_stream(), launches)) {
+        (void)cudaGetLastError();
+        return -1;
+    }
+    note_launches(launches);
+    return 0;
+}

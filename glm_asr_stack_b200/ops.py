@@ -268,6 +268,137 @@ def paged_decode_attention(query, k_cache, v_cache, block_tables, seq_lens, num_
     return out
 
 
+def _kv8_rows(t: torch.Tensor, name: str, device, heads: Optional[int] = None):
+    """Rows of heads * 128 bf16 elements at any pitch: [rows, heads, 128]."""
+    if t.dtype != torch.bfloat16:
+        raise TypeError(f"{name}: expected torch.bfloat16, got {t.dtype}")
+    if t.dim() != 3 or t.shape[2] != 128 or t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != 128):
+        raise ValueError(f"{name}: must be [rows, heads, 128] with the heads of a row side by side")
+    if t.device != device:
+        raise ValueError(f"{name}: not on the cache's device")
+    if heads is not None and t.shape[1] != heads:
+        raise ValueError(f"{name}: expected {heads} heads, got {t.shape[1]}")
+
+
+def _kv8_cache(k_cache, v_cache, k_scale, v_scale):
+    device = k_cache.device
+    if device.type != "cuda":
+        raise ValueError("expected a CUDA tensor")
+    if device.index != torch.cuda.current_device():
+        raise ValueError("the cache is not on the current device")
+    for t, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
+        if t.dtype not in (torch.float8_e4m3fn, torch.uint8):
+            raise TypeError(f"{name}: expected torch.float8_e4m3fn or torch.uint8, got {t.dtype}")
+    shape = k_cache.shape
+    if len(shape) != 4 or v_cache.shape != shape or not k_cache.is_contiguous() or not v_cache.is_contiguous():
+        raise ValueError("k_cache, v_cache: must be contiguous [num_blocks, kv_heads, block_size, 128] of one shape")
+    for t, name in ((k_scale, "k_scale"), (v_scale, "v_scale")):
+        _check(t, torch.float32, name)
+        if t.shape != (shape[0], shape[1], shape[2] // 16):
+            raise ValueError(f"{name}: must be [num_blocks, kv_heads, block_size / 16]")
+    if v_cache.device != device or k_scale.device != device or v_scale.device != device:
+        raise ValueError("codes and scales must be on one device")
+    return _lib.Kv8Cache(k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), shape[0], shape[2], shape[1],
+                         shape[3]), device
+
+
+def _kv8_batch(block_tables, seq_lens, cu_new, device):
+    _check(block_tables, torch.int32, "block_tables")
+    _check(seq_lens, torch.int32, "seq_lens")
+    _check(cu_new, torch.int32, "cu_new")
+    n = seq_lens.numel()
+    if block_tables.dim() != 2 or block_tables.shape[0] != n or seq_lens.dim() != 1 or cu_new.dim() != 1 or cu_new.numel() != n + 1:
+        raise ValueError("expected block_tables [num_seqs, max_blocks], seq_lens [num_seqs], cu_new [num_seqs + 1]")
+    if block_tables.device != device or seq_lens.device != device or cu_new.device != device:
+        raise ValueError("block_tables, seq_lens, cu_new: not on the cache's device")
+    return n
+
+
+def kv8_append(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, key: torch.Tensor,
+               value: torch.Tensor, block_tables: torch.Tensor, seq_lens: torch.Tensor, cu_new: torch.Tensor,
+               query: Optional[torch.Tensor] = None, query_out: Optional[torch.Tensor] = None,
+               theta: float = 10000.0) -> Optional[torch.Tensor]:
+    """New tokens into the 8-bit paged cache (glmasr_kv8_append): keys, and queries where given, are rotated to their positions,
+    keys and values quantised to e4m3 with one power-of-two scale per 16 tokens and head.
+
+    k_cache, v_cache [num_blocks, kv_heads, block_size, 128] (float8_e4m3fn or uint8), k_scale, v_scale float32
+    [num_blocks, kv_heads, block_size / 16]; key, value [tokens, kv_heads, 128], query [tokens, q_heads, 128] bf16, row slices
+    of a fused projection included.  Sequence s owns the rows cu_new[s] .. cu_new[s + 1] and has seq_lens[s] tokens WITH them
+    (device int32).  theta = 0: no rotation.  Returns the rotated queries (query_out, which may be query itself), or None."""
+    cache, device = _kv8_cache(k_cache, v_cache, k_scale, v_scale)
+    n = _kv8_batch(block_tables, seq_lens, cu_new, device)
+    kv_heads = k_cache.shape[1]
+    _kv8_rows(key, "key", device, kv_heads)
+    _kv8_rows(value, "value", device, kv_heads)
+    tokens = key.shape[0]
+    if value.shape[0] != tokens:
+        raise ValueError("key and value: different numbers of rows")
+    q = qo = None
+    q_heads = ldq = ldqo = 0
+    if query is not None:
+        _kv8_rows(query, "query", device)
+        if query_out is None:
+            query_out = torch.empty(query.shape, dtype=torch.bfloat16, device=device)
+        else:
+            _kv8_rows(query_out, "query_out", device, query.shape[1])
+        if query.shape[0] != tokens or query_out.shape[0] != tokens:
+            raise ValueError("query, query_out: not as many rows as key")
+        q, qo, q_heads, ldq, ldqo = query.data_ptr(), query_out.data_ptr(), query.shape[1], query.stride(0), query_out.stride(0)
+    elif query_out is not None:
+        raise ValueError("query_out without query")
+    if n == 0 or tokens == 0:
+        return query_out
+    rc = _lib.load().glmasr_kv8_append(ctypes.byref(cache), key.data_ptr(), key.stride(0), value.data_ptr(), value.stride(0), q, ldq, qo, ldqo,
+                                       q_heads, block_tables.data_ptr(), block_tables.shape[1], seq_lens.data_ptr(), cu_new.data_ptr(),
+                                       n, tokens, theta)
+    if rc != 0:
+        raise ValueError("glmasr_kv8_append rejected the arguments")
+    return query_out
+
+
+def kv8_attention(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                  block_tables: torch.Tensor, seq_lens: torch.Tensor, cu_new: torch.Tensor, max_new: Optional[int] = None,
+                  max_len: Optional[int] = None, window: int = 0, sinks: int = 0, scale: Optional[float] = None,
+                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of the new tokens' (rotated) queries over the 8-bit paged cache (glmasr_kv8_attention), after kv8_append of the
+    same batch: decode steps, drafted tokens, prompts and pieces of prompts.
+
+    query [tokens, q_heads, 128] bf16; the rest as in kv8_append.  The query at position p sees the positions j <= p with
+    window == 0, or p - j < window, or j < sinks; one that sees nothing gets zeros.  max_new / max_len: the most new tokens and
+    the longest sequence to expect -- they choose kernels, not results (default: all rows / the table's width).  scale defaults to
+    128 ** -0.5.  Rows behind cu_new[num_seqs] are left as they are.  out must not overlap query."""
+    cache, device = _kv8_cache(k_cache, v_cache, k_scale, v_scale)
+    n = _kv8_batch(block_tables, seq_lens, cu_new, device)
+    _kv8_rows(query, "query", device)
+    tokens, q_heads, _ = query.shape
+    if q_heads == 0 or q_heads % k_cache.shape[1] != 0:
+        raise ValueError("query: the head count must be a multiple of the cache's")
+    if out is None:
+        out = torch.empty((tokens, q_heads, 128), dtype=torch.bfloat16, device=device)
+    else:
+        _kv8_rows(out, "out", device, q_heads)
+        if out.shape[0] != tokens:
+            raise ValueError("out: not as many rows as query")
+        if out.data_ptr() == query.data_ptr() and tokens > 0:
+            raise ValueError("out must not overlap query")
+    if n == 0 or tokens == 0:
+        return out
+    lib = _lib.load()
+    size = lib.glmasr_kv8_attention_workspace(n)
+    workspace = torch.empty(size, dtype=torch.uint8, device=device)
+    rc = lib.glmasr_kv8_attention(out.data_ptr(), out.stride(0), query.data_ptr(), query.stride(0), ctypes.byref(cache),
+                                  block_tables.data_ptr(), block_tables.shape[1], seq_lens.data_ptr(), cu_new.data_ptr(), n, tokens,
+                                  q_heads, tokens if max_new is None else max_new,
+                                  block_tables.shape[1] * k_cache.shape[2] if max_len is None else max_len, window, sinks,
+                                  128 ** -0.5 if scale is None else scale, workspace.data_ptr(), size)
+    if rc != 0:
+        raise ValueError("glmasr_kv8_attention rejected the arguments")
+    used = _stream if _stream is not None else torch.cuda.default_stream(device)
+    if used.cuda_stream != torch.cuda.current_stream(device).cuda_stream:
+        workspace.record_stream(used)            # it came from another stream than the one that works on it
+    return out
+
+
 def argmax_rows(logits: torch.Tensor) -> torch.Tensor:
     lib = _lib.load()
     _check(logits, torch.bfloat16, "logits")
@@ -567,7 +698,12 @@ def profile_read(max_entries: int = 4096):
     return [(ms[i], fl[i], by[i]) for i in range(n)]
 
 
+_stream: Optional[torch.cuda.Stream] = None
+
+
 def set_stream(stream: Optional[torch.cuda.Stream]):
+    global _stream
+    _stream = stream
     _lib.load().glmasr_set_stream(ctypes.c_void_p(stream.cuda_stream) if stream is not None else None)
 
 

@@ -397,6 +397,47 @@ long long glmasr_launch_count(void);
  * launch order and clears the list.  Off by default. */
 void glmasr_profile_enable(int on);
 int glmasr_profile_read(int max_entries, double *ms, double *flops, double *bytes);
+/* ---- the 8-bit paged KV cache: no counterpart in the reference, whose cache is bf16 ----
+ * One layer's pool.  codes: e4m3 [num_blocks][kv_heads][block_size][128]; scales: fp32 [num_blocks][kv_heads][block_size / 16],
+ * one power of two per 16 tokens of a head, the smallest 2^e (e >= -126) with amax <= 448 * 2^e; value = code * scale.
+ * head_dim is 128, block_size a multiple of 16; codes 16-byte aligned.  A block of 16 tokens that got a value which is not
+ * finite, or beyond 448 * 2^60, has the scale NaN until its first token is written again, and queries that see it get NaN.
+ *
+ * A batch (both calls): sequence s has the packed rows [cu_new[s], cu_new[s + 1]) as its new tokens and seq_lens[s] tokens with
+ * them; row i of its n is at position seq_lens[s] - n + i, and position p lies in page block_tables[s][p / block_size].  All three
+ * are device arrays (int32), block_tables [num_seqs, max_blocks].  A sequence may have no new token.  A page that is not in
+ * [0, num_blocks), and a position below zero or behind the table, holds nothing: not written, not seen.  Rows of the packed
+ * arrays behind the last sequence are neither read nor written. */
+typedef struct {
+    uint8_t *k, *v;
+    float *k_scale, *v_scale;
+    int num_blocks, block_size, kv_heads, head_dim;
+} glmasr_kv8_cache;
+
+/* Rotate the new tokens' queries and keys to their positions (rotate-half, angle p * theta^(-2 d / 128) in 64 bits; theta = 0:
+ * no rotation) and write keys and values to the cache: per block of 16 positions the scale is that of its new tokens, or the
+ * one it had where that is larger and the block holds earlier tokens; their codes are rescaled when it grows.  Two sequences
+ * must not append to the same block in one call.  key, value, query, query_out: bf16 rows of kv_heads (q_heads) * 128 elements, row
+ * pitches in elements, multiples of 8, 16-byte aligned.  query and query_out may both be NULL, and may be the same rows.
+ * Returns 0, or -1 on bad arguments or a launch failure. */
+int glmasr_kv8_append(const glmasr_kv8_cache *cache, const uint16_t *key, long long ldk, const uint16_t *value, long long ldv,
+                      const uint16_t *query, long long ldq, uint16_t *query_out, long long ldqo, int q_heads,
+                      const int *block_tables, int max_blocks, const int *seq_lens, const int *cu_new, int num_seqs,
+                      int total_new, double theta);
+
+/* Softmax attention of the new tokens' queries (already rotated) over the cache, which holds the new tokens too: the query at
+ * position p sees the positions j <= p with window == 0, or p - j < window, or j < sinks.  A query that sees nothing gets zeros.
+ * out, query: bf16 [total_new, q_heads * 128] with row pitches ldo, ldq (multiples of 8; 16-byte aligned); q_heads a multiple of
+ * kv_heads.  scale: of the scores, before the softmax.  max_new (new tokens of a sequence) and max_len (tokens of a sequence)
+ * say what to expect: they choose kernels and never change what is computed.  |query| < 2^63.
+ * workspace: glmasr_kv8_attention_workspace(num_seqs) bytes of device memory, 16-byte aligned, contents irrelevant, not shared
+ * with a call that may run at the same time.  num_seqs <= 4096.  Returns 0, or -1 on bad arguments or a launch failure. */
+long long glmasr_kv8_attention_workspace(int num_seqs);
+int glmasr_kv8_attention(uint16_t *out, long long ldo, const uint16_t *query, long long ldq, const glmasr_kv8_cache *cache,
+                         const int *block_tables, int max_blocks, const int *seq_lens, const int *cu_new, int num_seqs,
+                         int total_new, int q_heads, int max_new, int max_len, int window, int sinks, float scale,
+                         void *workspace, long long workspace_bytes);
+
 /* Route all launches to the given cudaStream_t (NULL = legacy default stream). */
 void glmasr_set_stream(void *cuda_stream);
 /* Free every private workspace / cache (decoder_cleanup_all / lm_head_cleanup analogue). */
