@@ -18,6 +18,7 @@
 #include "gemm_simt.cuh"
 #include "gemm_skinny.cuh"
 #include "gemm_umma.cuh"
+#include "kv8.cuh"
 #include "runtime.cuh"
 
 namespace glmasr {
@@ -1650,7 +1651,8 @@ extern "C" int glmasr_fp4_status(void) {
         if (host[0] != 0) cudaMemset(g_noalloc_status_ptr[dev], 0, sizeof(host));
         if (code == 0) code = host[0];
     }
-    return code;
+    const int kv8 = kv8_take_status();
+    return code != 0 ? code : kv8;
 }
 
 extern "C" int glmasr_last_gemm_route(void) { return g_last_route; }

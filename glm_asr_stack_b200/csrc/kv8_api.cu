@@ -17,9 +17,12 @@ bool make_batch(Kv8Batch &b, const glmasr_kv8_cache *c, const int *block_tables,
     if (c == nullptr || c->k == nullptr || c->v == nullptr || c->k_scale == nullptr || c->v_scale == nullptr) return false;
     if (!aligned16(c->k) || !aligned16(c->v) || ((uintptr_t)c->k_scale & 3) != 0 || ((uintptr_t)c->v_scale & 3) != 0) return false;
     if (c->head_dim != kKv8Dim || c->kv_heads <= 0 || c->num_blocks <= 0 || c->block_size <= 0 || c->block_size % kKv8Group != 0) return false;
+    if ((long long)c->num_blocks * c->kv_heads > 0x7FFFFFFFLL / c->block_size) return false;      // rows of codes are numbered in 32 bits
     if (num_seqs < 0 || total_new < 0 || max_blocks <= 0 || q_heads < 0) return false;
     if ((num_seqs > 0 && total_new > 0) && (block_tables == nullptr || seq_lens == nullptr || cu_new == nullptr)) return false;
     if ((((uintptr_t)block_tables | (uintptr_t)seq_lens | (uintptr_t)cu_new) & 3) != 0) return false;
+    b.by_kv_heads = FastDiv(c->kv_heads);
+    b.by_page = FastDiv(c->block_size / kKv8Group);
     b.block_tables = block_tables;
     b.seq_lens = seq_lens;
     b.cu_new = cu_new;
@@ -78,7 +81,10 @@ extern "C" int glmasr_kv8_attention(uint16_t *out, long long ldo, const uint16_t
     a.query = (const __nv_bfloat16 *)query;
     a.out = (__nv_bfloat16 *)out;
     a.ldq = ldq, a.ldo = ldo;
+    if ((long long)total_new * q_heads > 0x7FFFFF00LL) return -1;                // rows are numbered in 32 bits
     a.group = q_heads / a.b.kv_heads;
+    a.by_group = FastDiv(a.group);
+    a.by_q_heads = FastDiv(q_heads);
     a.window = window;
     a.sinks = sinks;
     a.scale_log2 = scale * 1.4426950408889634f;

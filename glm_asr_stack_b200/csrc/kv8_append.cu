@@ -65,6 +65,9 @@ __device__ __forceinline__ int scale_exponent(uint32_t amax) {
 }
 __device__ __forceinline__ float pow2f(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }     // e in [-126, 127]
 
+// Angle tables: entry [token][j][i] is dim pair 8 i + j, so that the eight lanes that share a row read side by side.
+__device__ __forceinline__ int angle_at(int token, int d) { return token * HALF + (d & 7) * 8 + (d >> 3); }
+
 // One head of one block, K (rotated) or V, by a warp.  Half a warp per token: lane c (0..15) of it has dims 8c .. 8c + 7, two tokens
 // per step.
 template <bool KEY>
@@ -90,11 +93,11 @@ __device__ __forceinline__ void quantise_head(const AppendParams &p, int head, i
         if (KEY && 2 * i < n) {
             // the other half of the dims is eight lanes away; y = own * cos -+ other * sin
             const double sign = c < 8 ? -1.0 : 1.0;
-            const double2 *a = angles + min(t, n - 1) * HALF + (c & 7) * 8;
+            const double2 *a = angles + min(t, n - 1) * HALF + (c & 7);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const uint32_t other = __shfl_xor_sync(0xFFFFFFFFu, own[j], 8);
-                const double2 a0 = a[2 * j], a1 = a[2 * j + 1];
+                const double2 a0 = a[16 * j], a1 = a[16 * j + 8];
                 x[i][2 * j] = cut_odd(fma((double)x[i][2 * j], a0.x, sign * a0.y * (double)bf16_lo(other)));
                 x[i][2 * j + 1] = cut_odd(fma((double)x[i][2 * j + 1], a1.x, sign * a1.y * (double)bf16_hi(other)));
             }
@@ -127,7 +130,7 @@ __device__ __forceinline__ void quantise_head(const AppendParams &p, int head, i
             uint32_t v[2] = {w.x, w.y};
 #pragma unroll
             for (int j = 0; j < 2; ++j)
-                v[j] = poisoned ? 0x7F7F7F7Fu
+                v[j] = poisoned ? 0u
                                 : e4m3x4(e4m3_value(v[j] & 0xFFu) * ratio, e4m3_value((v[j] >> 8) & 0xFFu) * ratio,
                                          e4m3_value((v[j] >> 16) & 0xFFu) * ratio, e4m3_value(v[j] >> 24) * ratio);
             *at = make_uint2(v[0], v[1]);
@@ -138,7 +141,7 @@ __device__ __forceinline__ void quantise_head(const AppendParams &p, int head, i
         const int t = 2 * i + sub;
         const int r = first_row + t;
         if (t >= n || r < 0 || r >= p.b.total_new) continue;
-        uint2 w = make_uint2(0x7F7F7F7Fu, 0x7F7F7F7Fu);
+        uint2 w = make_uint2(0u, 0u);
         if (!poisoned)
             w = make_uint2(e4m3x4(x[i][0] * inv, x[i][1] * inv, x[i][2] * inv, x[i][3] * inv),
                            e4m3x4(x[i][4] * inv, x[i][5] * inv, x[i][6] * inv, x[i][7] * inv));
@@ -146,8 +149,9 @@ __device__ __forceinline__ void quantise_head(const AppendParams &p, int head, i
     }
 }
 
-__global__ void __launch_bounds__(THREADS, 3) kv8_append_kernel(const __grid_constant__ AppendParams p) {
+__global__ void __launch_bounds__(THREADS, 2) kv8_append_kernel(const __grid_constant__ AppendParams p) {
     __shared__ double2 angles[kKv8Group * HALF];                 // cos, sin
+    __shared__ float2 angles_q[kKv8Group * HALF];                // the same, rounded
     pdl_launch_dependents();
     pdl_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -170,7 +174,9 @@ __global__ void __launch_bounds__(THREADS, 3) kv8_append_kernel(const __grid_con
         const double turn = (double)(pos + i / HALF) * p.turns[i % HALF];
         double s, c;
         sincospi(2.0 * (turn - rint(turn)), &s, &c);
-        angles[i] = make_double2(c, s);
+        const int at = angle_at(i / HALF, i % HALF);
+        angles[at] = make_double2(c, s);
+        angles_q[at] = make_float2((float)c, (float)s);
     }
     __syncthreads();
 
@@ -183,28 +189,42 @@ __global__ void __launch_bounds__(THREADS, 3) kv8_append_kernel(const __grid_con
         else quantise_head<true>(p, head, first_row, first, n, first, row, angles);
     }
     if (p.query == nullptr) return;
-    // queries: half a warp per row of 128, as the keys, but nothing is decided by comparison: 32-bit arithmetic on rounded angles
-    const int c = lane & 15;
-    for (int r = warp * 2 + (lane >> 4); r < ((n * p.b.q_heads + 1) & ~1); r += THREADS / 16) {
-        const int t = r / p.b.q_heads, head = r - t * p.b.q_heads;
-        const int at = first_row + t;
-        const bool there = t < n && at >= 0 && at < p.b.total_new;
-        uint4 w = make_uint4(0u, 0u, 0u, 0u);
-        if (there) w = *reinterpret_cast<const uint4 *>(p.query + (long long)at * p.ldq + (size_t)head * kKv8Dim + c * 8);
-        uint32_t own[4] = {w.x, w.y, w.z, w.w};
-        const float sign = c < 8 ? -1.0f : 1.0f;
-        const double2 *a = angles + min(t, n - 1) * HALF + (c & 7) * 8;
+    // Queries: half a warp per token with its angles in registers, several tokens' share of the heads each where the block has few
+    // tokens.  Nothing is decided by comparison here: 32-bit arithmetic on rounded angles.
+    const int c = lane & 15, half_warp = warp * 2 + (lane >> 4);
+    const int t = half_warp % n, at = first_row + t;
+    const int shares = THREADS / 16 / n, share = half_warp / n;
+    const bool there = share < shares && at >= 0 && at < p.b.total_new;
+    float2 cs[8];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const uint32_t other = __shfl_xor_sync(0xFFFFFFFFu, own[j], 8);
-            const double2 a0 = a[2 * j], a1 = a[2 * j + 1];
-            const float y0 = fmaf(bf16_lo(own[j]), (float)a0.x, sign * (float)a0.y * bf16_lo(other));
-            const float y1 = fmaf(bf16_hi(own[j]), (float)a1.x, sign * (float)a1.y * bf16_hi(other));
-            const __nv_bfloat162 y = __floats2bfloat162_rn(y0, y1);
-            own[j] = *reinterpret_cast<const uint32_t *>(&y);
+    for (int j = 0; j < 8; ++j) cs[j] = angles_q[t * HALF + j * 8 + (c & 7)];
+    if (c < 8)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) cs[j].y = -cs[j].y;
+    const int step = max(1, shares);
+    for (int head0 = 0; head0 < p.b.q_heads; head0 += 4 * step) {
+        uint4 w[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int head = head0 + u * step + share;
+            w[u] = make_uint4(0u, 0u, 0u, 0u);
+            if (there && head < p.b.q_heads) w[u] = *reinterpret_cast<const uint4 *>(p.query + (long long)at * p.ldq + (size_t)head * kKv8Dim + c * 8);
         }
-        if (there)
-            *reinterpret_cast<uint4 *>(p.query_out + (long long)at * p.ldqo + (size_t)head * kKv8Dim + c * 8) = make_uint4(own[0], own[1], own[2], own[3]);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int head = head0 + u * step + share;
+            uint32_t own[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t other = __shfl_xor_sync(0xFFFFFFFFu, own[j], 8);
+                const float y0 = fmaf(bf16_lo(own[j]), cs[2 * j].x, cs[2 * j].y * bf16_lo(other));
+                const float y1 = fmaf(bf16_hi(own[j]), cs[2 * j + 1].x, cs[2 * j + 1].y * bf16_hi(other));
+                const __nv_bfloat162 y = __floats2bfloat162_rn(y0, y1);
+                own[j] = *reinterpret_cast<const uint32_t *>(&y);
+            }
+            if (there && head < p.b.q_heads)
+                *reinterpret_cast<uint4 *>(p.query_out + (long long)at * p.ldqo + (size_t)head * kKv8Dim + c * 8) = make_uint4(own[0], own[1], own[2], own[3]);
+        }
     }
 }
 

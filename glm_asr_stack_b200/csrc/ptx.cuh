@@ -164,6 +164,15 @@ __device__ __forceinline__ void umma_bf16(uint32_t d_tmem, uint64_t adesc, uint6
         ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
+// e4m3 x e4m3, fp32 accumulate, K = 32 (kind::f8f6f4; the formats are in the instruction descriptor).
+__device__ __forceinline__ void umma_f8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
 // Same with A in tensor memory: lane = row, bf16 pairs of consecutive k per 32-bit column (eight columns for K = 16).
 __device__ __forceinline__ void umma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
@@ -210,6 +219,17 @@ __device__ __forceinline__ void tmem_ld_x16(uint32_t taddr, uint32_t (&r)[16]) {
           "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(taddr)
         : "memory");
+}
+__device__ __forceinline__ void tmem_ld_x8(uint32_t taddr, uint32_t (&r)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(taddr)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st_x8(uint32_t taddr, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
 }
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 // Store 32 consecutive 32-bit columns of this thread's TMEM lane.
@@ -341,9 +361,9 @@ __device__ __forceinline__ uint64_t smem_desc_sw128(uint32_t saddr) {
     d |= (uint64_t)2 << 61;                       // layout: SWIZZLE_128B
     return d;
 }
-// MN-major operand (the contiguous dimension is M or N): rows of 64 elements (128 bytes, 128B-swizzled) per k, as a TMA box
-// of 64 elements x k rows leaves them.  Eight k rows are 1024 bytes, the next 64 columns start box_bytes further on; a K
-// step of 16 is 2048 bytes.
+// MN-major operand (the contiguous dimension is M or N): rows of 64 16-bit elements, or 128 8-bit ones (128 bytes, 128B-swizzled), per k,
+// as a TMA box of such rows leaves them.  Eight k rows are 1024 bytes, the next 128 bytes of columns start box_bytes further on;
+// a K step of 16 is 2048 bytes.
 __device__ __forceinline__ uint64_t smem_desc_sw128_mn(uint32_t saddr, uint32_t box_bytes) {
     uint64_t d = 0;
     d |= (uint64_t)((saddr & 0x3FFFF) >> 4);
@@ -371,6 +391,11 @@ __host__ __device__ constexpr uint32_t idesc_bf16(int m, int n) {
            | ((uint32_t)(n >> 3) << 17)   // N / 8
            | ((uint32_t)(m >> 4) << 24);  // M / 16
 }
+// kind::f8f6f4: e4m3 x e4m3 -> fp32 (both format fields are 0).
+__host__ __device__ constexpr uint32_t idesc_e4m3(int m, int n) {
+    return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+constexpr uint32_t kIdescAMnMajor = 1u << 15;   // A is MN-major
 constexpr uint32_t kIdescBMnMajor = 1u << 16;   // B is MN-major (both operands are K-major without it)
 // Instruction descriptor, kind::mxf4nvf4: e2m1 x e2m1, ue4m3 scales, K = 64, K-major.
 __host__ __device__ constexpr uint32_t idesc_nvfp4(int m, int n) {

@@ -401,7 +401,8 @@ int glmasr_profile_read(int max_entries, double *ms, double *flops, double *byte
  * One layer's pool.  codes: e4m3 [num_blocks][kv_heads][block_size][128]; scales: fp32 [num_blocks][kv_heads][block_size / 16],
  * one power of two per 16 tokens of a head, the smallest 2^e (e >= -126) with amax <= 448 * 2^e; value = code * scale.
  * head_dim is 128, block_size a multiple of 16; codes 16-byte aligned.  A block of 16 tokens that got a value which is not
- * finite, or beyond 448 * 2^60, has the scale NaN until its first token is written again, and queries that see it get NaN.
+ * finite, or beyond 448 * 2^60, has the scale NaN (and zero codes) until its first token is written again, and queries that see any
+ * token of it get NaN.
  *
  * A batch (both calls): sequence s has the packed rows [cu_new[s], cu_new[s + 1]) as its new tokens and seq_lens[s] tokens with
  * them; row i of its n is at position seq_lens[s] - n + i, and position p lies in page block_tables[s][p / block_size].  All three
@@ -429,7 +430,7 @@ int glmasr_kv8_append(const glmasr_kv8_cache *cache, const uint16_t *key, long l
  * position p sees the positions j <= p with window == 0, or p - j < window, or j < sinks.  A query that sees nothing gets zeros.
  * out, query: bf16 [total_new, q_heads * 128] with row pitches ldo, ldq (multiples of 8; 16-byte aligned); q_heads a multiple of
  * kv_heads.  scale: of the scores, before the softmax.  max_new (new tokens of a sequence) and max_len (tokens of a sequence)
- * say what to expect: they choose kernels and never change what is computed.  |query| < 2^63.
+ * say what to expect: they choose kernels and never change what is computed.
  * workspace: glmasr_kv8_attention_workspace(num_seqs) bytes of device memory, 16-byte aligned, contents irrelevant, not shared
  * with a call that may run at the same time.  num_seqs <= 4096.  Returns 0, or -1 on bad arguments or a launch failure. */
 long long glmasr_kv8_attention_workspace(int num_seqs);
