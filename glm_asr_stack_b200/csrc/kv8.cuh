@@ -47,6 +47,7 @@ struct Kv8Batch {
     const int *seq_lens;          // [num_seqs]
     const int *cu_new;            // [num_seqs + 1]
     int num_seqs, max_blocks, num_blocks, block_size, kv_heads, q_heads, total_new;
+    int max_tokens;               // that a row of the table has pages for
 };
 
 #ifdef __CUDACC__

@@ -33,6 +33,8 @@ bool make_batch(Kv8Batch &b, const glmasr_kv8_cache *c, const int *block_tables,
     b.kv_heads = c->kv_heads;
     b.q_heads = q_heads;
     b.total_new = total_new;
+    const long long tokens = (long long)max_blocks * c->block_size;
+    b.max_tokens = tokens > 0x7FFFFFF0LL ? 0x7FFFFFF0 : (int)tokens;
     return true;
 }
 
@@ -62,9 +64,7 @@ extern "C" int glmasr_kv8_append(const glmasr_kv8_cache *cache, const uint16_t *
     return 0;
 }
 
-extern "C" long long glmasr_kv8_attention_workspace(int num_seqs) {
-    return num_seqs < 0 ? -1 : (long long)kv8_attention_workspace_bytes(num_seqs);
-}
+extern "C" long long glmasr_kv8_attention_workspace(void) { return (long long)kv8_attention_workspace_bytes(); }
 
 extern "C" int glmasr_kv8_attention(uint16_t *out, long long ldo, const uint16_t *query, long long ldq, const glmasr_kv8_cache *cache,
                                     const int *block_tables, int max_blocks, const int *seq_lens, const int *cu_new, int num_seqs,
@@ -75,7 +75,7 @@ extern "C" int glmasr_kv8_attention(uint16_t *out, long long ldo, const uint16_t
     if (q_heads <= 0 || q_heads % a.b.kv_heads != 0 || window < 0 || sinks < 0 || max_new < 0 || max_len < 0 || !isfinite(scale)) return -1;
     if (num_seqs == 0 || total_new == 0) return 0;
     if (!rows_ok(query, ldq, q_heads, total_new) || !rows_ok(out, ldo, q_heads, total_new)) return -1;
-    if (workspace == nullptr || !aligned16(workspace) || workspace_bytes < glmasr_kv8_attention_workspace(num_seqs)) return -1;
+    if (workspace == nullptr || !aligned16(workspace) || workspace_bytes < glmasr_kv8_attention_workspace()) return -1;
     a.k_cache = cache->k, a.v_cache = cache->v;
     a.k_scale = cache->k_scale, a.v_scale = cache->v_scale;
     a.query = (const __nv_bfloat16 *)query;

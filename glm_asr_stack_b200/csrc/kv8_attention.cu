@@ -14,12 +14,15 @@
 //            2^(x_j + log2 v_scale_j - W + 6), at most 2^8, is split as p = hi + 2^-4 lo: off by 6.6e-4 of its size (rms; bf16: 1.6e-3) or 2^-20
 //            of the largest, whichever is more.
 //   lazily   m and W are touched when a term has grown past 2^8 m or 2^2 W: an ordinary tile needs one vote of its four warps.
-//   split    All visible groups of 16 tokens of all (sequence, kv head) pairs form one line, cut into equal pieces, one per CTA:
-//            uneven lengths cost nothing.  A piece that ends inside a context leaves m, W, the sum and the accumulator in the
-//            workspace, and a second launch joins those.
+//   split    Two ways to deal out the work, chosen on the host (see deal_whole()).  Whole: a CTA takes every gridDim-th (sequence, kv head)
+//            and there is nothing to join.  Pieces: all visible groups of 16 tokens of all (sequence, kv head) pairs form one line,
+//            cut into equal pieces, one per CTA, so that uneven lengths cost nothing; a piece that ends inside a context leaves m,
+//            W, the sum and the accumulator in the workspace, and a second launch joins those.
 // A CTA walks its piece context by context in tiles of up to eight groups: warp 4 copies (a TMA box of 2 KB per group, K or V; the
-// groups of a tile may lie anywhere), warp 5 issues the products, warp 6 prepares the queries of the next context, warps 0-3 are the
-// softmax, one thread per token, and write the results.
+// groups of a tile may lie anywhere), prepares the queries of the next context and says where its results go, warp 5 issues the
+// products, warps 0-3 are the softmax, one thread per token, and write the results.
+// K and V have two buffers each.  A tile's chain of waits, products and softmax is about 2000 cycles, and a copy takes as long: three
+// CTAs with 64 KB of tiles each keep HBM busy.  (Four with one buffer of each: every copy waits for a product, 4000 cycles a tile.)
 #include <cuda_fp16.h>
 #include <math.h>
 
@@ -34,7 +37,7 @@ __device__ int g_kv8_status[4];
 namespace {
 
 constexpr int SOFTMAX = 128;                                  // threads; also tokens of a tile and lanes of tensor memory
-constexpr int THREADS = SOFTMAX + 96;
+constexpr int THREADS = SOFTMAX + 64;
 constexpr int TILE_GROUPS = SOFTMAX / kKv8Group;
 constexpr int GROUP_BYTES = kKv8Group * kKv8Dim;
 constexpr int TILE_BYTES = TILE_GROUPS * GROUP_BYTES;         // 16 KB of K, or V
@@ -43,16 +46,28 @@ constexpr float kNothing = -3.4028234664e38f;                 // m and W before 
 constexpr float kTop = 8.0f, kWeightTop = 2.0f, kWeightBase = 6.0f;
 constexpr float kQLo = 1.0f / 32.0f, kPLo = 1.0f / 16.0f;
 
-enum : int { B_KFULL = 0, B_KEMPTY = 2, B_VFULL = 4, B_SFULL = 6, B_PFULL = 8, B_PVDONE = 10, B_QFULL = 12, B_QEMPTY = 14, B_OFREE = 16, B_COUNT = 17 };
+enum : int { B_KFULL = 0, B_KEMPTY = 2, B_VFULL = 4, B_PVDONE = 6, B_SFULL = 8, B_SCALES = 10, B_CFULL = 12, B_CEMPTY = 14, B_PFULL = 16, B_OFREE = 17, B_COUNT = 18 };
 
+// What the products and the softmax have to know of a context.
+template <int R>
+struct ContextInfo {
+    int groups;                           // in this piece; 0: the piece is done
+    int rows;                             // query rows that exist
+    int first, sink, from;                // group i of the piece is group first + i of the context; Kv8Span
+    int pos_lo, pos_hi;                   // positions of its queries
+    int slot;                             // of its parts in the workspace; -1: it is whole
+    float qscale[R];                      // softmax scale * log2(e) / the power of two in the row's queries
+    int pos[R];
+    __nv_bfloat16 *out[R];
+};
 // Shared memory; R = query rows of a context.
 template <int R>
 struct Smem {
     uint8_t k[2][TILE_BYTES], v[2][TILE_BYTES];
     uint8_t q[2][2 * R * kKv8Dim];        // B operand of S^T: rows hi, then lo
-    uint8_t p[2][2 * R * SOFTMAX];        // B operand of O^T: rows hi, then lo
-    float qscale[2][R];                   // softmax scale * log2(e) / the power of two in the row's queries
-    float top[R], wtop[R];
+    uint8_t p[2 * R * SOFTMAX];           // B operand of O^T: per 16 columns (rows hi, then lo) 16 bytes of each token
+    ContextInfo<R> ctx[2];
+    float4 row[R];                        // m + kTop, W + kWeightTop, -m, kWeightBase - W
     float red[4][R][2], factor[R][2];
     float2 scales[2][TILE_GROUPS];        // K, V
     int tokens[2][TILE_GROUPS];           // of each group that exist
@@ -132,7 +147,6 @@ struct Context {
     int seq, head, row_tile;
     int unit0, unit1;                 // its units on the line
     int from, to;                     // its groups in this piece, of w.span.count
-    __device__ __forceinline__ int tiles() const { return (to - from + TILE_GROUPS - 1) / TILE_GROUPS; }
 };
 __device__ __forceinline__ Context context_at(const Kv8Attend &a, const int *prefix, int rows, int seq, int at, int end) {
     Context c;
@@ -149,12 +163,19 @@ __device__ __forceinline__ Context context_at(const Kv8Attend &a, const int *pre
     return c;
 }
 
+// A context that begins in a piece and ends in a later one.
+struct JoinInfo {
+    int last;                     // the piece it ends in; -1: there is none
+    int slot;                     // of its first part; those of the others are 2 * piece
+    int rows, row0, head;         // its query rows: row0 + r counts (new token, head of the group) of the sequence
+    int first_token;              // packed row of the sequence's first new token
+};
 struct Partial {                  // workspace layout
     float4 *stats;                // [2 * CTAs][rows]: m, sum, W, -
     float *acc;                   // [2 * CTAs][rows][128]
-    int *prefix;                  // [num_seqs + 2]: units before each sequence, units in all, units per CTA
+    JoinInfo *join;               // [CTAs]: the context that begins in the CTA's piece and ends in another
 };
-inline size_t partial_bytes(int ctas, int rows, int num_seqs, void *base, Partial *out) {
+inline size_t partial_bytes(int ctas, int rows, void *base, Partial *out) {
     size_t off = 0;
     auto take = [&](size_t bytes) {
         const size_t at = off;
@@ -163,8 +184,8 @@ inline size_t partial_bytes(int ctas, int rows, int num_seqs, void *base, Partia
     };
     char *stats = take((size_t)2 * ctas * rows * sizeof(float4));
     char *acc = take((size_t)2 * ctas * rows * kKv8Dim * sizeof(float));
-    char *prefix = take((size_t)(num_seqs + 2) * sizeof(int));
-    if (out != nullptr) out->stats = (float4 *)stats, out->acc = (float *)acc, out->prefix = (int *)prefix;
+    char *join = take((size_t)ctas * sizeof(JoinInfo));
+    if (out != nullptr) out->stats = (float4 *)stats, out->acc = (float *)acc, out->join = (JoinInfo *)join;
     return off;
 }
 
@@ -172,11 +193,17 @@ struct Params {
     CUtensorMap tm_k, tm_v;       // [groups * 16 rows][128 bytes], boxes of 16 rows
     Kv8Attend a;
     Partial part;
-    int min_units;
+    int whole;                    // how the work is dealt out
+    int min_units;                // of a piece
 };
 
-template <int R>
-__global__ void __launch_bounds__(THREADS, R == 8 ? 3 : 2) kv8_attend_kernel(const __grid_constant__ Params p) {
+// CTAs on an SM: what registers, tensor memory and the tiles allow
+constexpr int max_ctas(int rows) { return rows <= 8 ? 3 : 2; }
+
+// R = query rows of a context as the products have them, U <= R how many the softmax works on (a group of four heads fills half
+// of the narrowest product).
+template <int R, int U>
+__global__ void __launch_bounds__(THREADS, max_ctas(R)) kv8_attend_kernel(const __grid_constant__ Params p) {
     constexpr int N = 2 * R;                                  // columns of both products
     constexpr int TMEM_COLS = 3 * N <= 64 ? 64 : 3 * N <= 128 ? 128 : 256;     // two score buffers, the accumulator
     extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -190,17 +217,18 @@ __global__ void __launch_bounds__(THREADS, R == 8 ? 3 : 2) kv8_attend_kernel(con
         return;
     }
     if (threadIdx.x == 0) {
+        mbar_init(bar(B_PFULL), SOFTMAX);
+        mbar_init(bar(B_OFREE), SOFTMAX);
         for (int i = 0; i < 2; ++i) {
             mbar_init(bar(B_KFULL + i), 1);
             mbar_init(bar(B_KEMPTY + i), 1);
             mbar_init(bar(B_VFULL + i), 1);
-            mbar_init(bar(B_SFULL + i), 1);
-            mbar_init(bar(B_PFULL + i), SOFTMAX);
             mbar_init(bar(B_PVDONE + i), 1);
-            mbar_init(bar(B_QFULL + i), 1);
-            mbar_init(bar(B_QEMPTY + i), 1 + SOFTMAX);        // the last product and the last look at the scales
+            mbar_init(bar(B_SFULL + i), 1);
+            mbar_init(bar(B_SCALES + i), 1);
+            mbar_init(bar(B_CFULL + i), 1);
+            mbar_init(bar(B_CEMPTY + i), 1 + SOFTMAX);        // the last product of scores and the results
         }
-        mbar_init(bar(B_OFREE), SOFTMAX);
         sm.abort = 0;
         fence_mbar_init();
         tma_prefetch_desc(&p.tm_k);
@@ -213,58 +241,54 @@ __global__ void __launch_bounds__(THREADS, R == 8 ? 3 : 2) kv8_attend_kernel(con
     pdl_wait();
     pdl_launch_dependents();          // after the wait: the join may look at the batch before its own
 
-    // ---- units before each sequence: two sequences of a thread at a time, their loads together ----
-    constexpr int EACH = 2;
-    int carry = 0;
-    for (int s0 = 0; s0 < a.b.num_seqs; s0 += THREADS * EACH) {
-        const int s = s0 + (int)threadIdx.x * EACH;
-        int mine[EACH], sum = 0;
-#pragma unroll
-        for (int e = 0; e < EACH; ++e) {
-            mine[e] = 0;
-            if (s + e < a.b.num_seqs) {
-                const SeqWork w = seq_work(a, s + e, R);
-                mine[e] = w.units * w.tiles * a.b.kv_heads;
-            }
-            sum += mine[e];
-        }
-        const int own_sum = sum;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const int up = __shfl_up_sync(0xFFFFFFFFu, sum, d);
-            if (lane >= d) sum += up;
-        }
-        if (lane == 31) sm.warp_sum[warp] = sum;
-        __syncthreads();
-        int before = carry + sum - own_sum;
-#pragma unroll
-        for (int w = 0; w < THREADS / 32; ++w) {
-            if (w < warp) before += sm.warp_sum[w];
-            carry += sm.warp_sum[w];
-        }
-#pragma unroll
-        for (int e = 0; e < EACH; ++e)
-            if (s + e < a.b.num_seqs) {
-                sm.prefix[s + e] = before;
-                before += mine[e];
-            }
-        __syncthreads();
+    // rows of the queries' operand that no row of a context fills stay zero
+    if (U < R && threadIdx.x < 4 * (R - U) * 8) {
+        const int row = (int)threadIdx.x / 8 % (R - U) + U + (threadIdx.x / 8 / (R - U) & 1 ? R : 0);
+        *reinterpret_cast<uint4 *>(sm.q[threadIdx.x / 8 / (R - U) / 2] + row * kKv8Dim + threadIdx.x % 8 * 16) = make_uint4(0u, 0u, 0u, 0u);
+        fence_proxy_async_smem();
     }
-    const int total = carry;
-    const int quota = max(p.min_units, (total + (int)gridDim.x - 1) / (int)gridDim.x);
-    if (blockIdx.x == 0) {
-        for (int s = threadIdx.x; s < a.b.num_seqs; s += THREADS) p.part.prefix[s] = sm.prefix[s];
-        if (threadIdx.x == 0) p.part.prefix[a.b.num_seqs] = total, p.part.prefix[a.b.num_seqs + 1] = quota;
-    }
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(&sm.tmem);
-    const long long begin_l = (long long)blockIdx.x * quota;
-    const int begin = (int)min(begin_l, (long long)total), end = (int)min((long long)total, begin_l + quota);
-    volatile int *abort_word = &sm.abort;
-    int seq0 = 0;                     // the sequence of the first unit
-    {
+    int begin = 0, end = 0, quota = 1, seq0 = 0;          // the piece, and the sequence of its first unit
+    if (!p.whole) {
+        // units before each sequence: two sequences of a thread at a time, their loads together
+        constexpr int EACH = 2;
+        int carry = 0;
+        for (int s0 = 0; s0 < a.b.num_seqs; s0 += THREADS * EACH) {
+            const int s = s0 + (int)threadIdx.x * EACH;
+            int mine[EACH], sum = 0;
+#pragma unroll
+            for (int e = 0; e < EACH; ++e) {
+                mine[e] = 0;
+                if (s + e < a.b.num_seqs) {
+                    const SeqWork w = seq_work(a, s + e, U);
+                    mine[e] = w.units * w.tiles * a.b.kv_heads;
+                }
+                sum += mine[e];
+            }
+            const int own_sum = sum;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const int up = __shfl_up_sync(0xFFFFFFFFu, sum, d);
+                if (lane >= d) sum += up;
+            }
+            if (lane == 31) sm.warp_sum[warp] = sum;
+            __syncthreads();
+            int before = carry + sum - own_sum;
+#pragma unroll
+            for (int w = 0; w < THREADS / 32; ++w) {
+                if (w < warp) before += sm.warp_sum[w];
+                carry += sm.warp_sum[w];
+            }
+#pragma unroll
+            for (int e = 0; e < EACH; ++e)
+                if (s + e < a.b.num_seqs) {
+                    sm.prefix[s + e] = before;
+                    before += mine[e];
+                }
+            __syncthreads();
+        }
+        quota = max(p.min_units, (carry + (int)gridDim.x - 1) / (int)gridDim.x);
+        const long long at = (long long)blockIdx.x * quota;
+        begin = (int)min(at, (long long)carry), end = (int)min((long long)carry, at + quota);
         int hi = a.b.num_seqs;
         while (hi - seq0 > 1) {
             const int mid = (seq0 + hi) >> 1;
@@ -272,19 +296,82 @@ __global__ void __launch_bounds__(THREADS, R == 8 ? 3 : 2) kv8_attend_kernel(con
             else hi = mid;
         }
     }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(&sm.tmem);
+    volatile int *abort_word = &sm.abort;
 
     if (warp == 4) {
-        // ================================ copies ================================
+        // ================================ copies, queries =======================
         const bool leader = elect_one();
-        uint32_t t = 0;               // tiles started
-        bool ok = true;
-        int seq = seq0;
-        for (int at = begin; ok && at < end;) {
-            const Context c = context_at(a, sm.prefix, R, seq, at, end);
-            seq = c.seq;
-            at = min(end, c.unit1);
-            // groups of a tile by lane; those of the next tile are looked up while this one's copies run
-            auto look_up = [&](int g, int &place, int &tokens, float2 &scale) {
+        uint32_t t = 0, contexts = 0; // tiles and contexts started
+        bool ok = true, have = false, first = false, more = true;
+        int at = begin, first_unit = begin, g = 0, rows = 0, item = (int)blockIdx.x;
+        JoinInfo join = {-1, 0, 0, 0, 0, 0};
+        Context c;
+        c.seq = seq0, c.to = 0, c.row_tile = 0, c.w.tiles = 0;
+        // the next context of the piece, or the next row tile of a whole (sequence, kv head), or the next one that has any
+        auto next_context = [&]() {
+            if (!p.whole) {
+                if (at >= end) return false;
+                c = context_at(a, sm.prefix, U, c.seq, at, end);
+                first_unit = at;
+                at = min(end, c.unit1);
+                if (first_unit == c.unit0 && at < c.unit1)
+                    join = {(c.unit1 - 1) / quota, 2 * (int)blockIdx.x + (c.unit0 > begin ? 1 : 0), 0, c.row_tile * U, c.head, c.w.row0};
+            } else if (++c.row_tile >= c.w.tiles) {
+                do {
+                    if (item >= a.b.num_seqs * a.b.kv_heads) return false;
+                    c.seq = a.b.by_kv_heads.div(item);
+                    c.head = item - c.seq * a.b.kv_heads;
+                    c.w = seq_work(a, c.seq, U);
+                    item += (int)gridDim.x;
+                } while (c.w.tiles == 0);
+                c.row_tile = c.from = 0;
+                c.to = c.w.span.count;
+            }
+            return true;
+        };
+        // of the coming tile, by lane: place in the pool in groups (-1: none) and existing tokens of a group, its scales
+        int place = -1, tokens = 0;
+        float2 scale = make_float2(0.0f, 0.0f);
+        // queries: QL lanes per row, all rows of a small tile or eight at a time; the first are asked for when a context is entered
+        constexpr int QL = U <= 4 ? 8 : 4, QROWS = 32 / QL, QI = 16 / QL;
+        uint4 q[QI];                                          // dims 8 QL i + 8 (lane % QL) .. + 7
+        auto place_of = [&](int r, int &tok) {                // first element of the row's head in a packed row, and the row
+            const int row = c.row_tile * U + r;
+            tok = a.by_group.div(row);
+            return (size_t)(c.head * a.group + row - tok * a.group) * kKv8Dim;
+        };
+        auto ask_queries = [&](int r) {
+            int tok;
+            const size_t col = place_of(r, tok);
+            const __nv_bfloat16 *src = a.query + (long long)(c.w.row0 + tok) * a.ldq + col + (lane % QL) * 8;
+#pragma unroll
+            for (int i = 0; i < QI; ++i) q[i] = r < rows ? *reinterpret_cast<const uint4 *>(src + i * 8 * QL) : make_uint4(0u, 0u, 0u, 0u);
+        };
+        for (;;) {
+            have = false;
+            while (!have && more) {
+                first = g >= c.to;
+                if (first) {
+                    more = next_context();
+                    if (!more) break;
+                    rows = min(U, c.w.n * a.group - c.row_tile * U);
+                    join.rows = rows;
+                    g = c.from;
+                    ask_queries(lane / QL);
+                }
+                if (g == c.to) {                              // nothing is visible
+                    for (int r = 0; r < rows; ++r) {
+                        int tok;
+                        const size_t col = place_of(r, tok);
+                        *reinterpret_cast<uint2 *>(a.out + (long long)(c.w.row0 + tok) * a.ldo + col + lane * 4) = make_uint2(0u, 0u);
+                    }
+                    continue;
+                }
+                have = true;
                 place = -1, tokens = 0;
                 scale = make_float2(0.0f, 0.0f);
                 if (lane < TILE_GROUPS && g + lane < c.to) {
@@ -296,65 +383,127 @@ __global__ void __launch_bounds__(THREADS, R == 8 ? 3 : 2) kv8_attend_kernel(con
                         scale = make_float2(a.k_scale[place], a.v_scale[place]);
                     }
                 }
-            };
-            int place, tokens;
-            float2 scale;
-            look_up(c.from, place, tokens, scale);
-            for (int g = c.from; g < c.to; g += TILE_GROUPS, ++t) {
-                const int s = (int)(t & 1u);
-                const uint32_t free_phase = ((t >> 1) & 1u) ^ 1u;
-                const uint32_t there = __ballot_sync(0xFFFFFFFFu, place >= 0);
-                const uint32_t bytes = (uint32_t)__popc(there) * GROUP_BYTES;
-                if (!mbar_wait_warp(bar(B_KEMPTY + s), free_phase, abort_word, ST_TIMEOUT_ATTENTION)) { ok = false; break; }
-                if (leader) mbar_expect_tx(bar(B_KFULL + s), bytes);
-                __syncwarp();
-                if (place >= 0) tma_load_2d(smem_u32(sm.k[s]) + lane * GROUP_BYTES, &p.tm_k, bar(B_KFULL + s), 0, place * kKv8Group);
-                if (!mbar_wait_warp(bar(B_PVDONE + s), free_phase, abort_word, ST_TIMEOUT_ATTENTION)) { ok = false; break; }
+                g += TILE_GROUPS;
+            }
+            if (!have) break;
+            const int s = (int)(t & 1u);
+            const uint32_t free_phase = ((t >> 1) & 1u) ^ 1u, bytes = (uint32_t)__popc(__ballot_sync(0xFFFFFFFFu, place >= 0)) * GROUP_BYTES;
+            ++t;
+            ok = mbar_wait_warp(bar(B_KEMPTY + s), free_phase, abort_word, ST_TIMEOUT_ATTENTION);
+            if (!ok) break;
+            if (leader) mbar_expect_tx(bar(B_KFULL + s), bytes);
+            __syncwarp();
+            if (place >= 0) tma_load_2d(smem_u32(sm.k[s]) + lane * GROUP_BYTES, &p.tm_k, bar(B_KFULL + s), 0, place * kKv8Group);
+            ok = mbar_wait_warp(bar(B_PVDONE + s), free_phase, abort_word, ST_TIMEOUT_ATTENTION);
+            if (!ok) break;
+            if (leader) mbar_expect_tx(bar(B_VFULL + s), bytes);
+            __syncwarp();
+            if (place >= 0) tma_load_2d(smem_u32(sm.v[s]) + lane * GROUP_BYTES, &p.tm_v, bar(B_VFULL + s), 0, place * kKv8Group);
+            // the softmax is done with the scales of two tiles ago: that tile has been summed
+            auto put_scales = [&]() {
                 if (lane < TILE_GROUPS) {
                     sm.scales[s][lane] = scale;
                     sm.tokens[s][lane] = tokens;
                 }
                 __syncwarp();
-                if (leader) mbar_expect_tx(bar(B_VFULL + s), bytes);
-                __syncwarp();
-                if (place >= 0) tma_load_2d(smem_u32(sm.v[s]) + lane * GROUP_BYTES, &p.tm_v, bar(B_VFULL + s), 0, place * kKv8Group);
-                look_up(g + TILE_GROUPS, place, tokens, scale);
+                if (leader) mbar_arrive(bar(B_SCALES + s));
+            };
+            if (!first) {
+                put_scales();
+                continue;
             }
+            const int cs = (int)(contexts & 1u);
+            ok = mbar_wait_warp(bar(B_CEMPTY + cs), ((contexts >> 1) & 1u) ^ 1u, abort_word, ST_TIMEOUT_ATTENTION);
+            if (!ok) break;
+            ++contexts;
+            ContextInfo<R> &info = sm.ctx[cs];
+            if (lane == 0) {
+                info.groups = c.to - c.from;
+                info.rows = rows;
+                info.first = c.from, info.sink = c.w.span.sink, info.from = c.w.span.from;
+                info.pos_lo = c.w.start + a.by_group.div(c.row_tile * U);
+                info.pos_hi = c.w.start + a.by_group.div(c.row_tile * U + rows - 1);
+                info.slot = p.whole || (first_unit == c.unit0 && at == c.unit1) ? -1 : 2 * (int)blockIdx.x + (c.unit0 > begin ? 1 : 0);
+            }
+#pragma unroll 1
+            for (int r = lane / QL; r < U; r += QROWS) {
+                if (r >= QROWS) ask_queries(r);
+                uint32_t most = 0u;
+#pragma unroll
+                for (int i = 0; i < QI; ++i) {
+                    const uint32_t high = __vmaxu2(__vmaxu2(q[i].x & 0x7FFF7FFFu, q[i].y & 0x7FFF7FFFu), __vmaxu2(q[i].z & 0x7FFF7FFFu, q[i].w & 0x7FFF7FFFu));
+                    most = __vmaxu2(most, high);
+                }
+#pragma unroll
+                for (int d = 1; d < QL; d <<= 1) most = __vmaxu2(most, __shfl_xor_sync(0xFFFFFFFFu, most, d));
+                most = max(most >> 16, most & 0xFFFFu);
+                // 2^shift brings the largest element to [2^7, 2^8) (one below 2^-119 less far); a row that is not finite gets NaN
+                // scores by its scale
+                const int expo = (int)(most >> 7);
+                const int shift = expo == 255 ? 0 : min(7 + 127 - expo, 126);
+                const float up = pow2(shift);
+#pragma unroll
+                for (int i = 0; i < QI; ++i) {
+                    const uint32_t w[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
+                    uint32_t hi[2] = {0u, 0u}, lo[2] = {0u, 0u};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float x0 = __uint_as_float(w[e] << 16) * up, x1 = __uint_as_float(w[e] & 0xFFFF0000u) * up;
+                        hi[e >> 1] |= e4m3_split(x0, x1) << (16 * (e & 1));
+                        lo[e >> 1] |= e4m3x2(x0 / kQLo, x1 / kQLo) << (16 * (e & 1));
+                    }
+                    const int b = i * 8 * QL + (lane % QL) * 8;
+                    *reinterpret_cast<uint2 *>(sm.q[cs] + swizzled(r, b)) = make_uint2(hi[0], hi[1]);
+                    *reinterpret_cast<uint2 *>(sm.q[cs] + swizzled(R + r, b)) = make_uint2(lo[0], lo[1]);
+                }
+                if (lane % QL == 0) {
+                    int tok;
+                    const size_t col = place_of(r, tok);
+                    info.qscale[r] = expo == 255 ? __int_as_float(0x7FFFFFFF) : a.scale_log2 * pow2(-shift);
+                    info.pos[r] = r < rows ? c.w.start + tok : -1;
+                    info.out[r] = a.out + (long long)(c.w.row0 + tok) * a.ldo + col;
+                }
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (leader) mbar_arrive(bar(B_CFULL + cs));
+            put_scales();
+        }
+        if (leader && !p.whole) p.part.join[blockIdx.x] = join;
+        const int cs = (int)(contexts & 1u);
+        if (ok && mbar_wait_warp(bar(B_CEMPTY + cs), ((contexts >> 1) & 1u) ^ 1u, abort_word, ST_TIMEOUT_ATTENTION) && leader) {
+            sm.ctx[cs].groups = 0;                            // the end
+            mbar_arrive(bar(B_CFULL + cs));
         }
     } else if (warp == 5) {
         // ================================ products ==============================
         const bool leader = elect_one();
         constexpr uint32_t idesc_s = idesc_e4m3(128, N);
-        constexpr uint32_t idesc_o = idesc_e4m3(128, N) | kIdescAMnMajor;
+        constexpr uint32_t idesc_o = idesc_e4m3(128, N) | kIdescAMnMajor | kIdescBMnMajor;
         const uint32_t t_o = tmem + 2 * N;
         uint32_t t = 0, contexts = 0;
         bool ok = true;
-        int seq = seq0;
         // O^T of tile u: `steps` of 32 tokens; the first tile of a context overwrites the accumulator once the last result has been read
         auto weigh = [&](uint32_t u, int steps, bool first) {
             const int s = (int)(u & 1u);
-            const uint32_t ph = (u >> 1) & 1u;
-            if (!mbar_wait_warp(bar(B_VFULL + s), ph, abort_word, ST_TIMEOUT_ATTENTION)) return false;
-            if (!mbar_wait_warp(bar(B_PFULL + s), ph, abort_word, ST_TIMEOUT_ATTENTION)) return false;
+            if (!mbar_wait_warp(bar(B_VFULL + s), (u >> 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION)) return false;
+            if (!mbar_wait_warp(bar(B_PFULL), u & 1u, abort_word, ST_TIMEOUT_ATTENTION)) return false;
             if (first && !mbar_wait_warp(bar(B_OFREE), ((contexts - 1) & 1u) ^ 1u, abort_word, ST_TIMEOUT_ATTENTION)) return false;
             tc_fence_after();
             if (leader) {
-                const uint64_t ad = smem_desc_sw128_mn(smem_u32(sm.v[s]), TILE_BYTES), bd = smem_desc_sw128(smem_u32(sm.p[s]));
+                const uint64_t ad = smem_desc_sw128_mn(smem_u32(sm.v[s]), TILE_BYTES), bd = smem_desc_mn(smem_u32(sm.p), 16 * SOFTMAX);
                 for (int k = 0; k < steps; ++k)
-                    umma_f8(t_o, ad + (uint64_t)((k * 4096) >> 4), bd + (uint64_t)((k * 32) >> 4), idesc_o, !first || k > 0 ? 1u : 0u);
+                    umma_f8(t_o, ad + (uint64_t)((k * 4096) >> 4), bd + (uint64_t)((k * 512) >> 4), idesc_o, !first || k > 0 ? 1u : 0u);
                 umma_commit(bar(B_PVDONE + s));
             }
             __syncwarp();
             return true;
         };
-        for (int at = begin; ok && at < end;) {
-            const Context c = context_at(a, sm.prefix, R, seq, at, end);
-            seq = c.seq;
-            at = min(end, c.unit1);
-            const int n = c.tiles();
-            if (n == 0) continue;
-            const int qs = (int)(contexts & 1u);
-            if (!mbar_wait_warp(bar(B_QFULL + qs), (contexts >> 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION)) break;
+        while (ok) {
+            const int cs = (int)(contexts & 1u);
+            if (!mbar_wait_warp(bar(B_CFULL + cs), (contexts >> 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION)) break;
+            const int groups_here = sm.ctx[cs].groups, n = (groups_here + TILE_GROUPS - 1) / TILE_GROUPS;
+            if (n == 0) break;
             ++contexts;
             for (int j = 0; j <= n; ++j) {
                 if (j < n) {
@@ -363,233 +512,194 @@ __global__ void __launch_bounds__(THREADS, R == 8 ? 3 : 2) kv8_attend_kernel(con
                     if (!mbar_wait_warp(bar(B_KFULL + s), (t >> 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION)) { ok = false; break; }
                     tc_fence_after();
                     if (leader) {
-                        const uint64_t ad = smem_desc_sw128(smem_u32(sm.k[s])), bd = smem_desc_sw128(smem_u32(sm.q[qs]));
+                        const uint64_t ad = smem_desc_sw128(smem_u32(sm.k[s])), bd = smem_desc_sw128(smem_u32(sm.q[cs]));
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
                             umma_f8(tmem + (uint32_t)s * N, ad + (uint64_t)((k * 32) >> 4), bd + (uint64_t)((k * 32) >> 4), idesc_s, k > 0 ? 1u : 0u);
                         umma_commit(bar(B_KEMPTY + s));
                         umma_commit(bar(B_SFULL + s));
-                        if (j == n - 1) umma_commit(bar(B_QEMPTY + qs));
+                        if (j == n - 1) umma_commit(bar(B_CEMPTY + cs));
                     }
                     __syncwarp();
                     ++t;
                 }
                 if (j >= 1) {
-                    const int groups = min(TILE_GROUPS, c.to - c.from - (j - 1) * TILE_GROUPS);
+                    const int groups = min(TILE_GROUPS, groups_here - (j - 1) * TILE_GROUPS);
                     const uint32_t u = j < n ? t - 2 : t - 1;
                     if (!weigh(u, (groups + 1) / 2, j == 1)) { ok = false; break; }
                 }
             }
-        }
-    } else if (warp == 6) {
-        // ================================ queries ===============================
-        uint32_t contexts = 0;
-        int seq = seq0;
-        for (int at = begin; at < end;) {
-            const Context c = context_at(a, sm.prefix, R, seq, at, end);
-            seq = c.seq;
-            at = min(end, c.unit1);
-            if (c.tiles() == 0) continue;
-            const int qs = (int)(contexts & 1u);
-            if (!mbar_wait_warp(bar(B_QEMPTY + qs), ((contexts >> 1) & 1u) ^ 1u, abort_word, ST_TIMEOUT_ATTENTION)) break;
-            ++contexts;
-#pragma unroll 4
-            for (int r = 0; r < R; ++r) {
-                const int row = c.row_tile * R + r, tok = a.by_group.div(row);
-                uint2 v = make_uint2(0u, 0u);                 // lane: dims 4 lane .. 4 lane + 3
-                if (tok < c.w.n)
-                    v = *reinterpret_cast<const uint2 *>(a.query + (long long)(c.w.row0 + tok) * a.ldq + (size_t)(c.head * a.group + row - tok * a.group) * kKv8Dim + lane * 4);
-                uint32_t most = max(max(v.x & 0x7FFF0000u, (v.x << 16) & 0x7FFF0000u), max(v.y & 0x7FFF0000u, (v.y << 16) & 0x7FFF0000u));
-                most = __reduce_max_sync(0xFFFFFFFFu, most);
-                // 2^shift brings the largest element to [2^7, 2^8); a row that is not finite gets NaN scores by its scale
-                const int expo = max(1, (int)(most >> 23));
-                const int shift = expo == 255 ? 0 : 7 + 127 - expo;
-                const float up0 = pow2(shift / 2), up1 = pow2(shift - shift / 2);
-                float x0 = __uint_as_float(v.x << 16) * up0 * up1, x1 = __uint_as_float(v.x & 0xFFFF0000u) * up0 * up1;
-                float x2 = __uint_as_float(v.y << 16) * up0 * up1, x3 = __uint_as_float(v.y & 0xFFFF0000u) * up0 * up1;
-                const uint32_t hi0 = e4m3_split(x0, x1), hi1 = e4m3_split(x2, x3);
-                *reinterpret_cast<uint32_t *>(sm.q[qs] + swizzled(r, lane * 4)) = hi0 | (hi1 << 16);
-                *reinterpret_cast<uint32_t *>(sm.q[qs] + swizzled(R + r, lane * 4)) =
-                    e4m3x2(x0 / kQLo, x1 / kQLo) | (e4m3x2(x2 / kQLo, x3 / kQLo) << 16);
-                if (lane == 0)
-                    sm.qscale[qs][r] = expo == 255 ? __int_as_float(0x7FFFFFFF) : a.scale_log2 * pow2(-(shift / 2)) * pow2(shift / 2 - shift);
-            }
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar(B_QFULL + qs));
         }
     } else {
         // ================================ softmax ===============================
         const int me = (int)threadIdx.x;                      // token of the tile, lane of tensor memory, dim of the result
         const uint32_t t_lane = tmem + ((uint32_t)(warp * 32) << 16);
         const uint32_t t_o = t_lane + 2 * N;
-        uint32_t t = 0, contexts = 0;
-        bool ok = true;
-        int seq = seq0;
-        for (int at = begin; at < end;) {
-            const Context c = context_at(a, sm.prefix, R, seq, at, end);
-            seq = c.seq;
-            const int first_unit = at;
-            at = min(end, c.unit1);
-            const int n = c.tiles(), qs = (int)(contexts & 1u);
-            const int pos_lo = c.w.start + a.by_group.div(c.row_tile * R);
-            const int pos_hi = c.w.start + min(c.w.n - 1, a.by_group.div(c.row_tile * R + R - 1));
-            float sum[R];
+        uint32_t t = 0;
+        for (uint32_t contexts = 0;; ++contexts) {
+            const int cs = (int)(contexts & 1u);
+            bool ok = mbar_wait_warp(bar(B_CFULL + cs), (contexts >> 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION);
+            const ContextInfo<R> &c = sm.ctx[cs];
+            const int n = (c.groups + TILE_GROUPS - 1) / TILE_GROUPS;
+            const int pos_lo = c.pos_lo, pos_hi = c.pos_hi;
+            float sum[U];
 #pragma unroll
-            for (int r = 0; r < R; ++r) sum[r] = 0.0f;
-            if (me < R) sm.top[me] = sm.wtop[me] = kNothing;
-            if (n > 0) {
-                ok = mbar_wait_warp(bar(B_QFULL + qs), (contexts >> 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION);
-                ++contexts;
-            }
-            if (any_of_softmax(!ok)) { ok = false; break; }
+            for (int r = 0; r < U; ++r) sum[r] = 0.0f;
+            if (me < U) sm.row[me] = make_float4(kNothing, kNothing, -kNothing, -kNothing);
+            if (any_of_softmax(!ok) || n == 0) break;
             for (int j = 0; j < n; ++j, ++t) {
                 const int s = (int)(t & 1u);
-                const uint32_t ph = (t >> 1) & 1u;
-                ok = mbar_wait_warp(bar(B_VFULL + s), ph, abort_word, ST_TIMEOUT_ATTENTION);
-                ok = ok && mbar_wait_warp(bar(B_SFULL + s), ph, abort_word, ST_TIMEOUT_ATTENTION);
-                // the weights of two tiles ago have been read
-                ok = ok && mbar_wait_warp(bar(B_PVDONE + s), ph ^ 1u, abort_word, ST_TIMEOUT_ATTENTION);
-                tc_fence_after();
-                const int g = c.from + j * TILE_GROUPS + me / kKv8Group;
+                ok = mbar_wait_warp(bar(B_SCALES + s), (t >> 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION);
+                const int in = c.first + j * TILE_GROUPS + me / kKv8Group;
+                const int tok = (in < c.sink ? in : c.from + (in - c.sink)) * kKv8Group + me % kKv8Group;
                 const bool there = me % kKv8Group < sm.tokens[s][me / kKv8Group];
-                const int tok = c.w.span.group_of(g) * kKv8Group + me % kKv8Group;
                 const float2 sc = sm.scales[s][me / kKv8Group];
                 const float vs = lg2(sc.y);
                 const bool all = there && tok <= pos_lo && (a.window == 0 || pos_hi - tok < a.window || tok < a.sinks);
-                float x[R];
+                ok = ok && mbar_wait_warp(bar(B_SFULL + s), (t >> 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION);
+                tc_fence_after();
+                float x[U];
+                uint32_t raw[N];
 #pragma unroll
-                for (int r0 = 0; r0 < R; r0 += 8) {
-                    uint32_t hi[8], lo[8];
-                    tmem_ld_x8(t_lane + (uint32_t)(s * N + r0), hi);
-                    tmem_ld_x8(t_lane + (uint32_t)(s * N + R + r0), lo);
-                    tmem_ld_wait();
+                for (int i = 0; i < N; i += 16) tmem_ld_x16(t_lane + (uint32_t)(s * N + i), *reinterpret_cast<uint32_t(*)[16]>(&raw[i]));
+                tmem_ld_wait();
 #pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        x[r0 + e] = fmaf(__uint_as_float(lo[e]), kQLo, __uint_as_float(hi[e])) * (sm.qscale[qs][r0 + e] * sc.x);
-                }
+                for (int r = 0; r < U; ++r) x[r] = fmaf(__uint_as_float(raw[R + r]), kQLo, __uint_as_float(raw[r])) * (c.qscale[r] * sc.x);
                 if (!all) {
 #pragma unroll
-                    for (int r = 0; r < R; ++r)
-                        if (!there || !kv8_sees(a, c.w.start + a.by_group.div(c.row_tile * R + r), tok)) x[r] = -INFINITY;
+                    for (int r = 0; r < U; ++r)
+                        if (!there || !kv8_sees(a, c.pos[r], tok)) x[r] = -INFINITY;
                 }
                 bool grown = !ok;
 #pragma unroll
-                for (int r = 0; r < R; ++r) grown = grown || x[r] > fminf(sm.top[r] + kTop, sm.wtop[r] + kWeightTop - vs);
+                for (int r = 0; r < U; ++r) {
+                    const float2 top = *reinterpret_cast<const float2 *>(&sm.row[r].x);
+                    grown = grown || x[r] > fminf(top.x, top.y - vs);
+                }
                 if (any_of_softmax(grown)) {
-                    // the maxima over the tile's tokens: order-preserving integers within a warp, shared memory between the warps
 #pragma unroll
-                    for (int r = 0; r < R; ++r) {
-                        const int m = __float_as_int(fmaxf(x[r], kNothing)), w = __float_as_int(fmaxf(x[r] + vs, kNothing));
-                        const int mm = __reduce_max_sync(0xFFFFFFFFu, m ^ ((m >> 31) & 0x7FFFFFFF)), ww = __reduce_max_sync(0xFFFFFFFFu, w ^ ((w >> 31) & 0x7FFFFFFF));
-                        if (lane == 0) {
-                            sm.red[warp][r][0] = __int_as_float(mm ^ ((mm >> 31) & 0x7FFFFFFF));
-                            sm.red[warp][r][1] = __int_as_float(ww ^ ((ww >> 31) & 0x7FFFFFFF));
-                        }
+                    for (int r = 0; r < U; ++r) {
+                        const float m = redux_max(fmaxf(x[r], kNothing)), w = redux_max(fmaxf(x[r] + vs, kNothing));
+                        if (lane == 0) *reinterpret_cast<float2 *>(sm.red[warp][r]) = make_float2(m, w);
                     }
                     // the accumulator is expressed against the new W: the product before has to be complete
-                    if (j > 0) ok = ok && mbar_wait_warp(bar(B_PVDONE + (s ^ 1)), ((t - 1) >> 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION);
+                    if (j > 0) ok = ok && mbar_wait_warp(bar(B_PVDONE + (int)((t - 1) & 1u)), ((t - 1) >> 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION);
                     if (any_of_softmax(!ok)) { ok = false; break; }
-                    if (me < R) {
-                        const float m = fmaxf(fmaxf(fmaxf(sm.red[0][me][0], sm.red[1][me][0]), fmaxf(sm.red[2][me][0], sm.red[3][me][0])), sm.top[me]);
-                        const float w = fmaxf(fmaxf(fmaxf(sm.red[0][me][1], sm.red[1][me][1]), fmaxf(sm.red[2][me][1], sm.red[3][me][1])), sm.wtop[me]);
-                        sm.factor[me][0] = ex2(sm.top[me] - m);
-                        sm.factor[me][1] = ex2(sm.wtop[me] - w);
-                        sm.top[me] = m;
-                        sm.wtop[me] = w;
+                    if (me < U) {
+                        const float4 was = sm.row[me];
+                        const float m = fmaxf(fmaxf(fmaxf(sm.red[0][me][0], sm.red[1][me][0]), fmaxf(sm.red[2][me][0], sm.red[3][me][0])), -was.z);
+                        const float w = fmaxf(fmaxf(fmaxf(sm.red[0][me][1], sm.red[1][me][1]), fmaxf(sm.red[2][me][1], sm.red[3][me][1])), kWeightBase - was.w);
+                        sm.factor[me][0] = ex2(-was.z - m);
+                        sm.factor[me][1] = ex2(kWeightBase - was.w - w);
+                        sm.row[me] = make_float4(m + kTop, w + kWeightTop, -m, kWeightBase - w);
                     }
-                    if (any_of_softmax(false)) {}
-#pragma unroll
-                    for (int r = 0; r < R; ++r) sum[r] *= sm.factor[r][0];
+                    (void)any_of_softmax(false);
                     if (j > 0) {
+#pragma unroll
+                        for (int r = 0; r < U; ++r) sum[r] *= sm.factor[r][0];
                         tc_fence_after();
 #pragma unroll
-                        for (int r0 = 0; r0 < N; r0 += 8) {
-                            uint32_t o[8];
-                            tmem_ld_x8(t_o + (uint32_t)r0, o);
+                        for (int r0 = 0; r0 < N; r0 += 16) {
+                            uint32_t o[16];
+                            tmem_ld_x16(t_o + (uint32_t)r0, o);
                             tmem_ld_wait();
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * sm.factor[(r0 + e) % R][1]);
-                            tmem_st_x8(t_o + (uint32_t)r0, o);
+                            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * sm.factor[(r0 + e) % R % U][1]);
+                            tmem_st_x16(t_o + (uint32_t)r0, o);
                         }
                         tmem_st_wait();
                     }
                 }
-                const uint32_t pb = smem_u32(sm.p[s]);
+                uint32_t w8[N / 4] = {};                      // the token's weights: R codes hi, R codes lo
 #pragma unroll
-                for (int r = 0; r < R; r += 2) {
+                for (int r = 0; r < U; r += 2) {
                     float w[2];
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        sum[r + e] += ex2(x[r + e] - sm.top[r + e]);
+                        const float2 ref = *reinterpret_cast<const float2 *>(&sm.row[r + e].z);
+                        sum[r + e] += ex2(x[r + e] + ref.x);
                         // a token that is not seen weighs 0 whatever its block's scale is
-                        w[e] = !all && x[r + e] == -INFINITY ? 0.0f : ex2(x[r + e] + (vs + kWeightBase - sm.wtop[r + e]));
+                        w[e] = !all && x[r + e] == -INFINITY ? 0.0f : ex2(x[r + e] + (vs + ref.y));
                     }
                     const uint32_t hi = e4m3_split(w[0], w[1]);
                     const uint32_t lo = e4m3x2(w[0] / kPLo, w[1] / kPLo);
-                    asm volatile("st.shared.u8 [%0], %1;" ::"r"(pb + swizzled(r, me)), "r"(hi & 0xFFu) : "memory");
-                    asm volatile("st.shared.u8 [%0], %1;" ::"r"(pb + swizzled(r + 1, me)), "r"(hi >> 8) : "memory");
-                    asm volatile("st.shared.u8 [%0], %1;" ::"r"(pb + swizzled(R + r, me)), "r"(lo & 0xFFu) : "memory");
-                    asm volatile("st.shared.u8 [%0], %1;" ::"r"(pb + swizzled(R + r + 1, me)), "r"(lo >> 8) : "memory");
+                    w8[r / 4] |= hi << (8 * (r & 2));
+                    w8[(R + r) / 4] |= lo << (8 * (r & 2));
                 }
+                // the weights of the tile before have been read
+                ok = t == 0 || mbar_wait_warp(bar(B_PVDONE + (s ^ 1)), ((t - 1) >> 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION);
                 // a token that does not exist weighs 0, but what lies in its place may be anything, and 0 * NaN is not 0
-                if (!there) {
+                if (__any_sync(0xFFFFFFFFu, !there)) {
+                    ok = ok && mbar_wait_warp(bar(B_VFULL + s), (t >> 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION);
+                    if (!there) {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(smem_u32(sm.v[s]) + me * kKv8Dim + i * 16), "r"(0) : "memory");
-                }
-                fence_proxy_async_smem();
-                tc_fence_before();
-                mbar_arrive(bar(B_PFULL + s));
-            }
-            if (!ok) break;
-            if (n > 0) mbar_arrive(bar(B_QEMPTY + qs));
-
-            // ---- the result of these groups ----
-            if (n > 0) ok = mbar_wait_warp(bar(B_PVDONE + (int)((t - 1) & 1u)), ((t - 1) >> 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION);
-#pragma unroll
-            for (int r = 0; r < R; ++r) {
-                float v = sum[r];
-#pragma unroll
-                for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, d);
-                if (lane == 0) sm.red[warp][r][0] = v;
-            }
-            if (any_of_softmax(!ok)) { ok = false; break; }
-            tc_fence_after();
-            const bool whole = first_unit == c.unit0 && at == c.unit1;
-            const int slot = 2 * (int)blockIdx.x + (c.unit0 > begin ? 1 : 0);
-            const int rows = min(R, c.w.n * a.group - c.row_tile * R);
-#pragma unroll
-            for (int r0 = 0; r0 < R; r0 += 8) {
-                uint32_t hi[8], lo[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) hi[e] = lo[e] = 0u;
-                if (n > 0) {
-                    tmem_ld_x8(t_o + (uint32_t)r0, hi);
-                    tmem_ld_x8(t_o + (uint32_t)(R + r0), lo);
-                    tmem_ld_wait();
-                }
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int r = r0 + e;
-                    if (r >= rows) break;
-                    const float o = fmaf(__uint_as_float(lo[e]), kPLo, __uint_as_float(hi[e]));
-                    const float l = (sm.red[0][r][0] + sm.red[1][r][0]) + (sm.red[2][r][0] + sm.red[3][r][0]);
-                    if (whole) {
-                        // a row that sees nothing has the sum 0 and the result 0; a NaN sum stays one
-                        const float inv = l == 0.0f ? 0.0f : ex2(sm.wtop[r] - kWeightBase - sm.top[r]) / l;
-                        const int row = c.row_tile * R + r, tk = a.by_group.div(row);
-                        a.out[(long long)(c.w.row0 + tk) * a.ldo + (size_t)(c.head * a.group + row - tk * a.group) * kKv8Dim + me] = __float2bfloat16(o * inv);
-                    } else {
-                        const size_t to = (size_t)slot * R + r;
-                        p.part.acc[to * kKv8Dim + me] = o;
-                        if (me == 0) p.part.stats[to] = make_float4(sm.top[r], l, sm.wtop[r] - kWeightBase, 0.0f);
+                        for (int i = 0; i < 8; ++i)
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(smem_u32(sm.v[s]) + me * kKv8Dim + i * 16), "r"(0) : "memory");
                     }
                 }
+                if (!ok) *abort_word = ST_TIMEOUT_ATTENTION;  // said at the next vote
+#pragma unroll
+                for (int i = 0; i < N / 16; ++i)
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(smem_u32(sm.p) + i * (16 * SOFTMAX) + me * 16), "r"(w8[4 * i]),
+                                 "r"(w8[4 * i + 1]), "r"(w8[4 * i + 2]), "r"(w8[4 * i + 3]) : "memory");
+                fence_proxy_async_smem();
+                tc_fence_before();
+                mbar_arrive(bar(B_PFULL));
             }
+
+            // ---- the result of these groups ----
+            ok = ok && mbar_wait_warp(bar(B_PVDONE + (int)((t - 1) & 1u)), ((t - 1) >> 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION);
+            // sums over the warp's 32 tokens: halves of the rows are exchanged until a lane has one, then the lanes that share it add up
+            {
+                constexpr int P2 = U <= 4 ? 4 : U <= 8 ? 8 : U <= 16 ? 16 : 32;
+                float v[P2];
+#pragma unroll
+                for (int r = 0; r < P2; ++r) v[r] = r < U ? sum[r < U ? r : 0] : 0.0f;
+                int held = P2;
+#pragma unroll
+                for (int d = 16; d > 0; d >>= 1) {
+                    if (held > 1) {
+                        held /= 2;
+                        const bool upper = (lane & d) != 0;
+#pragma unroll
+                        for (int i = 0; i < P2 / 2; ++i)
+                            if (i < held) {
+                                const float give = upper ? v[i] : v[held + i], keep = upper ? v[held + i] : v[i];
+                                v[i] = keep + __shfl_xor_sync(0xFFFFFFFFu, give, d);
+                            }
+                    } else {
+                        v[0] += __shfl_xor_sync(0xFFFFFFFFu, v[0], d);
+                    }
+                }
+                if ((lane & (32 / P2 - 1)) == 0 && lane / (32 / P2) < U) sm.red[warp][lane / (32 / P2)][0] = v[0];
+            }
+            if (any_of_softmax(!ok)) break;
+            if (me < c.rows) {
+                const float l = (sm.red[0][me][0] + sm.red[1][me][0]) + (sm.red[2][me][0] + sm.red[3][me][0]);
+                const float4 st = sm.row[me];
+                if (c.slot < 0) sm.factor[me][0] = l == 0.0f ? 0.0f : ex2(st.z - st.w) / l;      // NaN stays NaN
+                else p.part.stats[(size_t)c.slot * U + me] = make_float4(-st.z, l, -st.w, 0.0f);
+            }
+            tc_fence_after();
+            uint32_t raw[N];
+#pragma unroll
+            for (int i = 0; i < N; i += 16) tmem_ld_x16(t_o + (uint32_t)i, *reinterpret_cast<uint32_t(*)[16]>(&raw[i]));
+            tmem_ld_wait();
             tc_fence_before();
-            if (n > 0) mbar_arrive(bar(B_OFREE));
-            if (any_of_softmax(false)) {}                     // the state in shared memory is free for the next context
+            mbar_arrive(bar(B_OFREE));
+            (void)any_of_softmax(false);
+            if (c.slot < 0) {
+#pragma unroll
+                for (int r = 0; r < U; ++r)
+                    if (r < c.rows) c.out[r][me] = __float2bfloat16(fmaf(__uint_as_float(raw[R + r]), kPLo, __uint_as_float(raw[r])) * sm.factor[r][0]);
+            } else {
+                float *to = p.part.acc + (size_t)c.slot * U * kKv8Dim + me;
+#pragma unroll
+                for (int r = 0; r < U; ++r)
+                    if (r < c.rows) to[r * kKv8Dim] = fmaf(__uint_as_float(raw[R + r]), kPLo, __uint_as_float(raw[r]));
+            }
+            mbar_arrive(bar(B_CEMPTY + cs));
+            // the rows' state and factors are written again after the next context's first vote
         }
     }
 
@@ -620,56 +730,34 @@ struct Joined {
     }
 };
 
-// Contexts that several pieces share.  A CTA of eight warps takes 8 / per rows, `per` warps each: the row's parts are dealt out to
-// them, every one joins its own, and the first joins those.
-__global__ void __launch_bounds__(256) kv8_join_kernel(const __grid_constant__ Kv8Attend a, const Partial part, int rows, int per) {
-    __shared__ float4 stats[8], acc[8][kKv8Dim / 4];
+// Contexts that several pieces share: CTA (piece, row) joins that row of the context that begins in the piece, if there is one.  The parts
+// are dealt out to the warps, every one joins its own, and the first joins those.
+constexpr int JOIN_WARPS = 4;
+__global__ void __launch_bounds__(JOIN_WARPS * 32) kv8_join_kernel(const __grid_constant__ Kv8Attend a, const Partial part, int rows) {
+    __shared__ float4 stats[JOIN_WARPS], acc[JOIN_WARPS][kKv8Dim / 4];
     pdl_launch_dependents();
+    pdl_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int mine = warp % per;
-    const int item = (int)blockIdx.x * (8 / per) + warp / per;
-    const int token = a.by_q_heads.div(item), q_head = item - token * a.b.q_heads;
+    const int piece = (int)blockIdx.x, r = (int)blockIdx.y;
+    const JoinInfo info = part.join[piece];
+    if (info.last < 0 || r >= info.rows) return;
     Joined j;
-    bool shared_row = token < a.b.total_new;
-    int seq = -1, head = 0, r = 0;
-    SeqWork w;
-    if (shared_row) {
-        const int *cu = a.b.cu_new;
-        seq = warp_last_not_above(a.b.num_seqs + 1, (long long)token, [&](int s) { return (long long)cu[s]; });
-        shared_row = seq >= 0 && seq < a.b.num_seqs;
-    }
-    if (shared_row) {
-        w = seq_work(a, seq, rows);
-        head = a.by_group.div(q_head);
-        r = (token - w.row0) * a.group + q_head - head * a.group;
-        shared_row = token - w.row0 < w.n;
-    }
-    pdl_wait();                       // the parts are there
-    if (shared_row) {
-        const int quota = part.prefix[a.b.num_seqs + 1];
-        const int first = part.prefix[seq] + (r / rows * a.b.kv_heads + head) * w.units;
-        const int w0 = first / quota, w1 = (first + w.units - 1) / quota;
-        shared_row = w0 != w1;
-        if (shared_row) {
+    const int parts = info.last - piece + 1;
 #pragma unroll 4
-            for (int p = w0 + mine; p <= w1; p += per) {
-                const size_t at = (size_t)(2 * p + (first > p * quota ? 1 : 0)) * rows + r % rows;
-                j.add(part.stats[at], *reinterpret_cast<const float4 *>(part.acc + at * kKv8Dim + lane * 4));
-            }
-        }
+    for (int i = warp; i < parts; i += JOIN_WARPS) {
+        const size_t at = (size_t)(i == 0 ? info.slot : 2 * (piece + i)) * rows + r;
+        j.add(part.stats[at], *reinterpret_cast<const float4 *>(part.acc + at * kKv8Dim + lane * 4));
     }
-    if (per > 1) {
-        if (mine != 0) {
-            if (lane == 0) stats[warp] = make_float4(j.m, j.l, j.w, 0.0f);
-            acc[warp][lane] = j.o;
-        }
-        __syncthreads();
-        if (mine != 0 || !shared_row) return;
-        for (int p = 1; p < per; ++p) j.add(stats[warp + p], acc[warp + p][lane]);
+    if (warp != 0) {
+        if (lane == 0) stats[warp] = make_float4(j.m, j.l, j.w, 0.0f);
+        acc[warp][lane] = j.o;
     }
-    if (!shared_row) return;
+    __syncthreads();
+    if (warp != 0) return;
+    for (int w = 1; w < min(JOIN_WARPS, parts); ++w) j.add(stats[w], acc[w][lane]);
     const float inv = j.l == 0.0f ? 0.0f : ex2(j.w - j.m) / j.l;
-    *reinterpret_cast<uint2 *>(a.out + (long long)token * a.ldo + (size_t)q_head * kKv8Dim + lane * 4) =
+    const int row = info.row0 + r, tok = a.by_group.div(row);
+    *reinterpret_cast<uint2 *>(a.out + (long long)(info.first_token + tok) * a.ldo + (size_t)(info.head * a.group + row - tok * a.group) * kKv8Dim + lane * 4) =
         make_uint2(pack2(j.o.x * inv, j.o.y * inv), pack2(j.o.z * inv, j.o.w * inv));
 }
 
@@ -681,37 +769,48 @@ size_t smem_bytes(int num_seqs) { return sizeof(Smem<R>) + (size_t)num_seqs * si
 template <int R>
 int ctas_per_sm(int num_seqs) {
     const int fit = (int)(kSmemPerSm / (smem_bytes<R>(num_seqs) + kSmemReserved));
-    return fit < 1 ? 1 : fit > (R == 8 ? 3 : 2) ? (R == 8 ? 3 : 2) : fit;
+    return fit < 1 ? 1 : fit > max_ctas(R) ? max_ctas(R) : fit;
 }
 
-template <int R>
+template <int R, int U>
 bool launch_rows(Params &p, void *workspace, int num_seqs, cudaStream_t st, int &grid) {
     static PerDevice<bool> configured;
     const cudaError_t ready = once_per_device(configured, [] {
-        const cudaError_t e = cudaFuncSetAttribute(kv8_attend_kernel<R>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes<R>(MAX_SEQS));
+        const cudaError_t e = cudaFuncSetAttribute(kv8_attend_kernel<R, U>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes<R>(MAX_SEQS));
         if (e != cudaSuccess) return e;
-        return cudaFuncSetAttribute(kv8_attend_kernel<R>, cudaFuncAttributePreferredSharedMemoryCarveout, (int)cudaSharedmemCarveoutMaxShared);
+        return cudaFuncSetAttribute(kv8_attend_kernel<R, U>, cudaFuncAttributePreferredSharedMemoryCarveout, (int)cudaSharedmemCarveoutMaxShared);
     });
     if (ready != cudaSuccess) return false;
     grid = num_sms() * ctas_per_sm<R>(num_seqs);
-    partial_bytes(grid, R, num_seqs, workspace, &p.part);
-    return launch_chained(kv8_attend_kernel<R>, dim3(grid), dim3(THREADS), smem_bytes<R>(num_seqs), st, p) == cudaSuccess;
+    if (p.whole) grid = (long long)num_seqs * p.a.b.kv_heads < grid ? num_seqs * p.a.b.kv_heads : grid;
+    partial_bytes(grid, U, workspace, &p.part);
+    return launch_chained(kv8_attend_kernel<R, U>, dim3(grid), dim3(THREADS), smem_bytes<R>(num_seqs), st, p) == cudaSuccess;
 }
 
 }  // namespace
 
-size_t kv8_attention_workspace_bytes(int num_seqs) {
-    const size_t one = partial_bytes(num_sms() * 3, 8, num_seqs, nullptr, nullptr);
-    const size_t more = partial_bytes(num_sms() * 2, 32, num_seqs, nullptr, nullptr);
-    return one > more ? one : more;
+size_t kv8_attention_workspace_bytes() {
+    size_t most = 0;
+    for (int rows = 8; rows <= 32; rows += 8) {
+        const size_t bytes = partial_bytes(num_sms() * max_ctas(rows), rows, nullptr, nullptr);
+        if (bytes > most) most = bytes;
+    }
+    return most;
+}
+
+// Whole (sequence, kv head) pairs or pieces?
+static bool deal_whole(const Kv8Attend &a, int rows, int max_new, int max_len, int grid) {
+    const char *e = getenv("KV8_WHOLE");
+    if (e) return e[0] == '1';
+    return false;
 }
 
 bool kv8_attention_launch(const Kv8Attend &a, int max_new, int max_len, void *workspace, cudaStream_t st, int &launches) {
     if (a.b.num_seqs > MAX_SEQS) return false;
     const long long want = (long long)max_new * a.group;
-    const int rows = want <= 8 ? 8 : want <= 16 ? 16 : 32;
+    const int rows = want <= 4 ? 4 : want <= 24 ? (int)(want + 7) / 8 * 8 : 32;
     // units are counted in 32 bits
-    const long long groups = (long long)a.b.max_blocks * a.b.block_size / kKv8Group + 1;
+    const long long groups = (long long)a.b.max_tokens / kKv8Group + 1;
     const long long most = ((long long)a.b.total_new * a.group / rows + a.b.num_seqs) * a.b.kv_heads;
     if (most > 0x7FFFFFFFLL / groups) return false;
     Params p;
@@ -721,20 +820,20 @@ bool kv8_attention_launch(const Kv8Attend &a, int max_new, int max_len, void *wo
     if (!make_u8_tmap_sw128(&p.tm_v, a.v_cache, kKv8Dim, pool_rows, kKv8Dim, kKv8Dim, kKv8Group)) return false;
     p.a = a;
     p.min_units = 4;
+    p.whole = deal_whole(a, rows, max_new, max_len, 0) ? 1 : 0;
     int grid = 0;
     bool ok = false;
     switch (rows) {
-        case 8: ok = launch_rows<8>(p, workspace, a.b.num_seqs, st, grid); break;
-        case 16: ok = launch_rows<16>(p, workspace, a.b.num_seqs, st, grid); break;
-        default: ok = launch_rows<32>(p, workspace, a.b.num_seqs, st, grid); break;
+        case 4: ok = launch_rows<8, 4>(p, workspace, a.b.num_seqs, st, grid); break;
+        case 8: ok = launch_rows<8, 8>(p, workspace, a.b.num_seqs, st, grid); break;
+        case 16: ok = launch_rows<16, 16>(p, workspace, a.b.num_seqs, st, grid); break;
+        case 24: ok = launch_rows<24, 24>(p, workspace, a.b.num_seqs, st, grid); break;
+        default: ok = launch_rows<32, 32>(p, workspace, a.b.num_seqs, st, grid); break;
     }
     if (!ok) return false;
-    // warps per row of the join: about four parts for each, as many parts as there are CTAs for a context
-    const long long parts = (long long)grid / ((long long)a.b.num_seqs * a.b.kv_heads);
-    const int per = parts <= 4 ? 1 : parts <= 8 ? 2 : parts <= 16 ? 4 : 8;
-    const long long items = (long long)a.b.total_new * a.b.q_heads;
-    const long long ctas = (items + 8 / per - 1) / (8 / per);
-    if (launch_chained(kv8_join_kernel, dim3((unsigned)ctas), dim3(256), 0, st, a, p.part, rows, per) != cudaSuccess) return false;
+    launches = 1;
+    if (p.whole) return true;
+    if (launch_chained(kv8_join_kernel, dim3((unsigned)grid, (unsigned)rows), dim3(JOIN_WARPS * 32), 0, st, a, p.part, rows) != cudaSuccess) return false;
     launches = 2;
     return true;
 }

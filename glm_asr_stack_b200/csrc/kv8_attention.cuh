@@ -27,8 +27,7 @@ struct Kv8Span {
     __device__ __forceinline__ int group_of(int i) const { return i < sink ? i : from + (i - sink); }
 };
 __device__ __forceinline__ Kv8Span kv8_span(const Kv8Attend &a, int len, int p0, int p1) {
-    const long long cap = (long long)a.b.max_blocks * a.b.block_size;
-    const int end = (int)min((long long)min(len, p1 + 1), cap);           // tokens [0, end) exist for them
+    const int end = min(min(len, p1 + 1), a.b.max_tokens);               // tokens [0, end) exist for them
     Kv8Span s = {0, 0, 0};
     if (end <= 0) return s;
     const int to = (end + kKv8Group - 1) / kKv8Group;
@@ -45,7 +44,7 @@ __device__ __forceinline__ bool kv8_sees(const Kv8Attend &a, int pos, int tok) {
 #endif
 
 // Bytes of workspace the launch may use (partial results of contexts that several warps share), on the current device.
-size_t kv8_attention_workspace_bytes(int num_seqs);
+size_t kv8_attention_workspace_bytes();
 bool kv8_attention_launch(const Kv8Attend &a, int max_new, int max_len, void *workspace, cudaStream_t st, int &launches);
 
 }  // namespace glmasr

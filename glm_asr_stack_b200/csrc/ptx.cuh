@@ -318,6 +318,11 @@ __device__ __forceinline__ void tmem_cp_32x128b_warpx4_pair(uint32_t taddr, uint
 // ---- sm_100 arithmetic for instruction-bound loops (soft-max, quantising epilogues) -----------------
 // A three-input maximum and packed two-lane fp32 multiply / add / multiply-add (each lane IEEE round-to-nearest,
 // i.e. the same bits as the scalar instruction).
+__device__ __forceinline__ float redux_max(float x) {         // over a converged warp; NaN only where all are
+    float y;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
+    return y;
+}
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -371,6 +376,16 @@ __device__ __forceinline__ uint64_t smem_desc_sw128_mn(uint32_t saddr, uint32_t 
     d |= (uint64_t)(1024 >> 4) << 32;             // stride byte offset: next eight k rows
     d |= (uint64_t)1 << 46;
     d |= (uint64_t)2 << 61;
+    return d;
+}
+// MN-major operand without a swizzle: blocks of 16 bytes (columns) x 8 k rows are 128 bytes in one piece, the next eight k rows
+// follow at once, the next 16 bytes of columns start block_bytes further on.
+__device__ __forceinline__ uint64_t smem_desc_mn(uint32_t saddr, uint32_t block_bytes) {
+    uint64_t d = 0;
+    d |= (uint64_t)((saddr & 0x3FFFF) >> 4);
+    d |= (uint64_t)(128 >> 4) << 16;              // leading byte offset: next eight k rows
+    d |= (uint64_t)(block_bytes >> 4) << 32;      // stride byte offset: next 16 bytes of columns
+    d |= (uint64_t)1 << 46;
     return d;
 }
 // Un-swizzled descriptor for a 32-row x 16-byte block stored row after row (16-byte pitch):

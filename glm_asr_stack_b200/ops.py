@@ -384,7 +384,7 @@ def kv8_attention(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
     if n == 0 or tokens == 0:
         return out
     lib = _lib.load()
-    size = lib.glmasr_kv8_attention_workspace(n)
+    size = lib.glmasr_kv8_attention_workspace()
     workspace = torch.empty(size, dtype=torch.uint8, device=device)
     rc = lib.glmasr_kv8_attention(out.data_ptr(), out.stride(0), query.data_ptr(), query.stride(0), ctypes.byref(cache),
                                   block_tables.data_ptr(), block_tables.shape[1], seq_lens.data_ptr(), cu_new.data_ptr(), n, tokens,
