@@ -14,8 +14,8 @@
 //            2^(x_j + log2 v_scale_j - W + 6), at most 2^8, is split as p = hi + 2^-4 lo: off by 6.6e-4 of its size (rms; bf16: 1.6e-3) or 2^-20
 //            of the largest, whichever is more.
 //   lazily   m and W are touched when a term has grown past 2^8 m or 2^2 W: an ordinary tile needs one vote of its four warps.
-//   split    Two ways to deal out the work, chosen on the host (see deal_whole()).  Whole: a CTA takes every gridDim-th (sequence, kv head)
-//            and there is nothing to join.  Pieces: all visible groups of 16 tokens of all (sequence, kv head) pairs form one line,
+//   split    Two ways to deal out the work, chosen on the host (see deal_whole()).  Whole: one CTA of the grid for each (sequence, kv head); those that run take
+//            over the work of those that have not started, and there is nothing to join.  Pieces: all visible groups of 16 tokens of all (sequence, kv head) pairs form one line,
 //            cut into equal pieces, one per CTA, so that uneven lengths cost nothing; a piece that ends inside a context leaves m,
 //            W, the sum and the accumulator in the workspace, and a second launch joins those.
 // A CTA walks its piece context by context in tiles of up to eight groups: warp 4 copies (a TMA box of 2 KB per group, K or V; the
@@ -46,7 +46,7 @@ constexpr float kNothing = -3.4028234664e38f;                 // m and W before 
 constexpr float kTop = 8.0f, kWeightTop = 2.0f, kWeightBase = 6.0f;
 constexpr float kQLo = 1.0f / 32.0f, kPLo = 1.0f / 16.0f;
 
-enum : int { B_KFULL = 0, B_KEMPTY = 2, B_VFULL = 4, B_PVDONE = 6, B_SFULL = 8, B_SCALES = 10, B_CFULL = 12, B_CEMPTY = 14, B_PFULL = 16, B_OFREE = 17, B_COUNT = 18 };
+enum : int { B_KFULL = 0, B_KEMPTY = 2, B_VFULL = 4, B_PVDONE = 6, B_SFULL = 8, B_SCALES = 10, B_CFULL = 12, B_CEMPTY = 14, B_PFULL = 16, B_OFREE = 17, B_NEXT = 18, B_COUNT = 19 };
 
 // What the products and the softmax have to know of a context.
 template <int R>
@@ -71,6 +71,7 @@ struct Smem {
     float red[4][R][2], factor[R][2];
     float2 scales[2][TILE_GROUPS];        // K, V
     int tokens[2][TILE_GROUPS];           // of each group that exist
+    uint4 next;                           // answer to the question for more work
     unsigned long long bars[B_COUNT];
     uint32_t tmem;
     int abort, warp_sum[8];
@@ -148,12 +149,21 @@ struct Context {
     int unit0, unit1;                 // its units on the line
     int from, to;                     // its groups in this piece, of w.span.count
 };
+// x / d for x >= 0, d > 0: the fp32 quotient of rounded numbers is off by 2^-22 of itself, so its floor by one below 2^22; beyond, exactly.
+__device__ __forceinline__ int quotient(int x, int d) {
+    if (x >= (1 << 22)) return x / d;
+    int q = (int)__fdividef((float)x, (float)d);
+    const int r = x - q * d;
+    if (r < 0) --q;
+    if (r >= d) ++q;
+    return q;
+}
 __device__ __forceinline__ Context context_at(const Kv8Attend &a, const int *prefix, int rows, int seq, int at, int end) {
     Context c;
     while (seq + 1 < a.b.num_seqs && prefix[seq + 1] <= at) ++seq;
     c.seq = seq;
     c.w = seq_work(a, seq, rows);
-    const int x = (at - prefix[seq]) / c.w.units;
+    const int x = quotient(at - prefix[seq], c.w.units);
     c.unit0 = prefix[seq] + x * c.w.units;
     c.unit1 = c.unit0 + c.w.units;
     c.row_tile = a.b.by_kv_heads.div(x);
@@ -219,6 +229,7 @@ __global__ void __launch_bounds__(THREADS, max_ctas(R)) kv8_attend_kernel(const 
     if (threadIdx.x == 0) {
         mbar_init(bar(B_PFULL), SOFTMAX);
         mbar_init(bar(B_OFREE), SOFTMAX);
+        mbar_init(bar(B_NEXT), 1);
         for (int i = 0; i < 2; ++i) {
             mbar_init(bar(B_KFULL + i), 1);
             mbar_init(bar(B_KEMPTY + i), 1);
@@ -307,7 +318,8 @@ __global__ void __launch_bounds__(THREADS, max_ctas(R)) kv8_attend_kernel(const 
         const bool leader = elect_one();
         uint32_t t = 0, contexts = 0; // tiles and contexts started
         bool ok = true, have = false, first = false, more = true;
-        int at = begin, first_unit = begin, g = 0, rows = 0, item = (int)blockIdx.x;
+        int at = begin, first_unit = begin, g = 0, rows = 0, item = -1;
+        uint32_t asked = 0;           // for more work
         JoinInfo join = {-1, 0, 0, 0, 0, 0};
         Context c;
         c.seq = seq0, c.to = 0, c.row_tile = 0, c.w.tiles = 0;
@@ -322,11 +334,25 @@ __global__ void __launch_bounds__(THREADS, max_ctas(R)) kv8_attend_kernel(const 
                     join = {(c.unit1 - 1) / quota, 2 * (int)blockIdx.x + (c.unit0 > begin ? 1 : 0), 0, c.row_tile * U, c.head, c.w.row0};
             } else if (++c.row_tile >= c.w.tiles) {
                 do {
-                    if (item >= a.b.num_seqs * a.b.kv_heads) return false;
+                    if (item < 0) {
+                        item = (int)blockIdx.x;
+                    } else {
+                        ok = mbar_wait_warp(bar(B_NEXT), (asked - 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION);
+                        if (!ok) return false;
+                        item = cancelled_cta(smem_u32(&sm.next));
+                        if (item < 0) return false;
+                        fence_proxy_async_smem();             // the answer has been read before the next one is written
+                        __syncwarp();
+                    }
+                    if (leader) {
+                        mbar_expect_tx(bar(B_NEXT), 16);
+                        ask_cancelled_cta(smem_u32(&sm.next), bar(B_NEXT));
+                    }
+                    __syncwarp();
+                    ++asked;
                     c.seq = a.b.by_kv_heads.div(item);
                     c.head = item - c.seq * a.b.kv_heads;
                     c.w = seq_work(a, c.seq, U);
-                    item += (int)gridDim.x;
                 } while (c.w.tiles == 0);
                 c.row_tile = c.from = 0;
                 c.to = c.w.span.count;
@@ -344,7 +370,7 @@ __global__ void __launch_bounds__(THREADS, max_ctas(R)) kv8_attend_kernel(const 
             tok = a.by_group.div(row);
             return (size_t)(c.head * a.group + row - tok * a.group) * kKv8Dim;
         };
-        auto ask_queries = [&](int r) {
+        auto ask_queries = [&](int r, uint4 (&q)[QI]) {
             int tok;
             const size_t col = place_of(r, tok);
             const __nv_bfloat16 *src = a.query + (long long)(c.w.row0 + tok) * a.ldq + col + (lane % QL) * 8;
@@ -361,7 +387,7 @@ __global__ void __launch_bounds__(THREADS, max_ctas(R)) kv8_attend_kernel(const 
                     rows = min(U, c.w.n * a.group - c.row_tile * U);
                     join.rows = rows;
                     g = c.from;
-                    ask_queries(lane / QL);
+                    ask_queries(lane / QL, q);
                 }
                 if (g == c.to) {                              // nothing is visible
                     for (int r = 0; r < rows; ++r) {
@@ -394,22 +420,24 @@ __global__ void __launch_bounds__(THREADS, max_ctas(R)) kv8_attend_kernel(const 
             if (leader) mbar_expect_tx(bar(B_KFULL + s), bytes);
             __syncwarp();
             if (place >= 0) tma_load_2d(smem_u32(sm.k[s]) + lane * GROUP_BYTES, &p.tm_k, bar(B_KFULL + s), 0, place * kKv8Group);
-            ok = mbar_wait_warp(bar(B_PVDONE + s), free_phase, abort_word, ST_TIMEOUT_ATTENTION);
-            if (!ok) break;
-            if (leader) mbar_expect_tx(bar(B_VFULL + s), bytes);
-            __syncwarp();
-            if (place >= 0) tma_load_2d(smem_u32(sm.v[s]) + lane * GROUP_BYTES, &p.tm_v, bar(B_VFULL + s), 0, place * kKv8Group);
-            // the softmax is done with the scales of two tiles ago: that tile has been summed
-            auto put_scales = [&]() {
+            // V, and the scales: the tile of two before, whose places they take, has to be summed
+            auto put_v = [&]() {
+                ok = mbar_wait_warp(bar(B_PVDONE + s), free_phase, abort_word, ST_TIMEOUT_ATTENTION);
+                if (!ok) return false;
+                if (leader) mbar_expect_tx(bar(B_VFULL + s), bytes);
+                __syncwarp();
+                if (place >= 0) tma_load_2d(smem_u32(sm.v[s]) + lane * GROUP_BYTES, &p.tm_v, bar(B_VFULL + s), 0, place * kKv8Group);
                 if (lane < TILE_GROUPS) {
                     sm.scales[s][lane] = scale;
                     sm.tokens[s][lane] = tokens;
                 }
                 __syncwarp();
                 if (leader) mbar_arrive(bar(B_SCALES + s));
+                __syncwarp();
+                return true;
             };
             if (!first) {
-                put_scales();
+                if (!put_v()) break;
                 continue;
             }
             const int cs = (int)(contexts & 1u);
@@ -427,7 +455,8 @@ __global__ void __launch_bounds__(THREADS, max_ctas(R)) kv8_attend_kernel(const 
             }
 #pragma unroll 1
             for (int r = lane / QL; r < U; r += QROWS) {
-                if (r >= QROWS) ask_queries(r);
+                uint4 next[QI];
+                if (r + QROWS < U) ask_queries(r + QROWS, next);
                 uint32_t most = 0u;
 #pragma unroll
                 for (int i = 0; i < QI; ++i) {
@@ -463,11 +492,15 @@ __global__ void __launch_bounds__(THREADS, max_ctas(R)) kv8_attend_kernel(const 
                     info.pos[r] = r < rows ? c.w.start + tok : -1;
                     info.out[r] = a.out + (long long)(c.w.row0 + tok) * a.ldo + col;
                 }
+                if (r + QROWS < U) {
+#pragma unroll
+                    for (int i = 0; i < QI; ++i) q[i] = next[i];
+                }
             }
             fence_proxy_async_smem();
             __syncwarp();
             if (leader) mbar_arrive(bar(B_CFULL + cs));
-            put_scales();
+            if (!put_v()) break;
         }
         if (leader && !p.whole) p.part.join[blockIdx.x] = join;
         const int cs = (int)(contexts & 1u);
@@ -565,10 +598,15 @@ __global__ void __launch_bounds__(THREADS, max_ctas(R)) kv8_attend_kernel(const 
                 tmem_ld_wait();
 #pragma unroll
                 for (int r = 0; r < U; ++r) x[r] = fmaf(__uint_as_float(raw[R + r]), kQLo, __uint_as_float(raw[r])) * (c.qscale[r] * sc.x);
-                if (!all) {
+                if (!there) {
+#pragma unroll
+                    for (int r = 0; r < U; ++r) x[r] = -INFINITY;
+                } else if (!all) {
+                    // 0 <= p - tok < window as one comparison (a row that does not exist has the position -1)
+                    const uint32_t reach = a.window == 0 || tok < a.sinks ? 0x80000000u : (uint32_t)a.window;
 #pragma unroll
                     for (int r = 0; r < U; ++r)
-                        if (!there || !kv8_sees(a, c.pos[r], tok)) x[r] = -INFINITY;
+                        if ((uint32_t)(c.pos[r] - tok) >= reach) x[r] = -INFINITY;
                 }
                 bool grown = !ok;
 #pragma unroll
@@ -782,7 +820,7 @@ bool launch_rows(Params &p, void *workspace, int num_seqs, cudaStream_t st, int 
     });
     if (ready != cudaSuccess) return false;
     grid = num_sms() * ctas_per_sm<R>(num_seqs);
-    if (p.whole) grid = (long long)num_seqs * p.a.b.kv_heads < grid ? num_seqs * p.a.b.kv_heads : grid;
+    if (p.whole) grid = num_seqs * p.a.b.kv_heads;
     partial_bytes(grid, U, workspace, &p.part);
     return launch_chained(kv8_attend_kernel<R, U>, dim3(grid), dim3(THREADS), smem_bytes<R>(num_seqs), st, p) == cudaSuccess;
 }
@@ -798,11 +836,21 @@ size_t kv8_attention_workspace_bytes() {
     return most;
 }
 
-// Whole (sequence, kv head) pairs or pieces?
-static bool deal_whole(const Kv8Attend &a, int rows, int max_new, int max_len, int grid) {
-    const char *e = getenv("KV8_WHOLE");
-    if (e) return e[0] == '1';
-    return false;
+// Whole (sequence, kv head) pairs or pieces?  In cycles, from what the phases of the kernel take: a tile's chain 2200, the steps around a
+// context 2600, an SM's share of HBM 1400 a tile; pieces need 2000 for the table of units and 5000 for the join.  The longest
+// context stands for all, which flatters whole pairs where lengths are uneven, hence their limit of 16 tiles.
+static bool deal_whole(const Kv8Attend &a, int max_len, int slots) {
+    const long long contexts = (long long)a.b.num_seqs * a.b.kv_heads;
+    long long tokens = max_len < a.b.max_tokens ? max_len : a.b.max_tokens;
+    if (a.window > 0) {
+        const long long most = (long long)a.window + a.sinks + 2 * kKv8Group;
+        if (most < tokens) tokens = most;
+    }
+    const long long tiles = (tokens + SOFTMAX - 1) / SOFTMAX;
+    const long long memory = contexts * tiles * 1400 / num_sms();
+    const long long whole = (contexts + slots - 1) / slots * (2600 + tiles * 2200);
+    const long long pieces = (contexts * tiles * 2200 + contexts * 2600) / slots + 2200 + 2600;
+    return tiles <= 16 && (whole > memory ? whole : memory) <= 7000 + (pieces > memory ? pieces : memory);
 }
 
 bool kv8_attention_launch(const Kv8Attend &a, int max_new, int max_len, void *workspace, cudaStream_t st, int &launches) {
@@ -820,7 +868,7 @@ bool kv8_attention_launch(const Kv8Attend &a, int max_new, int max_len, void *wo
     if (!make_u8_tmap_sw128(&p.tm_v, a.v_cache, kKv8Dim, pool_rows, kKv8Dim, kKv8Dim, kKv8Group)) return false;
     p.a = a;
     p.min_units = 4;
-    p.whole = deal_whole(a, rows, max_new, max_len, 0) ? 1 : 0;
+    p.whole = deal_whole(a, max_len, num_sms() * max_ctas(rows)) ? 1 : 0;
     int grid = 0;
     bool ok = false;
     switch (rows) {

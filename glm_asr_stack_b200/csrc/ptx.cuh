@@ -125,6 +125,23 @@ __device__ __forceinline__ void bulk_load_1d(uint32_t dst, const void *src, uint
         : "memory");
 }
 
+// Ask for the work of a CTA of this launch that has not started, 16 bytes of answer to shared memory; not to be asked again after
+// the answer that there is none.
+__device__ __forceinline__ void ask_cancelled_cta(uint32_t dst, uint32_t bar) {
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(dst), "r"(bar) : "memory");
+}
+// Its index (x), -1: none is left.
+__device__ __forceinline__ int cancelled_cta(uint32_t answer) {
+    int x = -1;
+    asm volatile(
+        "{\n\t.reg .b128 h;\n\t.reg .pred p;\n\t"
+        "ld.shared.b128 h, [%1];\n\t"
+        "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\t"
+        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %0, h;\n\t}"
+        : "+r"(x) : "r"(answer) : "memory");
+    return x;
+}
+
 // 2-D tiled store shared -> global (bulk async group of the issuing thread); elements outside the
 // tensor are not written, so ragged tile edges need no predication.
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap *tm, uint32_t src, int x, int y) {
