@@ -72,7 +72,7 @@ extern "C" int glmasr_kv8_attention(uint16_t *out, long long ldo, const uint16_t
                                     void *workspace, long long workspace_bytes) {
     Kv8Attend a;
     if (!make_batch(a.b, cache, block_tables, max_blocks, seq_lens, cu_new, num_seqs, total_new, q_heads)) return -1;
-    if (q_heads <= 0 || q_heads % a.b.kv_heads != 0 || window < 0 || sinks < 0 || max_new < 0 || max_len < 0 || !isfinite(scale)) return -1;
+    if (q_heads <= 0 || q_heads % a.b.kv_heads != 0 || window < 0 || sinks < 0 || max_new < 0 || max_len < 0 || !(scale >= 0.0f) || !isfinite(scale)) return -1;
     if (num_seqs == 0 || total_new == 0) return 0;
     if (!rows_ok(query, ldq, q_heads, total_new) || !rows_ok(out, ldo, q_heads, total_new)) return -1;
     if (workspace == nullptr || !aligned16(workspace) || workspace_bytes < glmasr_kv8_attention_workspace()) return -1;
@@ -85,8 +85,8 @@ extern "C" int glmasr_kv8_attention(uint16_t *out, long long ldo, const uint16_t
     a.group = q_heads / a.b.kv_heads;
     a.by_group = FastDiv(a.group);
     a.by_q_heads = FastDiv(q_heads);
-    a.window = window;
-    a.sinks = sinks;
+    a.window = window >= a.b.max_tokens ? 0 : window;              // one that reaches past the table leaves nothing out
+    a.sinks = sinks < a.b.max_tokens ? sinks : a.b.max_tokens;
     a.scale_log2 = scale * 1.4426950408889634f;
     int launches = 0;
     if (!kv8_attention_launch(a, max_new, max_len, workspace, current_stream(), launches)) {

@@ -23,7 +23,6 @@
 // products, warps 0-3 are the softmax, one thread per token, and write the results.
 // K and V have two buffers each.  A tile's chain of waits, products and softmax is about 2000 cycles, and a copy takes as long: three
 // CTAs with 64 KB of tiles each keep HBM busy.  (Four with one buffer of each: every copy waits for a product, 4000 cycles a tile.)
-#include <cuda_fp16.h>
 #include <math.h>
 
 #include "kv8_attention.cuh"
@@ -32,7 +31,7 @@
 
 namespace glmasr {
 
-__device__ int g_kv8_status[4];
+static __device__ int g_kv8_status[4];
 
 namespace {
 
@@ -42,7 +41,6 @@ constexpr int TILE_GROUPS = SOFTMAX / kKv8Group;
 constexpr int GROUP_BYTES = kKv8Group * kKv8Dim;
 constexpr int TILE_BYTES = TILE_GROUPS * GROUP_BYTES;         // 16 KB of K, or V
 constexpr int MAX_SEQS = 4096;                                // the line's table lies in shared memory
-constexpr float kNothing = -3.4028234664e38f;                 // m and W before the first term: every term is above it, and 2^(it - m) is 0
 constexpr float kTop = 8.0f, kWeightTop = 2.0f, kWeightBase = 6.0f;
 constexpr float kQLo = 1.0f / 32.0f, kPLo = 1.0f / 16.0f;
 
@@ -78,36 +76,6 @@ struct Smem {
     int prefix[1];                        // num_seqs entries: units before each sequence
 };
 
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ float lg2(float x) {
-    float y;
-    asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }      // e in [-126, 127]
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-    const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t *>(&b);
-}
-// two values -> two e4m3 codes, nearest (the first in the low byte), and what is left of each
-__device__ __forceinline__ uint32_t e4m3_split(float &a, float &b) {
-    uint16_t c;
-    uint32_t h;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(c) : "f"(b), "f"(a));
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(c));
-    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h));
-    a -= f.x, b -= f.y;
-    return c;
-}
-__device__ __forceinline__ uint32_t e4m3x2(float a, float b) {
-    uint16_t c;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(c) : "f"(b), "f"(a));
-    return c;
-}
 // Whether any of the softmax threads says so (and a barrier among them).
 __device__ __forceinline__ bool any_of_softmax(bool x) {
     uint32_t r;
@@ -119,9 +87,6 @@ __device__ __forceinline__ bool any_of_softmax(bool x) {
         : "=r"(r) : "r"(x ? 1u : 0u) : "memory");
     return r != 0;
 }
-// byte b (0..127) of row r of an operand with 128-byte rows under the 128-byte swizzle
-__device__ __forceinline__ uint32_t swizzled(int r, int b) { return (uint32_t)(r * 128 + ((((b >> 4) ^ (r & 7)) << 4) | (b & 15))); }
-
 // The line of work.  rows = query rows (new token, head of the group) a context has at most; a sequence with more of them has
 // several row tiles.  Unit = one visible group of 16 tokens (or the one empty unit of a context in which nothing is visible) of
 // (sequence, row tile, kv head), in that order.
@@ -854,9 +819,13 @@ static bool deal_whole(const Kv8Attend &a, int max_len, int slots) {
 }
 
 bool kv8_attention_launch(const Kv8Attend &a, int max_new, int max_len, void *workspace, cudaStream_t st, int &launches) {
-    if (a.b.num_seqs > MAX_SEQS) return false;
     const long long want = (long long)max_new * a.group;
-    const int rows = want <= 4 ? 4 : want <= 24 ? (int)(want + 7) / 8 * 8 : 32;
+    if (want > 32) {
+        launches = 1;
+        return kv8_prefill_launch(a, st);
+    }
+    if (a.b.num_seqs > MAX_SEQS) return false;
+    const int rows = want <= 4 ? 4 : (int)(want + 7) / 8 * 8;
     // units are counted in 32 bits
     const long long groups = (long long)a.b.max_tokens / kKv8Group + 1;
     const long long most = ((long long)a.b.total_new * a.group / rows + a.b.num_seqs) * a.b.kv_heads;
@@ -893,7 +862,8 @@ int kv8_take_status() {
         const int zero[4] = {0, 0, 0, 0};
         (void)cudaMemcpyToSymbol(g_kv8_status, zero, sizeof(zero));
     }
-    return code[0];
+    const int prefill = kv8_prefill_take_status();
+    return code[0] != 0 ? code[0] : prefill;
 }
 
 }  // namespace glmasr
