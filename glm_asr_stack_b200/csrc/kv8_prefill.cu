@@ -6,9 +6,10 @@
 //                     elements down to 2^-9 of the largest, off by 2^-17 of the largest below.  Two products of 8-bit operands
 //                     cost what one of 16-bit operands does, and no key is converted.
 //   p = 2^(x - m)     x = s * (row scale) * (K scale of the block of 16 keys); m is touched when a row's maximum has grown past 2^8 m.
-//   O += P V          f16 x f16: weights have 11 bits.  V's codes become f16, times the scale of their block over the largest scale of
-//                     the item so far (exact: a power of two), which O is expressed against.  Where a block's scale is 2^15
-//                     below that one f16 would lose bits of it: such a step's P and V are bf16.
+//   O += P V          f16 x f16: weights have 11 bits down to 2^-14 of the largest, and are off by 2^-25 of it below.  V's codes become
+//                     f16, times the scale of their block over the largest scale of the item so far (exact: a power of two),
+//                     which O is expressed against.  From the first block on whose scale is 2^5 below that one, small weights
+//                     on large values may be what counts: P and V are bf16, 8 bits of any size (a block of zeros does not count).
 // Bound: the two products are 2 x 128 x 128 x 128 multiply-adds a step, 1024 cycles at the tensor cores' nominal rate, and the
 // exponentials 1024 of the special-function units, under each other in the best case.  A step is a chain (scores, softmax, weighted
 // sum), so two CTAs share an SM and one's softmax runs under the other's products.
@@ -34,7 +35,7 @@ constexpr int QT = 128, KT = 128, THREADS = 320;
 constexpr int GROUPS = KT / kKv8Group, GROUP_BYTES = kKv8Group * kKv8Dim;
 constexpr int TMEM_COLS = 256, COL_O = 128;
 constexpr float kLazy = 8.0f;                 // log2: P may grow to 2^8
-constexpr float kF16Range = 1.0f / 32768.0f;
+constexpr float kF16Range = 1.0f / 32.0f;     // of V scales
 
 enum : int { B_KFULL = 0, B_KEMPTY = 2, B_STEP = 4, B_PVDONE = 6, B_INFO = 8, B_INFOFREE = 10, B_SFULL = 12, B_PFULL = 13, B_VFULL = 14, B_QFULL = 15,
              B_OFREE = 16, B_NEXT = 17, B_COUNT = 18 };
@@ -167,6 +168,7 @@ __global__ void __launch_bounds__(THREADS, 2) kv8_prefill_kernel(const __grid_co
                 __syncwarp();
                 ++items;
                 float vref = 0.0f;
+                bool wide = false;
                 for (int g = 0; g < span.count; g += GROUPS, ++t) {
                     const int s = (int)(t & 1u);
                     const uint32_t free_phase = ((t >> 1) & 1u) ^ 1u;
@@ -198,7 +200,8 @@ __global__ void __launch_bounds__(THREADS, 2) kv8_prefill_kernel(const __grid_co
                     const bool plain_here = tokens == kKv8Group && key + kKv8Group - 1 <= pos_lo &&
                                             (a.window == 0 || pos_hi - key < a.window || key + kKv8Group <= a.sinks);
                     const bool mine = lane < GROUPS;
-                    const uint32_t plain = __ballot_sync(0xFFFFFFFFu, mine && plain_here), wide = __ballot_sync(0xFFFFFFFFu, mine && vmul > 0.0f && vmul < kF16Range);
+                    const uint32_t plain = __ballot_sync(0xFFFFFFFFu, mine && plain_here), far = __ballot_sync(0xFFFFFFFFu, mine && vs > 0x1p-126f && vmul < kF16Range && number);
+                    wide = wide || far != 0u;
                     const uint32_t poisoned = __ballot_sync(0xFFFFFFFFu, mine && !number);
                     // the step two before, whose place this is, has been summed: softmax and V are done with it
                     ok = mbar_wait_warp(bar(B_PVDONE + s), free_phase, abort_word, ST_TIMEOUT_ATTENTION);
@@ -212,7 +215,7 @@ __global__ void __launch_bounds__(THREADS, 2) kv8_prefill_kernel(const __grid_co
                         st.vref = most;
                         st.vstep = most > 0.0f ? vref / most : 1.0f;
                         st.plain = plain == (1u << GROUPS) - 1u ? 1 : 0;
-                        st.wide = wide != 0u ? 1 : 0;
+                        st.wide = wide ? 1 : 0;
                         st.poisoned = poisoned;
                     }
                     __syncwarp();

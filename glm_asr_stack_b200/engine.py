@@ -192,6 +192,25 @@ class KVPool:
         self.block_size, self.max_blocks_per_seq = block_size, max_blocks_per_seq
 
 
+class KV8Pool:
+    """Paged KV pool in 8 bits (ops.kv8_append, ops.kv8_attention): per layer e4m3 codes
+    [num_blocks, kv_heads, block_size, 128] and fp32 scales [num_blocks, kv_heads, block_size / 16] for K and V, half the bytes
+    of KVPool.  ``layer(i)`` is the four tensors in the order both calls take them; block tables are the caller's, int32
+    [sequences, pages] on the device, one for all layers."""
+
+    def __init__(self, num_blocks, block_size, num_layers, kv_heads, device="cuda"):
+        if block_size <= 0 or block_size % 16 != 0:
+            raise ValueError("block_size must be a multiple of 16")
+        codes = (num_layers, num_blocks, kv_heads, block_size, 128)
+        scales = (num_layers, num_blocks, kv_heads, block_size // 16)
+        self.k, self.v = (torch.zeros(codes, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn) for _ in range(2))
+        self.k_scale, self.v_scale = (torch.zeros(scales, dtype=torch.float32, device=device) for _ in range(2))
+        self.block_size = block_size
+
+    def layer(self, i):
+        return self.k[i], self.v[i], self.k_scale[i], self.v_scale[i]
+
+
 class BlockTables:
     """``BlockTable[num_seqs]`` with host mirrors; row i of the pool's device table belongs to sequence i."""
 
