@@ -92,9 +92,9 @@ SIGNATURES = {
     "glmasr_fp4_layer_proj": (c_int, [c_int, P, P, POINTER(LayerWeights), c_int]),
     "glmasr_fp4_layer_proj_host": (c_int, [c_int, P, P, POINTER(LayerWeights), c_int]),
     "glmasr_nvfp4_linear_noalloc": (c_int, [P, P, P, P, c_float, c_float, c_int, c_int, c_int]),
-    "glmasr_kv8_append": (c_int, [POINTER(Kv8Cache), P, L, P, L, P, L, P, L, c_int, P, c_int, P, P, c_int, c_int, c_double]),
+    "glmasr_kv8_append": (c_int, [P, P, L, P, L, P, L, P, L, c_int, P, c_int, P, P, c_int, c_int, c_double]),
     "glmasr_kv8_attention_workspace": (L, []),
-    "glmasr_kv8_attention": (c_int, [P, L, P, L, POINTER(Kv8Cache), P, c_int, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
+    "glmasr_kv8_attention": (c_int, [P, L, P, L, P, P, c_int, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
                                      c_float, P, L]),
     "glmasr_fp4_status": (c_int, []),
     "glmasr_last_gemm_route": (c_int, []),

@@ -242,7 +242,13 @@ bool kv8_append_launch(uint8_t *k_cache, uint8_t *v_cache, float *k_scale, float
     p.query = query, p.query_out = query_out;
     p.ldq = ldq, p.ldqo = ldqo;
     p.b = b;
-    for (int d = 0; d < HALF; ++d) p.turns[d] = theta > 0.0 ? pow(theta, -(double)d / HALF) / 6.283185307179586476925 : 0.0;
+    // a function of theta alone, kept for the next layer's call
+    static double known = -1.0, turns[HALF];
+    if (theta != known) {
+        for (int d = 0; d < HALF; ++d) turns[d] = theta > 0.0 ? pow(theta, -(double)d / HALF) / 6.283185307179586476925 : 0.0;
+        known = theta;
+    }
+    memcpy(p.turns, turns, sizeof(turns));
     const long long blocks = (long long)b.total_new / 16 + 2LL * b.num_seqs;
     return launch_chained(kv8_append_kernel, dim3((unsigned)blocks), dim3(THREADS), 0, st, p) == cudaSuccess;
 }

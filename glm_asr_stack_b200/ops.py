@@ -7,6 +7,7 @@ torch is used only for device memory; every computation happens inside libglmasr
 from __future__ import annotations
 
 import ctypes
+import struct
 import weakref
 from dataclasses import dataclass
 from typing import Optional, Sequence
@@ -268,50 +269,60 @@ def paged_decode_attention(query, k_cache, v_cache, block_tables, seq_lens, num_
     return out
 
 
-def _kv8_rows(t: torch.Tensor, name: str, device, heads: Optional[int] = None):
-    """Rows of heads * 128 bf16 elements at any pitch: [rows, heads, 128]."""
+_KV8_STRUCT = struct.Struct("@QQQQiiii")        # glmasr_kv8_cache
+_KV8_SCALE = 128 ** -0.5
+_KV8_CODES = (torch.float8_e4m3fn, torch.uint8)
+_kv8_workspace_bytes = {}          # by device: a constant of the device's size
+
+
+def _kv8_rows(t: torch.Tensor, name: str, device: int, heads: Optional[int] = None):
+    """Rows of heads * 128 bf16 elements at any pitch, [rows, heads, 128]: (address, pitch, rows).  A decode step makes these calls
+    once per layer, so the good case is one condition and the reason is looked for afterwards."""
+    shape, stride = t.shape, t.stride()
+    if (t.dtype is torch.bfloat16 and len(shape) == 3 and shape[2] == 128 and stride[2] == 1 and (stride[1] == 128 or shape[1] == 1)
+            and t.get_device() == device and (shape[1] == heads or heads is None)):
+        return t.data_ptr(), stride[0], shape[0]
     if t.dtype != torch.bfloat16:
         raise TypeError(f"{name}: expected torch.bfloat16, got {t.dtype}")
-    if t.dim() != 3 or t.shape[2] != 128 or t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != 128):
-        raise ValueError(f"{name}: must be [rows, heads, 128] with the heads of a row side by side")
-    if t.device != device:
+    if t.get_device() != device:
         raise ValueError(f"{name}: not on the cache's device")
-    if heads is not None and t.shape[1] != heads:
-        raise ValueError(f"{name}: expected {heads} heads, got {t.shape[1]}")
+    if heads is not None and len(shape) == 3 and shape[1] != heads:
+        raise ValueError(f"{name}: expected {heads} heads, got {shape[1]}")
+    raise ValueError(f"{name}: must be [rows, heads, 128] with the heads of a row side by side")
 
 
 def _kv8_cache(k_cache, v_cache, k_scale, v_scale):
-    device = k_cache.device
-    if device.type != "cuda":
+    """(the C struct's bytes, device, kv heads, block size) of one layer's pool."""
+    shape, device = k_cache.shape, k_cache.get_device()
+    if (len(shape) == 4 and v_cache.shape == shape and k_cache.dtype in _KV8_CODES and v_cache.dtype in _KV8_CODES
+            and k_cache.is_contiguous() and v_cache.is_contiguous() and k_scale.dtype is torch.float32 and v_scale.dtype is torch.float32
+            and k_scale.shape == v_scale.shape == (shape[0], shape[1], shape[2] // 16) and k_scale.is_contiguous() and v_scale.is_contiguous()
+            and device >= 0 and device == v_cache.get_device() == k_scale.get_device() == v_scale.get_device() == torch.cuda.current_device()):
+        return _KV8_STRUCT.pack(k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), shape[0], shape[2], shape[1],
+                                shape[3]), device, shape[1], shape[2]
+    if device < 0:
         raise ValueError("expected a CUDA tensor")
-    if device.index != torch.cuda.current_device():
+    if device != torch.cuda.current_device():
         raise ValueError("the cache is not on the current device")
     for t, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
-        if t.dtype not in (torch.float8_e4m3fn, torch.uint8):
+        if t.dtype not in _KV8_CODES:
             raise TypeError(f"{name}: expected torch.float8_e4m3fn or torch.uint8, got {t.dtype}")
-    shape = k_cache.shape
-    if len(shape) != 4 or v_cache.shape != shape or not k_cache.is_contiguous() or not v_cache.is_contiguous():
-        raise ValueError("k_cache, v_cache: must be contiguous [num_blocks, kv_heads, block_size, 128] of one shape")
-    for t, name in ((k_scale, "k_scale"), (v_scale, "v_scale")):
-        _check(t, torch.float32, name)
-        if t.shape != (shape[0], shape[1], shape[2] // 16):
-            raise ValueError(f"{name}: must be [num_blocks, kv_heads, block_size / 16]")
-    if v_cache.device != device or k_scale.device != device or v_scale.device != device:
-        raise ValueError("codes and scales must be on one device")
-    return _lib.Kv8Cache(k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), shape[0], shape[2], shape[1],
-                         shape[3]), device
+    _check(k_scale, torch.float32, "k_scale")
+    _check(v_scale, torch.float32, "v_scale")
+    raise ValueError("expected codes [num_blocks, kv_heads, block_size, 128] and scales [num_blocks, kv_heads, block_size / 16], contiguous and on one device")
 
 
-def _kv8_batch(block_tables, seq_lens, cu_new, device):
+def _kv8_batch(block_tables, seq_lens, cu_new, device: int):
+    """(sequences, pages of a table row)."""
+    n, tables = seq_lens.numel(), block_tables.shape
+    if (block_tables.dtype is torch.int32 and seq_lens.dtype is torch.int32 and cu_new.dtype is torch.int32 and len(tables) == 2 and tables[0] == n
+            and cu_new.numel() == n + 1 and block_tables.is_contiguous() and seq_lens.is_contiguous() and cu_new.is_contiguous()
+            and device == block_tables.get_device() == seq_lens.get_device() == cu_new.get_device()):
+        return n, tables[1]
     _check(block_tables, torch.int32, "block_tables")
     _check(seq_lens, torch.int32, "seq_lens")
     _check(cu_new, torch.int32, "cu_new")
-    n = seq_lens.numel()
-    if block_tables.dim() != 2 or block_tables.shape[0] != n or seq_lens.dim() != 1 or cu_new.dim() != 1 or cu_new.numel() != n + 1:
-        raise ValueError("expected block_tables [num_seqs, max_blocks], seq_lens [num_seqs], cu_new [num_seqs + 1]")
-    if block_tables.device != device or seq_lens.device != device or cu_new.device != device:
-        raise ValueError("block_tables, seq_lens, cu_new: not on the cache's device")
-    return n
+    raise ValueError("expected block_tables [num_seqs, max_blocks], seq_lens [num_seqs], cu_new [num_seqs + 1] on the cache's device")
 
 
 def kv8_append(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, key: torch.Tensor,
@@ -325,33 +336,28 @@ def kv8_append(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tens
     [num_blocks, kv_heads, block_size / 16]; key, value [tokens, kv_heads, 128], query [tokens, q_heads, 128] bf16, row slices
     of a fused projection included.  Sequence s owns the rows cu_new[s] .. cu_new[s + 1] and has seq_lens[s] tokens WITH them
     (device int32).  theta = 0: no rotation.  Returns the rotated queries (query_out, which may be query itself), or None."""
-    cache, device = _kv8_cache(k_cache, v_cache, k_scale, v_scale)
-    n = _kv8_batch(block_tables, seq_lens, cu_new, device)
-    kv_heads = k_cache.shape[1]
-    _kv8_rows(key, "key", device, kv_heads)
-    _kv8_rows(value, "value", device, kv_heads)
-    tokens = key.shape[0]
-    if value.shape[0] != tokens:
+    cache, device, kv_heads, _ = _kv8_cache(k_cache, v_cache, k_scale, v_scale)
+    n, max_blocks = _kv8_batch(block_tables, seq_lens, cu_new, device)
+    k, ldk, tokens = _kv8_rows(key, "key", device, kv_heads)
+    v, ldv, v_tokens = _kv8_rows(value, "value", device, kv_heads)
+    if v_tokens != tokens:
         raise ValueError("key and value: different numbers of rows")
     q = qo = None
     q_heads = ldq = ldqo = 0
     if query is not None:
-        _kv8_rows(query, "query", device)
+        q, ldq, q_tokens = _kv8_rows(query, "query", device)
+        q_heads = query.shape[1]
         if query_out is None:
-            query_out = torch.empty(query.shape, dtype=torch.bfloat16, device=device)
-        else:
-            _kv8_rows(query_out, "query_out", device, query.shape[1])
-        if query.shape[0] != tokens or query_out.shape[0] != tokens:
+            query_out = torch.empty(query.shape, dtype=torch.bfloat16, device=query.device)
+        qo, ldqo, o_tokens = _kv8_rows(query_out, "query_out", device, q_heads)
+        if q_tokens != tokens or o_tokens != tokens:
             raise ValueError("query, query_out: not as many rows as key")
-        q, qo, q_heads, ldq, ldqo = query.data_ptr(), query_out.data_ptr(), query.shape[1], query.stride(0), query_out.stride(0)
     elif query_out is not None:
         raise ValueError("query_out without query")
     if n == 0 or tokens == 0:
         return query_out
-    rc = _lib.load().glmasr_kv8_append(ctypes.byref(cache), key.data_ptr(), key.stride(0), value.data_ptr(), value.stride(0), q, ldq, qo, ldqo,
-                                       q_heads, block_tables.data_ptr(), block_tables.shape[1], seq_lens.data_ptr(), cu_new.data_ptr(),
-                                       n, tokens, theta)
-    if rc != 0:
+    if _lib.load().glmasr_kv8_append(cache, k, ldk, v, ldv, q, ldq, qo, ldqo, q_heads, block_tables.data_ptr(), max_blocks, seq_lens.data_ptr(),
+                                     cu_new.data_ptr(), n, tokens, theta) != 0:
         raise ValueError("glmasr_kv8_append rejected the arguments")
     return query_out
 
@@ -367,35 +373,34 @@ def kv8_attention(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
     window == 0, or p - j < window, or j < sinks; one that sees nothing gets zeros.  max_new / max_len: the most new tokens and
     the longest sequence to expect -- they choose kernels, not results (default: all rows / the table's width).  scale defaults to
     128 ** -0.5.  Rows behind cu_new[num_seqs] are left as they are.  out must not overlap query."""
-    cache, device = _kv8_cache(k_cache, v_cache, k_scale, v_scale)
-    n = _kv8_batch(block_tables, seq_lens, cu_new, device)
-    _kv8_rows(query, "query", device)
-    tokens, q_heads, _ = query.shape
-    if q_heads == 0 or q_heads % k_cache.shape[1] != 0:
+    cache, device, kv_heads, block_size = _kv8_cache(k_cache, v_cache, k_scale, v_scale)
+    n, max_blocks = _kv8_batch(block_tables, seq_lens, cu_new, device)
+    q, ldq, tokens = _kv8_rows(query, "query", device)
+    q_heads = query.shape[1]
+    if q_heads == 0 or q_heads % kv_heads != 0:
         raise ValueError("query: the head count must be a multiple of the cache's")
     if out is None:
-        out = torch.empty((tokens, q_heads, 128), dtype=torch.bfloat16, device=device)
-    else:
-        _kv8_rows(out, "out", device, q_heads)
-        if out.shape[0] != tokens:
-            raise ValueError("out: not as many rows as query")
-        if out.data_ptr() == query.data_ptr() and tokens > 0:
-            raise ValueError("out must not overlap query")
+        out = torch.empty((tokens, q_heads, 128), dtype=torch.bfloat16, device=query.device)
+    o, ldo, o_tokens = _kv8_rows(out, "out", device, q_heads)
+    if o_tokens != tokens:
+        raise ValueError("out: not as many rows as query")
+    if o == q and tokens > 0:
+        raise ValueError("out must not overlap query")
     if n == 0 or tokens == 0:
         return out
     lib = _lib.load()
-    size = lib.glmasr_kv8_attention_workspace()
-    workspace = torch.empty(size, dtype=torch.uint8, device=device)
-    rc = lib.glmasr_kv8_attention(out.data_ptr(), out.stride(0), query.data_ptr(), query.stride(0), ctypes.byref(cache),
-                                  block_tables.data_ptr(), block_tables.shape[1], seq_lens.data_ptr(), cu_new.data_ptr(), n, tokens,
-                                  q_heads, tokens if max_new is None else max_new,
-                                  block_tables.shape[1] * k_cache.shape[2] if max_len is None else max_len, window, sinks,
-                                  128 ** -0.5 if scale is None else scale, workspace.data_ptr(), size)
-    if rc != 0:
+    size = _kv8_workspace_bytes.get(device)
+    if size is None:
+        size = _kv8_workspace_bytes[device] = lib.glmasr_kv8_attention_workspace()
+    workspace = torch.empty(size, dtype=torch.uint8, device=query.device)
+    if lib.glmasr_kv8_attention(o, ldo, q, ldq, cache, block_tables.data_ptr(), max_blocks, seq_lens.data_ptr(), cu_new.data_ptr(), n, tokens, q_heads,
+                                tokens if max_new is None else max_new, max_blocks * block_size if max_len is None else max_len, window, sinks,
+                                _KV8_SCALE if scale is None else scale, workspace.data_ptr(), size) != 0:
         raise ValueError("glmasr_kv8_attention rejected the arguments")
-    used = _stream if _stream is not None else torch.cuda.default_stream(device)
-    if used.cuda_stream != torch.cuda.current_stream(device).cuda_stream:
-        workspace.record_stream(used)            # it came from another stream than the one that works on it
+    used = 0 if _stream is None else _stream.cuda_stream
+    if used != torch._C._cuda_getCurrentRawStream(device):
+        # the workspace came from another stream than the one that works on it
+        workspace.record_stream(torch.cuda.default_stream(device) if _stream is None else _stream)
     return out
 
 
