@@ -5,7 +5,7 @@
 // queries are the narrow one:
 //   S^T [128 tokens, rows] = K Q^T,    O^T [128 dims, rows] += V^T P^T      (tcgen05, e4m3 x e4m3, sums in fp32)
 // so no code is ever converted and no thread touches a key or a value.  (Warp-level products of the same formulas on converted
-// codes took 450 instructions per 32 tokens and warp, and 29 us where this kernel takes TIME_256 us for 256 sequences of 200 to 450 tokens.)
+// codes took 450 instructions per 32 tokens and warp, and 29 us where this kernel takes 24.6 us for 256 sequences of 200 to 450 tokens.)
 //   queries  A row is taken times a power of two that brings its largest element to 2^7 and split into two e4m3 numbers,
 //            q = hi + 2^-5 lo, side by side as columns: a bf16 number has 8 bits, each of them carries 4, so the split is exact for
 //            elements down to 2^-14 of the largest, and off by 2^-22 of the largest below.
@@ -218,9 +218,10 @@ __global__ void __launch_bounds__(THREADS, max_ctas(R)) kv8_attend_kernel(const 
     pdl_launch_dependents();          // after the wait: the join may look at the batch before its own
 
     // rows of the queries' operand that no row of a context fills stay zero
-    if (U < R && threadIdx.x < 4 * (R - U) * 8) {
-        const int row = (int)threadIdx.x / 8 % (R - U) + U + (threadIdx.x / 8 / (R - U) & 1 ? R : 0);
-        *reinterpret_cast<uint4 *>(sm.q[threadIdx.x / 8 / (R - U) / 2] + row * kKv8Dim + threadIdx.x % 8 * 16) = make_uint4(0u, 0u, 0u, 0u);
+    if constexpr (U < R) {
+        constexpr int SPARE = R - U;
+        const int i = (int)threadIdx.x / 8, row = i % SPARE + U + (i / SPARE & 1 ? R : 0);
+        if (i < 4 * SPARE) *reinterpret_cast<uint4 *>(sm.q[i / SPARE / 2] + row * kKv8Dim + threadIdx.x % 8 * 16) = make_uint4(0u, 0u, 0u, 0u);
         fence_proxy_async_smem();
     }
     int begin = 0, end = 0, quota = 1, seq0 = 0;          // the piece, and the sequence of its first unit
@@ -302,7 +303,7 @@ __global__ void __launch_bounds__(THREADS, max_ctas(R)) kv8_attend_kernel(const 
                     if (item < 0) {
                         item = (int)blockIdx.x;
                     } else {
-                        ok = mbar_wait_warp(bar(B_NEXT), (asked - 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION);
+                        ok = mbar_wait_short(bar(B_NEXT), (asked - 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION);
                         if (!ok) return false;
                         item = cancelled_cta(smem_u32(&sm.next));
                         if (item < 0) return false;
@@ -380,14 +381,14 @@ __global__ void __launch_bounds__(THREADS, max_ctas(R)) kv8_attend_kernel(const 
             const int s = (int)(t & 1u);
             const uint32_t free_phase = ((t >> 1) & 1u) ^ 1u, bytes = (uint32_t)__popc(__ballot_sync(0xFFFFFFFFu, place >= 0)) * GROUP_BYTES;
             ++t;
-            ok = mbar_wait_warp(bar(B_KEMPTY + s), free_phase, abort_word, ST_TIMEOUT_ATTENTION);
+            ok = mbar_wait_short(bar(B_KEMPTY + s), free_phase, abort_word, ST_TIMEOUT_ATTENTION);
             if (!ok) break;
             if (leader) mbar_expect_tx(bar(B_KFULL + s), bytes);
             __syncwarp();
             if (place >= 0) tma_load_2d(smem_u32(sm.k[s]) + lane * GROUP_BYTES, &p.tm_k, bar(B_KFULL + s), 0, place * kKv8Group);
             // V, and the scales: the tile of two before, whose places they take, has to be summed
             auto put_v = [&]() {
-                ok = mbar_wait_warp(bar(B_PVDONE + s), free_phase, abort_word, ST_TIMEOUT_ATTENTION);
+                ok = mbar_wait_short(bar(B_PVDONE + s), free_phase, abort_word, ST_TIMEOUT_ATTENTION);
                 if (!ok) return false;
                 if (leader) mbar_expect_tx(bar(B_VFULL + s), bytes);
                 __syncwarp();
@@ -406,7 +407,7 @@ __global__ void __launch_bounds__(THREADS, max_ctas(R)) kv8_attend_kernel(const 
                 continue;
             }
             const int cs = (int)(contexts & 1u);
-            ok = mbar_wait_warp(bar(B_CEMPTY + cs), ((contexts >> 1) & 1u) ^ 1u, abort_word, ST_TIMEOUT_ATTENTION);
+            ok = mbar_wait_short(bar(B_CEMPTY + cs), ((contexts >> 1) & 1u) ^ 1u, abort_word, ST_TIMEOUT_ATTENTION);
             if (!ok) break;
             ++contexts;
             ContextInfo<R> &info = sm.ctx[cs];
@@ -469,7 +470,7 @@ __global__ void __launch_bounds__(THREADS, max_ctas(R)) kv8_attend_kernel(const 
         }
         if (leader && !p.whole) p.part.join[blockIdx.x] = join;
         const int cs = (int)(contexts & 1u);
-        if (ok && mbar_wait_warp(bar(B_CEMPTY + cs), ((contexts >> 1) & 1u) ^ 1u, abort_word, ST_TIMEOUT_ATTENTION) && leader) {
+        if (ok && mbar_wait_short(bar(B_CEMPTY + cs), ((contexts >> 1) & 1u) ^ 1u, abort_word, ST_TIMEOUT_ATTENTION) && leader) {
             sm.ctx[cs].groups = 0;                            // the end
             mbar_arrive(bar(B_CFULL + cs));
         }
@@ -484,9 +485,9 @@ __global__ void __launch_bounds__(THREADS, max_ctas(R)) kv8_attend_kernel(const 
         // O^T of tile u: `steps` of 32 tokens; the first tile of a context overwrites the accumulator once the last result has been read
         auto weigh = [&](uint32_t u, int steps, bool first) {
             const int s = (int)(u & 1u);
-            if (!mbar_wait_warp(bar(B_VFULL + s), (u >> 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION)) return false;
-            if (!mbar_wait_warp(bar(B_PFULL), u & 1u, abort_word, ST_TIMEOUT_ATTENTION)) return false;
-            if (first && !mbar_wait_warp(bar(B_OFREE), ((contexts - 1) & 1u) ^ 1u, abort_word, ST_TIMEOUT_ATTENTION)) return false;
+            if (!mbar_wait_short(bar(B_VFULL + s), (u >> 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION)) return false;
+            if (!mbar_wait_short(bar(B_PFULL), u & 1u, abort_word, ST_TIMEOUT_ATTENTION)) return false;
+            if (first && !mbar_wait_short(bar(B_OFREE), ((contexts - 1) & 1u) ^ 1u, abort_word, ST_TIMEOUT_ATTENTION)) return false;
             tc_fence_after();
             if (leader) {
                 const uint64_t ad = smem_desc_sw128_mn(smem_u32(sm.v[s]), TILE_BYTES), bd = smem_desc_mn(smem_u32(sm.p), 16 * SOFTMAX);
@@ -499,7 +500,7 @@ __global__ void __launch_bounds__(THREADS, max_ctas(R)) kv8_attend_kernel(const 
         };
         while (ok) {
             const int cs = (int)(contexts & 1u);
-            if (!mbar_wait_warp(bar(B_CFULL + cs), (contexts >> 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION)) break;
+            if (!mbar_wait_short(bar(B_CFULL + cs), (contexts >> 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION)) break;
             const int groups_here = sm.ctx[cs].groups, n = (groups_here + TILE_GROUPS - 1) / TILE_GROUPS;
             if (n == 0) break;
             ++contexts;
@@ -507,7 +508,7 @@ __global__ void __launch_bounds__(THREADS, max_ctas(R)) kv8_attend_kernel(const 
                 if (j < n) {
                     const int s = (int)(t & 1u);
                     // the score buffer is free: the weights of two tiles ago came after its last read, and their product was issued
-                    if (!mbar_wait_warp(bar(B_KFULL + s), (t >> 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION)) { ok = false; break; }
+                    if (!mbar_wait_short(bar(B_KFULL + s), (t >> 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION)) { ok = false; break; }
                     tc_fence_after();
                     if (leader) {
                         const uint64_t ad = smem_desc_sw128(smem_u32(sm.k[s])), bd = smem_desc_sw128(smem_u32(sm.q[cs]));
@@ -536,7 +537,7 @@ __global__ void __launch_bounds__(THREADS, max_ctas(R)) kv8_attend_kernel(const 
         uint32_t t = 0;
         for (uint32_t contexts = 0;; ++contexts) {
             const int cs = (int)(contexts & 1u);
-            bool ok = mbar_wait_warp(bar(B_CFULL + cs), (contexts >> 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION);
+            bool ok = mbar_wait_short(bar(B_CFULL + cs), (contexts >> 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION);
             const ContextInfo<R> &c = sm.ctx[cs];
             const int n = (c.groups + TILE_GROUPS - 1) / TILE_GROUPS;
             const int pos_lo = c.pos_lo, pos_hi = c.pos_hi;
@@ -547,14 +548,14 @@ __global__ void __launch_bounds__(THREADS, max_ctas(R)) kv8_attend_kernel(const 
             if (any_of_softmax(!ok) || n == 0) break;
             for (int j = 0; j < n; ++j, ++t) {
                 const int s = (int)(t & 1u);
-                ok = mbar_wait_warp(bar(B_SCALES + s), (t >> 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION);
+                ok = mbar_wait_short(bar(B_SCALES + s), (t >> 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION);
                 const int in = c.first + j * TILE_GROUPS + me / kKv8Group;
                 const int tok = (in < c.sink ? in : c.from + (in - c.sink)) * kKv8Group + me % kKv8Group;
                 const bool there = me % kKv8Group < sm.tokens[s][me / kKv8Group];
                 const float2 sc = sm.scales[s][me / kKv8Group];
                 const float vs = lg2(sc.y);
                 const bool all = there && tok <= pos_lo && (a.window == 0 || pos_hi - tok < a.window || tok < a.sinks);
-                ok = ok && mbar_wait_warp(bar(B_SFULL + s), (t >> 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION);
+                ok = ok && mbar_wait_short(bar(B_SFULL + s), (t >> 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION);
                 tc_fence_after();
                 float x[U];
                 uint32_t raw[N];
@@ -586,7 +587,7 @@ __global__ void __launch_bounds__(THREADS, max_ctas(R)) kv8_attend_kernel(const 
                         if (lane == 0) *reinterpret_cast<float2 *>(sm.red[warp][r]) = make_float2(m, w);
                     }
                     // the accumulator is expressed against the new W: the product before has to be complete
-                    if (j > 0) ok = ok && mbar_wait_warp(bar(B_PVDONE + (int)((t - 1) & 1u)), ((t - 1) >> 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION);
+                    if (j > 0) ok = ok && mbar_wait_short(bar(B_PVDONE + (int)((t - 1) & 1u)), ((t - 1) >> 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION);
                     if (any_of_softmax(!ok)) { ok = false; break; }
                     if (me < U) {
                         const float4 was = sm.row[me];
@@ -630,10 +631,10 @@ __global__ void __launch_bounds__(THREADS, max_ctas(R)) kv8_attend_kernel(const 
                     w8[(R + r) / 4] |= lo << (8 * (r & 2));
                 }
                 // the weights of the tile before have been read
-                ok = t == 0 || mbar_wait_warp(bar(B_PVDONE + (s ^ 1)), ((t - 1) >> 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION);
+                ok = t == 0 || mbar_wait_short(bar(B_PVDONE + (s ^ 1)), ((t - 1) >> 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION);
                 // a token that does not exist weighs 0, but what lies in its place may be anything, and 0 * NaN is not 0
                 if (__any_sync(0xFFFFFFFFu, !there)) {
-                    ok = ok && mbar_wait_warp(bar(B_VFULL + s), (t >> 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION);
+                    ok = ok && mbar_wait_short(bar(B_VFULL + s), (t >> 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION);
                     if (!there) {
 #pragma unroll
                         for (int i = 0; i < 8; ++i)
@@ -651,7 +652,7 @@ __global__ void __launch_bounds__(THREADS, max_ctas(R)) kv8_attend_kernel(const 
             }
 
             // ---- the result of these groups ----
-            ok = ok && mbar_wait_warp(bar(B_PVDONE + (int)((t - 1) & 1u)), ((t - 1) >> 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION);
+            ok = ok && mbar_wait_short(bar(B_PVDONE + (int)((t - 1) & 1u)), ((t - 1) >> 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION);
             // sums over the warp's 32 tokens: halves of the rows are exchanged until a lane has one, then the lanes that share it add up
             {
                 constexpr int P2 = U <= 4 ? 4 : U <= 8 ? 8 : U <= 16 ? 16 : 32;

@@ -5,7 +5,8 @@
 //                     element to 2^7 and split into two e4m3 numbers, q = hi + lo, both products into the same sums: exact for
 //                     elements down to 2^-9 of the largest, off by 2^-17 of the largest below.  Two products of 8-bit operands
 //                     cost what one of 16-bit operands does, and no key is converted.
-//   p = 2^(x - m)     x = s * (row scale) * (K scale of the block of 16 keys); m is touched when a row's maximum has grown past 2^8 m.
+//   p = 2^(x - m)     x = s * (row scale) * (K scale of the block of 16 keys), in one pass over the scores: m is what the steps before
+//                     left, and moves when weights get too large for it.
 //   O += P V          f16 x f16: weights have 11 bits down to 2^-14 of the largest, and are off by 2^-25 of it below.  V's codes become
 //                     f16, times the scale of their block over the largest scale of the item so far (exact: a power of two),
 //                     which O is expressed against.  From the first block on whose scale is 2^5 below that one, small weights
@@ -13,10 +14,13 @@
 // Bound: the two products are 2 x 128 x 128 x 128 multiply-adds a step, 1024 cycles at the tensor cores' nominal rate, and the
 // exponentials 1024 of the special-function units, under each other in the best case.  A step is a chain (scores, softmax, weighted
 // sum), so two CTAs share an SM and one's softmax runs under the other's products.
-//   warp 8      producer: the work items, K tiles (a TMA box of 2 KB per group of 16 keys), pages and scales of each step
+//   warp 8      producer: the work items, K and V tiles (a TMA box of 2 KB per group of 16 keys), pages and scales of each step
 //   warp 9      products; scores [0, 128) and output [128, 256) of tensor memory, P as f16 over the scores it was made from
-//   warps 4-7   queries of an item, V of a step: from global memory, converted, to shared memory
-//   warps 0-3   softmax: thread = row = lane of tensor memory
+//   warps 4-7   V of a step as f16 (or bf16)
+//   warps 0-3   softmax: thread = row = lane of tensor memory; it also brings its row of queries, which for the next item are on their
+//               way while the last sum of the present one is waited for
+// (warps 10 and 11 only give their registers to the softmax.)  The loops are kept rolled up: fully unrolled, the kernel was 92 KB of code
+// and its softmax waited for instructions, 3700 cycles a step instead of 2800 (491 us instead of 383 for two sequences of 2000 new tokens behind 5000).
 // The grid has a CTA for every work item there could be; those that run take over the items of those that have not started.
 // The last tiles of a sequence, which see most keys, come first.
 #include <math.h>
@@ -31,14 +35,16 @@ static __device__ int g_kv8_prefill_status[4];
 
 namespace {
 
-constexpr int QT = 128, KT = 128, THREADS = 320;
+constexpr int QT = 128, KT = 128, THREADS = 384;
+// Registers of a thread by warpgroup: two CTAs share an SM, 80 each at launch, and 144 + 56 + 40 = 3 x 80.
+constexpr int REGS_SOFTMAX = 152, REGS_VALUES = 48, REGS_REST = 40;
 constexpr int GROUPS = KT / kKv8Group, GROUP_BYTES = kKv8Group * kKv8Dim;
 constexpr int TMEM_COLS = 256, COL_O = 128;
-constexpr float kLazy = 8.0f;                 // log2: P may grow to 2^8
+constexpr float kLazy = 8.0f, kFar = 15.0f;   // log2: weights of 2^8 move the reference with the next step, of 2^15 (f16 ends at 2^16) at once
 constexpr float kF16Range = 1.0f / 32.0f;     // of V scales
 
-enum : int { B_KFULL = 0, B_KEMPTY = 2, B_STEP = 4, B_PVDONE = 6, B_INFO = 8, B_INFOFREE = 10, B_SFULL = 12, B_PFULL = 13, B_VFULL = 14, B_QFULL = 15,
-             B_OFREE = 16, B_NEXT = 17, B_COUNT = 18 };
+enum : int { B_KFULL = 0, B_KEMPTY, B_RFULL, B_REMPTY, B_VFULL, B_SFULL, B_PFULL, B_QFULL, B_OFREE, B_NEXT, B_STEP, B_PVDONE = B_STEP + 2, B_INFO = B_PVDONE + 2,
+             B_INFOFREE = B_INFO + 2, B_COUNT = B_INFOFREE + 2 };
 
 struct ItemInfo {
     int rows;                                 // query rows that exist; 0: no more work
@@ -46,9 +52,10 @@ struct ItemInfo {
     int start;                                // position of the sequence's first new token
 };
 struct StepInfo {
-    int place[GROUPS], tokens[GROUPS];        // of each group of 16 keys: in the pool (-1: none), keys of it that exist
+    int tokens[GROUPS];                       // keys of each group of 16 that exist
     int key[GROUPS];                          // first position
-    float ks[GROUPS], vmul[GROUPS];           // K scale; V scale over vref
+    alignas(16) float ks[GROUPS];             // K scale
+    float vmul[GROUPS];                       // V scale over vref
     float vref, vstep;                        // the largest V scale so far, and the one before over it
     int plain;                                // every row sees every key
     int wide;                                 // bf16
@@ -56,9 +63,8 @@ struct StepInfo {
 };
 struct Smem {
     uint8_t q[2][QT * kKv8Dim];               // hi, lo
-    uint8_t k[2][KT * kKv8Dim];
+    uint8_t k[KT * kKv8Dim], raw[KT * kKv8Dim];       // codes of K and V
     uint8_t v[2][KT * 128];                   // f16, two boxes of 64 dims
-    float qscale[QT];
     ItemInfo item[2];
     StepInfo step[2];
     uint4 next;
@@ -68,7 +74,7 @@ struct Smem {
 };
 
 struct Params {
-    CUtensorMap tm_k;
+    CUtensorMap tm_k, tm_v;
     Kv8Attend a;
     int tiles;                                // row tiles there could be, all sequences
 };
@@ -87,6 +93,43 @@ __device__ __forceinline__ uint32_t f16_codes(uint32_t w, bool high) {
     return r;
 }
 
+// This lane's 128 output columns times f.
+__device__ __forceinline__ void scale_columns(uint32_t t_o, float f) {
+#pragma unroll 1
+    for (int c = 0; c < 8; ++c) {
+        uint32_t o[16];
+        tmem_ld_x16(t_o + (uint32_t)c * 16, o);
+        tmem_ld_wait();
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+        tmem_st_x16(t_o + (uint32_t)c * 16, o);
+    }
+}
+
+// The weights in this lane's first n columns times f.
+__device__ __forceinline__ void scale_weights(uint32_t t_row, int n, float f, bool wide) {
+    tmem_st_wait();
+#pragma unroll 1
+    for (int c = 0; c < n; c += 8) {
+        uint32_t w[8];
+        tmem_ld_x8(t_row + (uint32_t)c, w);
+        tmem_ld_wait();
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            float2 v;
+            if (wide) v = make_float2(__uint_as_float(w[e] << 16), __uint_as_float(w[e] & 0xFFFF0000u));
+            else v = __half22float2(*reinterpret_cast<const __half2 *>(&w[e]));
+            w[e] = wide ? pack2(v.x * f, v.y * f) : pack2_f16(v.x * f, v.y * f);
+        }
+        tmem_st_x8(t_row + (uint32_t)c, w);
+    }
+}
+
+template <int N>
+__device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
 __global__ void __launch_bounds__(THREADS, 2) kv8_prefill_kernel(const __grid_constant__ Params p) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     Smem &sm = *reinterpret_cast<Smem *>(smem_raw);
@@ -98,23 +141,26 @@ __global__ void __launch_bounds__(THREADS, 2) kv8_prefill_kernel(const __grid_co
         return;
     }
     if (threadIdx.x == 0) {
+        mbar_init(bar(B_KFULL), 1);
+        mbar_init(bar(B_KEMPTY), 1);
+        mbar_init(bar(B_RFULL), 1);
+        mbar_init(bar(B_REMPTY), 128);
+        mbar_init(bar(B_VFULL), 128);
+        mbar_init(bar(B_SFULL), 1);
+        mbar_init(bar(B_PFULL), 128);
+        mbar_init(bar(B_QFULL), 128);
+        mbar_init(bar(B_OFREE), 128);
+        mbar_init(bar(B_NEXT), 1);
         for (int i = 0; i < 2; ++i) {
-            mbar_init(bar(B_KFULL + i), 1);
-            mbar_init(bar(B_KEMPTY + i), 1);
             mbar_init(bar(B_STEP + i), 1);
             mbar_init(bar(B_PVDONE + i), 1);
             mbar_init(bar(B_INFO + i), 1);
             mbar_init(bar(B_INFOFREE + i), 128 + 128 + 1);
         }
-        mbar_init(bar(B_SFULL), 1);
-        mbar_init(bar(B_PFULL), 128);
-        mbar_init(bar(B_VFULL), 128);
-        mbar_init(bar(B_QFULL), 128);
-        mbar_init(bar(B_OFREE), 128);
-        mbar_init(bar(B_NEXT), 1);
         sm.abort = 0;
         fence_mbar_init();
         tma_prefetch_desc(&p.tm_k);
+        tma_prefetch_desc(&p.tm_v);
     }
     if (warp == 9) {
         tmem_alloc(smem_u32(&sm.tmem), TMEM_COLS);
@@ -128,240 +174,202 @@ __global__ void __launch_bounds__(THREADS, 2) kv8_prefill_kernel(const __grid_co
     pdl_wait();                                               // nothing above touched global memory
     pdl_launch_dependents();
 
-    if (warp == 8) {
-        // ================================ producer ================================
-        const bool leader = elect_one();
-        const int *cu = a.b.cu_new;
-        uint32_t t = 0, items = 0, asked = 0;                 // steps and items started, answers had
-        bool ok = true;
-        int work = (int)blockIdx.x;
-        while (ok) {
-            if (leader) {                                     // the item after this one
-                mbar_expect_tx(bar(B_NEXT), 16);
-                ask_cancelled_cta(smem_u32(&sm.next), bar(B_NEXT));
-            }
-            __syncwarp();
-            const int y0 = a.b.by_kv_heads.div(work), head = work - y0 * a.b.kv_heads, y = p.tiles - 1 - y0;
-            // sequence s has the tiles from cu_new[s] * group / 128 + s on: a bound that needs no pass over the lengths
-            const int seq = warp_last_not_above(a.b.num_seqs, (long long)y, [&](int s) { return (((long long)cu[s] * a.group) >> 7) + s; });
-            int rows = 0, tile = 0, row0 = 0, n = 0, start = 0, len = 0;
-            if (seq >= 0) {
-                row0 = cu[seq];
-                const int end = cu[seq + 1];
-                n = row0 < 0 ? 0 : max(0, min(end, a.b.total_new) - row0);
-                len = a.b.seq_lens[seq];
-                start = len - (end - row0);
-                tile = y - (int)(((long long)row0 * a.group) >> 7) - seq;
-                rows = min(QT, n * a.group - tile * QT);
-            }
-            if (rows > 0) {
-                const int pos_lo = start + a.by_group.div(tile * QT), pos_hi = start + a.by_group.div(tile * QT + rows - 1);
-                const Kv8Span span = kv8_span(a, len, pos_lo, pos_hi);
-                const int steps = (span.count + GROUPS - 1) / GROUPS;
-                const int is = (int)(items & 1u);
-                ok = mbar_wait_warp(bar(B_INFOFREE + is), ((items >> 1) & 1u) ^ 1u, abort_word, ST_TIMEOUT_ATTENTION);
-                if (!ok) break;
-                if (leader) {
-                    sm.item[is] = {rows, steps, head, tile * QT, row0, start};
-                    mbar_arrive(bar(B_INFO + is));
+    if (warp >= 8) {
+        fewer_registers<REGS_REST>();           // the whole warpgroup, before its warps part
+        if (warp == 8) {
+            // ================================ producer ================================
+            const bool leader = elect_one();
+            const int *cu = a.b.cu_new;
+            uint32_t t = 0, items = 0, asked = 0;                 // steps and items started, answers had
+            bool ok = true;
+            int work = (int)blockIdx.x;
+            while (ok) {
+                if (leader) {                                     // the item after this one
+                    mbar_expect_tx(bar(B_NEXT), 16);
+                    ask_cancelled_cta(smem_u32(&sm.next), bar(B_NEXT));
                 }
                 __syncwarp();
-                ++items;
-                float vref = 0.0f;
-                bool wide = false;
-                for (int g = 0; g < span.count; g += GROUPS, ++t) {
-                    const int s = (int)(t & 1u);
-                    const uint32_t free_phase = ((t >> 1) & 1u) ^ 1u;
-                    int place = -1, tokens = 0, key = 0;
-                    float ks = 0.0f, vs = 0.0f;
-                    if (lane < GROUPS && g + lane < span.count) {
-                        const int group = span.group_of(g + lane);
-                        key = group * kKv8Group;
-                        const long long row = kv8_group_row(a.b, seq, head, group);
-                        if (row >= 0) {
-                            place = (int)(row / kKv8Group);
-                            tokens = min(kKv8Group, len - key);
-                            ks = a.k_scale[place];
-                            vs = a.v_scale[place];
+                const int y0 = a.b.by_kv_heads.div(work), head = work - y0 * a.b.kv_heads, y = p.tiles - 1 - y0;
+                // sequence s has the tiles from cu_new[s] * group / 128 + s on: a bound that needs no pass over the lengths
+                const int seq = warp_last_not_above(a.b.num_seqs, (long long)y, [&](int s) { return (((long long)cu[s] * a.group) >> 7) + s; });
+                int rows = 0, tile = 0, row0 = 0, n = 0, start = 0, len = 0;
+                if (seq >= 0) {
+                    row0 = cu[seq];
+                    const int end = cu[seq + 1];
+                    n = row0 < 0 ? 0 : max(0, min(end, a.b.total_new) - row0);
+                    len = a.b.seq_lens[seq];
+                    start = len - (end - row0);
+                    tile = y - (int)(((long long)row0 * a.group) >> 7) - seq;
+                    rows = min(QT, n * a.group - tile * QT);
+                }
+                if (rows > 0) {
+                    const int pos_lo = start + a.by_group.div(tile * QT), pos_hi = start + a.by_group.div(tile * QT + rows - 1);
+                    const Kv8Span span = kv8_span(a, len, pos_lo, pos_hi);
+                    const int steps = (span.count + GROUPS - 1) / GROUPS;
+                    const int is = (int)(items & 1u);
+                    ok = mbar_wait_short(bar(B_INFOFREE + is), ((items >> 1) & 1u) ^ 1u, abort_word, ST_TIMEOUT_ATTENTION);
+                    if (!ok) break;
+                    if (leader) {
+                        sm.item[is] = {rows, steps, head, tile * QT, row0, start};
+                        mbar_arrive(bar(B_INFO + is));
+                    }
+                    __syncwarp();
+                    ++items;
+                    float vref = 0.0f;
+                    bool wide = false;
+                    for (int g = 0; g < span.count; g += GROUPS, ++t) {
+                        const int s = (int)(t & 1u);
+                        const uint32_t free_phase = (t & 1u) ^ 1u;
+                        int place = -1, tokens = 0, key = 0;
+                        float ks = 0.0f, vs = 0.0f;
+                        if (lane < GROUPS && g + lane < span.count) {
+                            const int group = span.group_of(g + lane);
+                            key = group * kKv8Group;
+                            const long long row = kv8_group_row(a.b, seq, head, group);
+                            if (row >= 0) {
+                                place = (int)(row / kKv8Group);
+                                tokens = min(kKv8Group, len - key);
+                                ks = a.k_scale[place];
+                                vs = a.v_scale[place];
+                            }
                         }
-                    }
-                    const uint32_t bytes = (uint32_t)__popc(__ballot_sync(0xFFFFFFFFu, place >= 0)) * GROUP_BYTES;
-                    ok = mbar_wait_warp(bar(B_KEMPTY + s), free_phase, abort_word, ST_TIMEOUT_ATTENTION);
-                    if (!ok) break;
-                    if (leader) mbar_expect_tx(bar(B_KFULL + s), bytes);
-                    __syncwarp();
-                    if (place >= 0) tma_load_2d(smem_u32(sm.k[s]) + lane * GROUP_BYTES, &p.tm_k, bar(B_KFULL + s), 0, place * kKv8Group);
-                    const bool number = vs >= 0.0f && vs <= 3.4028234664e38f;
-                    float most = number ? vs : 0.0f;
+                        const uint32_t bytes = (uint32_t)__popc(__ballot_sync(0xFFFFFFFFu, place >= 0)) * GROUP_BYTES;
+                        ok = mbar_wait_short(bar(B_KEMPTY), free_phase, abort_word, ST_TIMEOUT_ATTENTION);
+                        if (!ok) break;
+                        if (leader) mbar_expect_tx(bar(B_KFULL), bytes);
+                        __syncwarp();
+                        if (place >= 0) tma_load_2d(smem_u32(sm.k) + lane * GROUP_BYTES, &p.tm_k, bar(B_KFULL), 0, place * kKv8Group);
+                        ok = mbar_wait_short(bar(B_REMPTY), free_phase, abort_word, ST_TIMEOUT_ATTENTION);
+                        if (!ok) break;
+                        if (leader) mbar_expect_tx(bar(B_RFULL), bytes);
+                        __syncwarp();
+                        if (place >= 0) tma_load_2d(smem_u32(sm.raw) + lane * GROUP_BYTES, &p.tm_v, bar(B_RFULL), 0, place * kKv8Group);
+                        const bool number = vs >= 0.0f && vs <= 3.4028234664e38f;
+                        float most = number ? vs : 0.0f;
 #pragma unroll
-                    for (int d = 1; d < GROUPS; d <<= 1) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, d));
-                    most = fmaxf(most, vref);
-                    const float vmul = number && most > 0.0f ? vs / most : 0.0f;
-                    const bool plain_here = tokens == kKv8Group && key + kKv8Group - 1 <= pos_lo &&
-                                            (a.window == 0 || pos_hi - key < a.window || key + kKv8Group <= a.sinks);
-                    const bool mine = lane < GROUPS;
-                    const uint32_t plain = __ballot_sync(0xFFFFFFFFu, mine && plain_here), far = __ballot_sync(0xFFFFFFFFu, mine && vs > 0x1p-126f && vmul < kF16Range && number);
-                    wide = wide || far != 0u;
-                    const uint32_t poisoned = __ballot_sync(0xFFFFFFFFu, mine && !number);
-                    // the step two before, whose place this is, has been summed: softmax and V are done with it
-                    ok = mbar_wait_warp(bar(B_PVDONE + s), free_phase, abort_word, ST_TIMEOUT_ATTENTION);
+                        for (int d = 1; d < GROUPS; d <<= 1) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, d));
+                        most = fmaxf(most, vref);
+                        const float vmul = number && most > 0.0f ? vs / most : 0.0f;
+                        const bool plain_here = tokens == kKv8Group && key + kKv8Group - 1 <= pos_lo &&
+                                                (a.window == 0 || pos_hi - key < a.window || key + kKv8Group <= a.sinks);
+                        const bool mine = lane < GROUPS;
+                        const uint32_t plain = __ballot_sync(0xFFFFFFFFu, mine && plain_here), far = __ballot_sync(0xFFFFFFFFu, mine && vs > 0x1p-126f && vmul < kF16Range && number);
+                        wide = wide || far != 0u;
+                        const uint32_t poisoned = __ballot_sync(0xFFFFFFFFu, mine && !number);
+                        // the step two before, whose place this is, has been summed: softmax and V are done with it
+                        ok = mbar_wait_short(bar(B_PVDONE + s), ((t >> 1) & 1u) ^ 1u, abort_word, ST_TIMEOUT_ATTENTION);
+                        if (!ok) break;
+                        StepInfo &st = sm.step[s];
+                        if (mine) {
+                            st.tokens[lane] = tokens, st.key[lane] = key;
+                            st.ks[lane] = ks, st.vmul[lane] = vmul;
+                        }
+                        if (lane == 0) {
+                            st.vref = most;
+                            st.vstep = most > 0.0f ? vref / most : 1.0f;
+                            st.plain = plain == (1u << GROUPS) - 1u ? 1 : 0;
+                            st.wide = wide ? 1 : 0;
+                            st.poisoned = poisoned;
+                        }
+                        __syncwarp();
+                        if (leader) mbar_arrive(bar(B_STEP + s));
+                        vref = most;
+                    }
                     if (!ok) break;
-                    StepInfo &st = sm.step[s];
-                    if (mine) {
-                        st.place[lane] = place, st.tokens[lane] = tokens, st.key[lane] = key;
-                        st.ks[lane] = ks, st.vmul[lane] = vmul;
-                    }
-                    if (lane == 0) {
-                        st.vref = most;
-                        st.vstep = most > 0.0f ? vref / most : 1.0f;
-                        st.plain = plain == (1u << GROUPS) - 1u ? 1 : 0;
-                        st.wide = wide ? 1 : 0;
-                        st.poisoned = poisoned;
-                    }
-                    __syncwarp();
-                    if (leader) mbar_arrive(bar(B_STEP + s));
-                    vref = most;
                 }
+                ok = mbar_wait_short(bar(B_NEXT), asked & 1u, abort_word, ST_TIMEOUT_ATTENTION);
                 if (!ok) break;
+                ++asked;
+                work = cancelled_cta(smem_u32(&sm.next));
+                fence_proxy_async_smem();                         // the answer has been read before the next one is written
+                __syncwarp();
+                if (work < 0) break;
             }
-            ok = mbar_wait_warp(bar(B_NEXT), asked & 1u, abort_word, ST_TIMEOUT_ATTENTION);
-            if (!ok) break;
-            ++asked;
-            work = cancelled_cta(smem_u32(&sm.next));
-            fence_proxy_async_smem();                         // the answer has been read before the next one is written
-            __syncwarp();
-            if (work < 0) break;
-        }
-        const int is = (int)(items & 1u);
-        if (ok && mbar_wait_warp(bar(B_INFOFREE + is), ((items >> 1) & 1u) ^ 1u, abort_word, ST_TIMEOUT_ATTENTION) && leader) {
-            sm.item[is].rows = 0;                             // the end
-            mbar_arrive(bar(B_INFO + is));
-        }
-    } else if (warp == 9) {
-        // ================================ products ================================
-        const bool leader = elect_one();
-        constexpr uint32_t idesc_s = idesc_e4m3(QT, KT);
-        const uint32_t t_o = tmem + COL_O;
-        uint32_t t = 0, items = 0, worked = 0;                // worked: items with any step
-        bool ok = true;
-        while (ok) {
             const int is = (int)(items & 1u);
-            if (!mbar_wait_warp(bar(B_INFO + is), (items >> 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION)) break;
-            const int rows = sm.item[is].rows, steps = sm.item[is].steps;
-            if (rows == 0) break;
-            ++items;
-            __syncwarp();
-            if (leader) mbar_arrive(bar(B_INFOFREE + is));
-            if (steps == 0) continue;
-            if (!mbar_wait_warp(bar(B_QFULL), worked & 1u, abort_word, ST_TIMEOUT_ATTENTION)) break;
-            for (int j = 0; j < steps; ++j, ++t) {
-                const int s = (int)(t & 1u);
-                ok = mbar_wait_warp(bar(B_KFULL + s), (t >> 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION);
-                // the scores take the place of the weights of the step before
-                ok = ok && (t == 0 || mbar_wait_warp(bar(B_PVDONE + (s ^ 1)), ((t - 1) >> 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION));
-                if (!ok) break;
-                tc_fence_after();
-                if (leader) {
-                    const uint64_t bd = smem_desc_sw128(smem_u32(sm.k[s]));
-#pragma unroll
-                    for (int k = 0; k < 8; ++k)
-                        umma_f8(tmem, smem_desc_sw128(smem_u32(sm.q[k >> 2])) + (uint64_t)(((k & 3) * 32) >> 4), bd + (uint64_t)(((k & 3) * 32) >> 4), idesc_s, k > 0 ? 1u : 0u);
-                    umma_commit(bar(B_KEMPTY + s));
-                    umma_commit(bar(B_SFULL));
-                }
-                __syncwarp();
-                ok = mbar_wait_warp(bar(B_VFULL), t & 1u, abort_word, ST_TIMEOUT_ATTENTION) && mbar_wait_warp(bar(B_PFULL), t & 1u, abort_word, ST_TIMEOUT_ATTENTION);
-                // the first weighted sum of an item overwrites the output of the item before
-                if (ok && j == 0) ok = mbar_wait_warp(bar(B_OFREE), (worked & 1u) ^ 1u, abort_word, ST_TIMEOUT_ATTENTION);
-                if (!ok) break;
-                tc_fence_after();
-                const bool wide = sm.step[s].wide != 0;
-                if (leader) {
-                    const uint64_t bd = smem_desc_sw128_mn(smem_u32(sm.v[0]), KT * 128);
-                    const uint32_t idesc_o = wide ? idesc_bf16(QT, kKv8Dim) | kIdescBMnMajor : kIdescF16;
-#pragma unroll
-                    for (int k = 0; k < KT / 16; ++k)
-                        umma_bf16_ts(t_o, tmem + (uint32_t)k * 8, bd + (uint64_t)((k * 2048) >> 4), idesc_o, j > 0 || k > 0 ? 1u : 0u);
-                    umma_commit(bar(B_PVDONE + s));
-                }
-                __syncwarp();
+            if (ok && mbar_wait_short(bar(B_INFOFREE + is), ((items >> 1) & 1u) ^ 1u, abort_word, ST_TIMEOUT_ATTENTION) && leader) {
+                sm.item[is].rows = 0;                             // the end
+                mbar_arrive(bar(B_INFO + is));
             }
-            ++worked;
+        } else if (warp == 9) {
+            // ================================ products ================================
+            const bool leader = elect_one();
+            constexpr uint32_t idesc_s = idesc_e4m3(QT, KT);
+            const uint32_t t_o = tmem + COL_O;
+            uint32_t t = 0, items = 0, worked = 0;                // worked: items with any step
+            bool ok = true;
+            while (ok) {
+                const int is = (int)(items & 1u);
+                if (!mbar_wait_short(bar(B_INFO + is), (items >> 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION)) break;
+                const int rows = sm.item[is].rows, steps = sm.item[is].steps;
+                if (rows == 0) break;
+                ++items;
+                __syncwarp();
+                if (leader) mbar_arrive(bar(B_INFOFREE + is));
+                if (steps == 0) continue;
+                if (!mbar_wait_short(bar(B_QFULL), worked & 1u, abort_word, ST_TIMEOUT_ATTENTION)) break;
+                for (int j = 0; j < steps; ++j, ++t) {
+                    const int s = (int)(t & 1u);
+                    ok = mbar_wait_short(bar(B_KFULL), t & 1u, abort_word, ST_TIMEOUT_ATTENTION);
+                    // the scores take the place of the weights of the step before
+                    ok = ok && (t == 0 || mbar_wait_short(bar(B_PVDONE + (s ^ 1)), ((t - 1) >> 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION));
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (leader) {
+                        const uint64_t bd = smem_desc_sw128(smem_u32(sm.k));
+#pragma unroll
+                        for (int k = 0; k < 8; ++k)
+                            umma_f8(tmem, smem_desc_sw128(smem_u32(sm.q[k >> 2])) + (uint64_t)(((k & 3) * 32) >> 4), bd + (uint64_t)(((k & 3) * 32) >> 4), idesc_s, k > 0 ? 1u : 0u);
+                        umma_commit(bar(B_KEMPTY));
+                        umma_commit(bar(B_SFULL));
+                    }
+                    __syncwarp();
+                    ok = mbar_wait_short(bar(B_VFULL), t & 1u, abort_word, ST_TIMEOUT_ATTENTION) && mbar_wait_short(bar(B_PFULL), t & 1u, abort_word, ST_TIMEOUT_ATTENTION);
+                    // the first weighted sum of an item overwrites the output of the item before
+                    if (ok && j == 0) ok = mbar_wait_short(bar(B_OFREE), (worked & 1u) ^ 1u, abort_word, ST_TIMEOUT_ATTENTION);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const bool wide = sm.step[s].wide != 0;
+                    if (leader) {
+                        const uint64_t bd = smem_desc_sw128_mn(smem_u32(sm.v[0]), KT * 128);
+                        const uint32_t idesc_o = wide ? idesc_bf16(QT, kKv8Dim) | kIdescBMnMajor : kIdescF16;
+#pragma unroll
+                        for (int k = 0; k < KT / 16; ++k)
+                            umma_bf16_ts(t_o, tmem + (uint32_t)k * 8, bd + (uint64_t)((k * 2048) >> 4), idesc_o, j > 0 || k > 0 ? 1u : 0u);
+                        umma_commit(bar(B_PVDONE + s));
+                    }
+                    __syncwarp();
+                }
+                ++worked;
+            }
         }
     } else if (warp >= 4) {
-        // ================================ queries and V ================================
+        // ================================ V ================================
+        fewer_registers<REGS_VALUES>();
         const int w4 = warp - 4, chunk = lane & 7, in_group = w4 * 4 + (lane >> 3);       // a thread has 16 dims of one key of each group
+        const uint32_t src = smem_u32(sm.raw) + (uint32_t)(in_group * kKv8Dim + ((chunk ^ (in_group & 7)) << 4));
+        const uint32_t dst = smem_u32(sm.v[chunk >> 2]) + (uint32_t)(in_group * 128), c0 = (uint32_t)(((chunk & 3) * 2) ^ (in_group & 7)) << 4;
         uint32_t t = 0, items = 0;
         bool ok = true;
         while (ok) {
             const int is = (int)(items & 1u);
-            if (!mbar_wait_warp(bar(B_INFO + is), (items >> 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION)) break;
-            const ItemInfo info = sm.item[is];
-            if (info.rows == 0) break;
+            if (!mbar_wait_short(bar(B_INFO + is), (items >> 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION)) break;
+            const int rows = sm.item[is].rows, steps = sm.item[is].steps;
+            if (rows == 0) break;
             ++items;
             mbar_arrive(bar(B_INFOFREE + is));
-            if (info.steps == 0) continue;
-            uint4 v[GROUPS];
-            auto ask = [&](uint32_t u) {
-                const StepInfo &st = sm.step[u & 1u];
-#pragma unroll
-                for (int i = 0; i < GROUPS; ++i) {
-                    v[i] = make_uint4(0u, 0u, 0u, 0u);        // behind the end may be anything: zeros instead
-                    if (in_group < st.tokens[i]) v[i] = *reinterpret_cast<const uint4 *>(a.v_cache + ((size_t)st.place[i] * kKv8Group + in_group) * kKv8Dim + chunk * 16);
-                }
-            };
-            // queries, four lanes per row: the tile before has been used when the last weighted sum is done
-            if (t > 0 && !mbar_wait_warp(bar(B_PVDONE + (int)((t - 1) & 1u)), ((t - 1) >> 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION)) break;
-#pragma unroll 2
-            for (int pass = 0; pass < 4; ++pass) {
-                const int r = w4 * 32 + pass * 8 + (lane >> 2), row = info.row0 + r, tok = a.by_group.div(row);
-                const __nv_bfloat16 *src = a.query + (long long)(info.first_token + tok) * a.ldq + (size_t)(info.head * a.group + row - tok * a.group) * kKv8Dim + (lane & 3) * 8;
-                uint4 q[4];                                   // dims 32 i + 8 (lane & 3) .. + 7
-                uint32_t most = 0u;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) q[i] = r < info.rows ? *reinterpret_cast<const uint4 *>(src + i * 32) : make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    most = __vmaxu2(most, __vmaxu2(__vmaxu2(q[i].x & 0x7FFF7FFFu, q[i].y & 0x7FFF7FFFu), __vmaxu2(q[i].z & 0x7FFF7FFFu, q[i].w & 0x7FFF7FFFu)));
-                most = __vmaxu2(most, __shfl_xor_sync(0xFFFFFFFFu, most, 1));
-                most = __vmaxu2(most, __shfl_xor_sync(0xFFFFFFFFu, most, 2));
-                most = max(most >> 16, most & 0xFFFFu);
-                // 2^shift brings the largest element to [2^7, 2^8) (one below 2^-119 less far); a row that is not finite gets NaN
-                // scores by its scale
-                const int expo = (int)(most >> 7), shift = expo == 255 ? 0 : min(7 + 127 - expo, 126);
-                const float up = pow2(shift);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint32_t w[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
-                    uint32_t hi[2] = {0u, 0u}, lo[2] = {0u, 0u};
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        float x0 = __uint_as_float(w[e] << 16) * up, x1 = __uint_as_float(w[e] & 0xFFFF0000u) * up;
-                        hi[e >> 1] |= e4m3_split(x0, x1) << (16 * (e & 1));
-                        lo[e >> 1] |= e4m3x2(x0, x1) << (16 * (e & 1));
-                    }
-                    const uint32_t at = swizzled(r, i * 32 + (lane & 3) * 8);
-                    *reinterpret_cast<uint2 *>(sm.q[0] + at) = make_uint2(hi[0], hi[1]);
-                    *reinterpret_cast<uint2 *>(sm.q[1] + at) = make_uint2(lo[0], lo[1]);
-                }
-                if ((lane & 3) == 0) sm.qscale[r] = expo == 255 ? __int_as_float(0x7FFFFFFF) : a.scale_log2 * pow2(-shift);
-            }
-            fence_proxy_async_smem();
-            mbar_arrive(bar(B_QFULL));
-            ok = mbar_wait_warp(bar(B_STEP + (int)(t & 1u)), (t >> 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION);
-            if (!ok) break;
-            ask(t);
-            for (int j = 0; j < info.steps; ++j) {
+            for (int j = 0; j < steps; ++j, ++t) {
                 const StepInfo &st = sm.step[t & 1u];
-                ok = t == 0 || mbar_wait_warp(bar(B_PVDONE + (int)((t - 1) & 1u)), ((t - 1) >> 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION);
+                ok = mbar_wait_short(bar(B_STEP + (int)(t & 1u)), (t >> 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION) &&
+                     mbar_wait_short(bar(B_RFULL), t & 1u, abort_word, ST_TIMEOUT_ATTENTION) &&
+                     (t == 0 || mbar_wait_short(bar(B_PVDONE + (int)((t - 1) & 1u)), ((t - 1) >> 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION));
                 if (!ok) break;
                 const bool wide = st.wide != 0;
-#pragma unroll
+#pragma unroll 2
                 for (int i = 0; i < GROUPS; ++i) {
-                    const int r = i * kKv8Group + in_group;
-                    const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-                    const float mul = st.vmul[i];
-                    uint32_t h[8];
+                    uint32_t w[4], h[8];
+                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(src + i * GROUP_BYTES) : "memory");
+                    float mul = st.vmul[i];
+                    if (in_group >= st.tokens[i]) w[0] = w[1] = w[2] = w[3] = 0u;         // behind the end may be anything: zeros instead
                     if (!wide) {
                         const __half2 m2 = __float2half2_rn(mul);
 #pragma unroll
@@ -378,165 +386,192 @@ __global__ void __launch_bounds__(THREADS, 2) kv8_prefill_kernel(const __grid_co
                             h[e] = pack2(f.x * mul, f.y * mul);
                         }
                     }
-                    uint8_t *dst = sm.v[chunk >> 2] + r * 128;
-                    const int c0 = (chunk & 3) * 2;
-                    *reinterpret_cast<uint4 *>(dst + ((c0 ^ (r & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
-                    *reinterpret_cast<uint4 *>(dst + (((c0 + 1) ^ (r & 7)) << 4)) = make_uint4(h[4], h[5], h[6], h[7]);
+                    // the 16-byte chunks 2 (chunk % 4) and the next of the row, swizzled: they differ in the lowest bit
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + i * (kKv8Group * 128) + c0), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + i * (kKv8Group * 128) + (c0 ^ 16u)), "r"(h[4]), "r"(h[5]), "r"(h[6]), "r"(h[7]) : "memory");
                 }
+                mbar_arrive(bar(B_REMPTY));
                 fence_proxy_async_smem();
                 mbar_arrive(bar(B_VFULL));
-                ++t;
-                if (j + 1 < info.steps) {
-                    ok = mbar_wait_warp(bar(B_STEP + (int)(t & 1u)), (t >> 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION);
-                    if (!ok) break;
-                    ask(t);
-                }
             }
         }
     } else {
         // ================================ softmax ================================
+        more_registers<REGS_SOFTMAX>();
         const int me = (int)threadIdx.x;                      // row of the tile, lane of tensor memory
         const uint32_t t_row = tmem + ((uint32_t)(warp * 32) << 16), t_o = t_row + COL_O;
-        uint32_t t = 0, items = 0, worked = 0;
+        uint32_t t = 0, items = 0;
         bool ok = true;
-        while (ok) {
+        ItemInfo info, next;
+        uint4 q[16];                                          // this row's queries of the next item
+        // the next item, and its queries asked for
+        auto look_ahead = [&]() {
             const int is = (int)(items & 1u);
-            if (!mbar_wait_warp(bar(B_INFO + is), (items >> 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION)) break;
-            const ItemInfo info = sm.item[is];
-            if (info.rows == 0) break;
+            if (!mbar_wait_short(bar(B_INFO + is), (items >> 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION)) return false;
+            next = sm.item[is];
             ++items;
+            if (next.rows == 0) return true;
             mbar_arrive(bar(B_INFOFREE + is));
+            const int row = next.row0 + me, tok = a.by_group.div(row);
+            const uint4 *src = reinterpret_cast<const uint4 *>(a.query + (long long)(next.first_token + tok) * a.ldq + (size_t)(next.head * a.group + row - tok * a.group) * kKv8Dim);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) q[i] = me < next.rows && next.steps > 0 ? src[i] : make_uint4(0u, 0u, 0u, 0u);
+            return true;
+        };
+        ok = look_ahead();
+        while (ok && next.rows > 0) {
+            info = next;
             const int row = info.row0 + me, tok = a.by_group.div(row);
             const int pos = me < info.rows ? info.start + tok : -1;
             __nv_bfloat16 *out = a.out + (long long)(info.first_token + tok) * a.ldo + (size_t)(info.head * a.group + row - tok * a.group) * kKv8Dim;
-            float m = kNothing, l = 0.0f, qs = 0.0f, vref = 1.0f;
+            float m = kNothing, most = kNothing, l = 0.0f, qs = 0.0f, vref = 1.0f;      // most: the largest score so far
+            if (info.steps > 0) {
+                // Queries: the scores of the item before are done with them (its last were waited for).  2^shift brings the largest
+                // element to [2^7, 2^8) (one below 2^-119 less far); a row that is not finite gets NaN scores by its scale.
+                uint32_t big = 0u;
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    big = __vmaxu2(big, __vmaxu2(__vmaxu2(q[i].x & 0x7FFF7FFFu, q[i].y & 0x7FFF7FFFu), __vmaxu2(q[i].z & 0x7FFF7FFFu, q[i].w & 0x7FFF7FFFu)));
+                big = max(big >> 16, big & 0xFFFFu);
+                const int expo = (int)(big >> 7), shift = expo == 255 ? 0 : min(7 + 127 - expo, 126);
+                const float up = pow2(shift);
+                qs = expo == 255 ? __int_as_float(0x7FFFFFFF) : a.scale_log2 * pow2(-shift);
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {                 // 16 dims
+                    uint32_t hi[4] = {0u, 0u, 0u, 0u}, lo[4] = {0u, 0u, 0u, 0u};
+                    const uint32_t w[8] = {q[2 * c].x, q[2 * c].y, q[2 * c].z, q[2 * c].w, q[2 * c + 1].x, q[2 * c + 1].y, q[2 * c + 1].z, q[2 * c + 1].w};
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        float x0 = __uint_as_float(w[e] << 16) * up, x1 = __uint_as_float(w[e] & 0xFFFF0000u) * up;
+                        hi[e >> 1] |= e4m3_split(x0, x1) << (16 * (e & 1));
+                        lo[e >> 1] |= e4m3x2(x0, x1) << (16 * (e & 1));
+                    }
+                    const uint32_t at = swizzled(me, c * 16);
+                    *reinterpret_cast<uint4 *>(sm.q[0] + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                    *reinterpret_cast<uint4 *>(sm.q[1] + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                }
+                fence_proxy_async_smem();
+                mbar_arrive(bar(B_QFULL));
+            }
             for (int j = 0; j < info.steps; ++j, ++t) {
                 const int s = (int)(t & 1u);
-                ok = mbar_wait_warp(bar(B_STEP + s), (t >> 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION) && mbar_wait_warp(bar(B_SFULL), t & 1u, abort_word, ST_TIMEOUT_ATTENTION);
-                if (ok && j == 0) ok = mbar_wait_warp(bar(B_QFULL), worked & 1u, abort_word, ST_TIMEOUT_ATTENTION);
+                ok = mbar_wait_short(bar(B_STEP + s), (t >> 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION) && mbar_wait_short(bar(B_SFULL), t & 1u, abort_word, ST_TIMEOUT_ATTENTION);
                 if (!ok) break;
                 tc_fence_after();
                 const StepInfo &st = sm.step[s];
-                if (j == 0) qs = sm.qscale[me];
-                const bool plain = st.plain != 0;
+                const bool plain = st.plain != 0, wide = st.wide != 0;
                 vref = st.vref;
-                uint32_t seen[GROUPS / 2];                    // bit 16 (g % 2) + i: this row sees key i of group g
+                // The sum of the step before is done (these scores were asked for after it): the output under the present references.
+                // m moves here where the steps before have seen more than 2^8 m, and at once below where a score is beyond 2^15 m.
+                float factor = j > 0 ? st.vstep : 1.0f;
+                if (most > m + kLazy) {
+                    const float alpha = ex2(m - most);
+                    l *= alpha;
+                    factor *= alpha;
+                    m = most;
+                }
                 if (!plain) {
-#pragma unroll
+                    // scores times their scales, -inf for keys that this row does not see, back to where they were
+#pragma unroll 1
                     for (int g = 0; g < GROUPS; ++g) {
                         const int k0 = st.key[g];
-                        uint32_t b = (1u << max(0, min(st.tokens[g], pos - k0 + 1))) - 1u;
+                        uint32_t seen = (1u << max(0, min(st.tokens[g], pos - k0 + 1))) - 1u;       // bit i: key i of the group
                         if (a.window > 0) {
                             const uint32_t gone = (1u << max(0, min(kKv8Group, pos - a.window + 1 - k0))) - 1u, first = (1u << max(0, min(kKv8Group, a.sinks - k0))) - 1u;
-                            b &= ~gone | first;
+                            seen &= ~gone | first;
                         }
-                        if (g & 1) seen[g >> 1] |= b << 16;
-                        else seen[g >> 1] = b;
-                        if ((st.poisoned >> g & 1u) != 0u && b != 0u) l = __int_as_float(0x7FFFFFFF);
+                        if ((st.poisoned >> g & 1u) != 0u && seen != 0u) l = __int_as_float(0x7FFFFFFF);
+                        const float f = qs * st.ks[g];
+                        uint32_t y[16];
+                        tmem_ld_x16(t_row + (uint32_t)g * 16, y);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) y[e] = (seen >> e & 1u) != 0u ? __float_as_uint(__uint_as_float(y[e]) * f) : 0xFF800000u;
+                        tmem_st_x16(t_row + (uint32_t)g * 16, y);
                     }
+                    tmem_st_wait();
                 } else if (st.poisoned != 0u) {
                     l = __int_as_float(0x7FFFFFFF);
                 }
-                // the maximum first: whether the row's reference has to move
-                float mx = kNothing;
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t x[32];
-                    tmem_ld_x32(t_row + (uint32_t)c * 32, x);
-                    tmem_ld_wait();
-                    if (!plain) {
-#pragma unroll
-                        for (int e = 0; e < 32; ++e)
-                            if ((seen[c] >> e & 1u) == 0u) x[e] = 0xFF800000u;
-                    }
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        float b = -INFINITY;
-#pragma unroll
-                        for (int e = 0; e < 16; e += 2) b = max3(b, __uint_as_float(x[16 * h + e]), __uint_as_float(x[16 * h + e + 1]));
-                        mx = fmaxf(mx, b * (qs * st.ks[2 * c + h]));
-                    }
-                }
-                float factor = j > 0 ? st.vstep : 1.0f;
-                if (mx > m + kLazy) {
-                    const float alpha = ex2(m - mx);
-                    l *= alpha;
-                    factor *= alpha;
-                    m = mx;
-                }
-                // the sum of the step before is done: these scores were asked for after it
-                if (j > 0 && __any_sync(0xFFFFFFFFu, factor != 1.0f)) {
+                unsigned long long sum2[2] = {pack_f32x2(0.0f, 0.0f), pack_f32x2(0.0f, 0.0f)};
 #pragma unroll 1
-                    for (int c = 0; c < 4; ++c) {
-                        uint32_t o[32];
-                        tmem_ld_x32(t_o + (uint32_t)c * 32, o);
-                        tmem_ld_wait();
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * factor);
-                        tmem_st_x32(t_o + (uint32_t)c * 32, o);
-                    }
-                }
-                const bool wide = st.wide != 0;
-                unsigned long long sum2 = pack_f32x2(0.0f, 0.0f);
-                const unsigned long long neg_m2 = pack_f32x2(-m, -m);
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t x[32], w[16];
-                    tmem_ld_x32(t_row + (uint32_t)c * 32, x);
+                for (int c = 0; c < KT / 64; ++c) {           // four groups at a time
+                    uint32_t y[2][32];
+                    tmem_ld_x32(t_row + (uint32_t)c * 64, y[0]);
+                    tmem_ld_x32(t_row + (uint32_t)c * 64 + 32, y[1]);
+                    const float4 ks = *reinterpret_cast<const float4 *>(&st.ks[4 * c]);
+                    const float f[4] = {plain ? qs * ks.x : 1.0f, plain ? qs * ks.y : 1.0f, plain ? qs * ks.z : 1.0f, plain ? qs * ks.w : 1.0f};
                     tmem_ld_wait();
+                    float high = kNothing;
+#pragma unroll
+                    for (int h = 0; h < 4; ++h) {
+                        const uint32_t *z = &y[h >> 1][16 * (h & 1)];
+                        float t0 = max3(__uint_as_float(z[0]), __uint_as_float(z[1]), __uint_as_float(z[2]));
+                        float t1 = max3(__uint_as_float(z[3]), __uint_as_float(z[4]), __uint_as_float(z[5]));
+#pragma unroll
+                        for (int e = 6; e < 14; e += 4) {
+                            t0 = max3(t0, __uint_as_float(z[e]), __uint_as_float(z[e + 1]));
+                            t1 = max3(t1, __uint_as_float(z[e + 2]), __uint_as_float(z[e + 3]));
+                        }
+                        high = fmaxf(high, max3(t0, t1, fmaxf(__uint_as_float(z[14]), __uint_as_float(z[15]))) * f[h]);
+                    }
+                    most = fmaxf(most, high);
+                    float alpha = 1.0f;
+                    if (high > m + kFar) {
+                        alpha = ex2(m - high);
+                        m = high;
+                    }
+                    // what is there already under the references as they are now
+                    if (__any_sync(0xFFFFFFFFu, factor != 1.0f || alpha != 1.0f)) {
+                        l *= alpha;
+                        sum2[0] = mul_f32x2(sum2[0], pack_f32x2(alpha, alpha));
+                        sum2[1] = mul_f32x2(sum2[1], pack_f32x2(alpha, alpha));
+                        if (j > 0) scale_columns(t_o, factor * alpha);
+                        if (c > 0) scale_weights(t_row, 32, alpha, wide);
+                        factor = 1.0f;
+                    }
+                    const unsigned long long neg_m2 = pack_f32x2(-m, -m);
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const float f = qs * st.ks[2 * c + h];
-                        const unsigned long long f2 = pack_f32x2(f, f);
+                        uint32_t w[16];
 #pragma unroll
-                        for (int e = 16 * h; e < 16 * h + 16; e += 2) {
+                        for (int e = 0; e < 32; e += 2) {
+                            const unsigned long long f2 = pack_f32x2(f[2 * h + (e >> 4)], f[2 * h + (e >> 4)]);
                             float y0, y1;
-                            unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), f2, neg_m2), y0, y1);
-                            float p0 = ex2(y0), p1 = ex2(y1);
-                            if (!plain) {
-                                if ((seen[c] >> e & 1u) == 0u) p0 = 0.0f;
-                                if ((seen[c] >> (e + 1) & 1u) == 0u) p1 = 0.0f;
-                            }
-                            sum2 = add_f32x2(sum2, pack_f32x2(p0, p1));
-                            x[e] = __float_as_uint(p0), x[e + 1] = __float_as_uint(p1);
+                            unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(y[h][e]), __uint_as_float(y[h][e + 1])), f2, neg_m2), y0, y1);
+                            const float p0 = ex2(y0), p1 = ex2(y1);
+                            sum2[e >> 4] = add_f32x2(sum2[e >> 4], pack_f32x2(p0, p1));
+                            w[e >> 1] = wide ? pack2(p0, p1) : pack2_f16(p0, p1);
                         }
+                        // over scores that have been read: the weights of these 64 keys take columns 32 c .. 32 c + 31
+                        tmem_st_x16(t_row + (uint32_t)(c * 32 + h * 16), w);
                     }
-                    if (!wide) {
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) w[e] = pack2_f16(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]));
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) w[e] = pack2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]));
-                    }
-                    tmem_st_x16(t_row + (uint32_t)c * 16, w);
                 }
                 float s0, s1;
-                unpack_f32x2(sum2, s0, s1);
+                unpack_f32x2(add_f32x2(sum2[0], sum2[1]), s0, s1);
                 l += s0 + s1;
                 tmem_st_wait();
                 tc_fence_before();
                 mbar_arrive(bar(B_PFULL));
             }
             if (!ok) break;
+            ok = look_ahead();
+            if (!ok) break;
             if (info.steps > 0) {
-                ok = mbar_wait_warp(bar(B_PVDONE + (int)((t - 1) & 1u)), ((t - 1) >> 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION);
+                ok = mbar_wait_short(bar(B_PVDONE + (int)((t - 1) & 1u)), ((t - 1) >> 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION);
                 if (!ok) break;
                 tc_fence_after();
-                ++worked;
             }
             const float inv = l == 0.0f ? 0.0f : vref / l;    // a row that sees nothing; NaN stays NaN
-#pragma unroll
+#pragma unroll 1
             for (int c = 0; c < 4; ++c) {
                 uint32_t o[32];
-#pragma unroll
-                for (int e = 0; e < 32; ++e) o[e] = 0u;
                 if (info.steps > 0) {
                     tmem_ld_x32(t_o + (uint32_t)c * 32, o);
                     tmem_ld_wait();
-                    if (c == 3) {
-                        tc_fence_before();
-                        mbar_arrive(bar(B_OFREE));
-                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) o[e] = 0u;
                 }
                 if (me < info.rows) {
 #pragma unroll
@@ -545,6 +580,10 @@ __global__ void __launch_bounds__(THREADS, 2) kv8_prefill_kernel(const __grid_co
                             make_uint4(pack2(__uint_as_float(o[8 * e]) * inv, __uint_as_float(o[8 * e + 1]) * inv), pack2(__uint_as_float(o[8 * e + 2]) * inv, __uint_as_float(o[8 * e + 3]) * inv),
                                        pack2(__uint_as_float(o[8 * e + 4]) * inv, __uint_as_float(o[8 * e + 5]) * inv), pack2(__uint_as_float(o[8 * e + 6]) * inv, __uint_as_float(o[8 * e + 7]) * inv));
                 }
+            }
+            if (info.steps > 0) {
+                tc_fence_before();
+                mbar_arrive(bar(B_OFREE));
             }
         }
     }
@@ -575,6 +614,7 @@ bool kv8_prefill_launch(const Kv8Attend &a, cudaStream_t st) {
     Params p;
     memset(&p, 0, sizeof(p));
     if (!make_u8_tmap_sw128(&p.tm_k, a.k_cache, kKv8Dim, (uint64_t)a.b.num_blocks * a.b.kv_heads * a.b.block_size, kKv8Dim, kKv8Dim, kKv8Group)) return false;
+    if (!make_u8_tmap_sw128(&p.tm_v, a.v_cache, kKv8Dim, (uint64_t)a.b.num_blocks * a.b.kv_heads * a.b.block_size, kKv8Dim, kKv8Dim, kKv8Group)) return false;
     p.a = a;
     const long long tiles = ((long long)a.b.total_new * a.group >> 7) + a.b.num_seqs;
     if (tiles * a.b.kv_heads > 0x7FFFFFFFLL) return false;

@@ -76,6 +76,19 @@ __device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, vo
     return __all_sync(0xFFFFFFFFu, ok);
 }
 
+// The same in a dozen instructions instead of forty, for kernels with many waits whose code should stay in the instruction cache: bounded by
+// the number of tries, each of which the hardware may hold for a microsecond or so.
+static constexpr int kWaitTries = 1 << 20;
+__device__ __forceinline__ bool mbar_wait_short(uint32_t bar, uint32_t parity, volatile int *abort_word, int code) {
+#pragma unroll 1
+    for (int i = 0; i < kWaitTries; ++i) {
+        if (__all_sync(0xFFFFFFFFu, mbar_try_wait(bar, parity))) return true;
+        if (__any_sync(0xFFFFFFFFu, *abort_word != 0)) return false;
+    }
+    *abort_word = code;
+    return false;
+}
+
 // One lane of a converged warp (always the same one).  Single-instruction work such as a TMA
 // issue or a tcgen05.mma is guarded by this while the surrounding address arithmetic runs
 // warp-uniformly, which lets it live in uniform registers.
