@@ -382,7 +382,7 @@ __global__ void __launch_bounds__(THREADS, 2) kv8_prefill_kernel(const __grid_co
                 if (!ok) break;
                 const bool wide = st.wide != 0;
                 const uint32_t src = src0 + (uint32_t)s * sizeof(sm.raw[0]), dst = dst0 + (uint32_t)s * sizeof(sm.v[0]);
-#pragma unroll 2
+#pragma unroll 1
                 for (int i = 0; i < GROUPS; ++i) {
                     uint32_t w[4], h[8];
                     asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(src + i * GROUP_BYTES) : "memory");
