@@ -14,8 +14,8 @@
 // Bound: the two products are 2 x 128 x 64 x 128 multiply-adds a step, 512 cycles at the tensor cores' nominal rate, and the exponentials 512
 // of the special-function units.  The softmax of a step is a chain of some 2000 cycles, so two CTAs share an SM, and a CTA's scores of
 // the next step are computed under its softmax: tensor memory has two of S and one of O.  (128 keys per step with one S: 382 us
-// where this takes 344, two sequences of 2000 new tokens behind 5000; 128 columns of S are all that O leaves of the half of
-// tensor memory that a CTA has.)
+// where this takes 335, two sequences of 2000 new tokens behind 5000; 128 columns of S are all that O leaves of the half of
+// tensor memory that a CTA has.  Two threads per row, eight warps of softmax: 386 there, and 63 us instead of 71 for 25 prompts of 400.)
 //   warp 8      producer: the work items, K and V tiles (a TMA box of 2 KB per group of 16 keys), scales of each step; places in the pool are
 //               looked up 8 steps ahead, which is worth 60 us there
 //   warp 9      products; scores [0, 64) and [64, 128), output [128, 256) of tensor memory, P as f16 over the scores it was made from
@@ -113,7 +113,11 @@ __device__ __forceinline__ void scale_columns(uint32_t t_o, float f) {
     }
 }
 
-
+// One arrival for the 32 threads of a warp, each of which is done.
+__device__ __forceinline__ void arrive_warp(uint32_t bar) {
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+}
 template <int N>
 __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N>
@@ -130,19 +134,19 @@ __global__ void __launch_bounds__(THREADS, 2) kv8_prefill_kernel(const __grid_co
         return;
     }
     if (threadIdx.x == 0) {
-        mbar_init(bar(B_QFULL), 128);
-        mbar_init(bar(B_OFREE), 128);
+        mbar_init(bar(B_QFULL), 4);
+        mbar_init(bar(B_OFREE), 4);
         mbar_init(bar(B_NEXT), 1);
         for (int i = 0; i < 2; ++i) {
             mbar_init(bar(B_KFULL + i), 1);
             mbar_init(bar(B_KEMPTY + i), 1);
             mbar_init(bar(B_RFULL + i), 1);
-            mbar_init(bar(B_REMPTY + i), 128);
-            mbar_init(bar(B_VFULL + i), 128);
+            mbar_init(bar(B_REMPTY + i), 4);
+            mbar_init(bar(B_VFULL + i), 4);
             mbar_init(bar(B_SFULL + i), 1);
-            mbar_init(bar(B_PFULL + i), 128);
+            mbar_init(bar(B_PFULL + i), 4);
             mbar_init(bar(B_INFO + i), 1);
-            mbar_init(bar(B_INFOFREE + i), 128 + 128 + 1);
+            mbar_init(bar(B_INFOFREE + i), 4 + 4 + 1);
         }
         for (int i = 0; i < STEPS; ++i) {
             mbar_init(bar(B_STEP + i), 1);
@@ -374,7 +378,7 @@ __global__ void __launch_bounds__(THREADS, 2) kv8_prefill_kernel(const __grid_co
             const int rows = sm.item[is].rows, steps = sm.item[is].steps;
             if (rows == 0) break;
             ++items;
-            mbar_arrive(bar(B_INFOFREE + is));
+            arrive_warp(bar(B_INFOFREE + is));
             for (int j = 0; j < steps; ++j, ++t) {
                 const int s = (int)(t & 1u);
                 const StepInfo &st = sm.step[t % STEPS];
@@ -408,9 +412,9 @@ __global__ void __launch_bounds__(THREADS, 2) kv8_prefill_kernel(const __grid_co
                     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
                     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at ^ 16u), "r"(h[4]), "r"(h[5]), "r"(h[6]), "r"(h[7]) : "memory");
                 }
-                mbar_arrive(bar(B_REMPTY + s));
+                arrive_warp(bar(B_REMPTY + s));
                 fence_proxy_async_smem();
-                mbar_arrive(bar(B_VFULL + s));
+                arrive_warp(bar(B_VFULL + s));
             }
         }
     } else {
@@ -427,7 +431,7 @@ __global__ void __launch_bounds__(THREADS, 2) kv8_prefill_kernel(const __grid_co
             next = sm.item[is];
             ++items;
             if (next.rows == 0) return true;
-            mbar_arrive(bar(B_INFOFREE + is));
+            arrive_warp(bar(B_INFOFREE + is));
             if (next.steps == 0) return true;
             const int part = lane & 15;
 #pragma unroll 4
@@ -476,7 +480,7 @@ __global__ void __launch_bounds__(THREADS, 2) kv8_prefill_kernel(const __grid_co
                     *reinterpret_cast<uint4 *>(sm.q[1] + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                 }
                 fence_proxy_async_smem();
-                mbar_arrive(bar(B_QFULL));
+                arrive_warp(bar(B_QFULL));
             }
             for (int j = 0; j < info.steps; ++j, ++t) {
                 const int s = (int)(t & 1u);
@@ -563,7 +567,7 @@ __global__ void __launch_bounds__(THREADS, 2) kv8_prefill_kernel(const __grid_co
                 l += s0 + s1;
                 tmem_st_wait();
                 tc_fence_before();
-                mbar_arrive(bar(B_PFULL + s));
+                arrive_warp(bar(B_PFULL + s));
             }
             if (!ok) break;
             ok = look_ahead();
@@ -608,7 +612,7 @@ __global__ void __launch_bounds__(THREADS, 2) kv8_prefill_kernel(const __grid_co
             }
             if (info.steps > 0) {
                 tc_fence_before();
-                mbar_arrive(bar(B_OFREE));
+                arrive_warp(bar(B_OFREE));
             }
         }
         cp_async_wait<0>();
