@@ -14,13 +14,15 @@
 //            2^(x_j + log2 v_scale_j - W + 6), at most 2^8, is split as p = hi + 2^-4 lo: off by 6.6e-4 of its size (rms; bf16: 1.6e-3) or 2^-20
 //            of the largest, whichever is more.
 //   lazily   m and W are touched when a term has grown past 2^8 m or 2^2 W: an ordinary tile needs one vote of its four warps.
-//   split    Two ways to deal out the work, chosen on the host (see deal_whole()).  Whole: one CTA of the grid for each (sequence, kv head); those that run take
-//            over the work of those that have not started, and there is nothing to join.  Pieces: all visible groups of 16 tokens of all (sequence, kv head) pairs form one line,
-//            cut into equal pieces, one per CTA, so that uneven lengths cost nothing; a piece that ends inside a context leaves m,
-//            W, the sum and the accumulator in the workspace, and a second launch joins those.
-// A CTA walks its piece context by context in tiles of up to eight groups: warp 4 copies (a TMA box of 2 KB per group, K or V; the
-// groups of a tile may lie anywhere), prepares the queries of the next context and says where its results go, warp 5 issues the
-// products, warps 0-3 are the softmax, one thread per token, and write the results.
+//   split    Two ways to deal out the work, chosen on the host (see deal_whole()).  Whole: one CTA of the grid for each (sequence, kv
+//            head); those that run take over the work of those that have not started, and there is nothing to join.  Pieces: all
+//            visible groups of 16 tokens of all (sequence, kv head) pairs form one line, cut into equal pieces, one per CTA, so that
+//            uneven lengths cost little; a piece that ends inside a context leaves m, W, the sum and the accumulator in the
+//            workspace, and a second launch joins those.
+// A CTA walks its piece context by context in tiles of up to eight groups: one warp copies (a TMA box of 2 KB per group, K or V; the
+// groups of a tile may lie anywhere), prepares the queries of the next context and says where its results go, one issues the
+// products, and the others are the softmax and write the results: a thread per token, or two where there are more than 8 rows, each
+// with half of them (64 sequences of 200 to 2000 tokens with 8 new ones, 32 rows: 50 us instead of 54).
 // K and V have two buffers each.  A tile's chain of waits, products and softmax is about 2000 cycles, and a copy takes as long: three
 // CTAs with 64 KB of tiles each keep HBM busy.  (Four with one buffer of each: every copy waits for a product, 4000 cycles a tile.)
 #include <math.h>
@@ -35,8 +37,10 @@ static __device__ int g_kv8_status[4];
 
 namespace {
 
-constexpr int SOFTMAX = 128;                                  // threads; also tokens of a tile and lanes of tensor memory
-constexpr int THREADS = SOFTMAX + 64;
+constexpr int SOFTMAX = 128;                                  // tokens of a tile, lanes of tensor memory
+// Softmax threads of a token, each of which has as many of the rows; then two more warps.
+constexpr int split(int rows) { return rows <= 8 ? 1 : 2; }
+constexpr int threads(int rows) { return split(rows) * SOFTMAX + 64; }
 constexpr int TILE_GROUPS = SOFTMAX / kKv8Group;
 constexpr int GROUP_BYTES = kKv8Group * kKv8Dim;
 constexpr int TILE_BYTES = TILE_GROUPS * GROUP_BYTES;         // 16 KB of K, or V
@@ -72,20 +76,39 @@ struct Smem {
     uint4 next;                           // answer to the question for more work
     unsigned long long bars[B_COUNT];
     uint32_t tmem;
-    int abort, warp_sum[8];
+    int abort, warp_sum[threads(R) / 32];
     int prefix[1];                        // num_seqs entries: units before each sequence
 };
 
 // Whether any of the softmax threads says so (and a barrier among them).
+template <int COUNT>
 __device__ __forceinline__ bool any_of_softmax(bool x) {
     uint32_t r;
     asm volatile(
         "{\n\t.reg .pred p, q;\n\t"
         "setp.ne.u32 p, %1, 0;\n\t"
-        "barrier.cta.red.or.pred q, 1, 128, p;\n\t"
+        "barrier.cta.red.or.pred q, 1, %2, p;\n\t"
         "selp.u32 %0, 1, 0, q;\n\t}"
-        : "=r"(r) : "r"(x ? 1u : 0u) : "memory");
+        : "=r"(r) : "r"(x ? 1u : 0u), "n"(COUNT) : "memory");
     return r != 0;
+}
+// V columns of tensor memory, 32 bits of this lane each
+template <int V>
+__device__ __forceinline__ void load_columns(uint32_t t, uint32_t (&r)[V]) {
+    static_assert(V == 4 || V == 8 || V == 12 || V == 16, "columns");
+    if constexpr (V >= 8) {
+        if constexpr (V == 16) tmem_ld_x16(t, r);
+        else tmem_ld_x8(t, *reinterpret_cast<uint32_t(*)[8]>(&r[0]));
+    }
+    if constexpr (V % 8 == 4) tmem_ld_x4(t + V / 8 * 8, *reinterpret_cast<uint32_t(*)[4]>(&r[V / 8 * 8]));
+}
+template <int V>
+__device__ __forceinline__ void store_columns(uint32_t t, const uint32_t (&r)[V]) {
+    if constexpr (V >= 8) {
+        if constexpr (V == 16) tmem_st_x16(t, r);
+        else tmem_st_x8(t, *reinterpret_cast<const uint32_t(*)[8]>(&r[0]));
+    }
+    if constexpr (V % 8 == 4) tmem_st_x4(t + V / 8 * 8, *reinterpret_cast<const uint32_t(*)[4]>(&r[V / 8 * 8]));
 }
 // The line of work.  rows = query rows (new token, head of the group) a context has at most; a sequence with more of them has
 // several row tiles.  Units of (sequence, row tile, kv head), in that order: its visible groups of 16 tokens, and behind them as many
@@ -180,8 +203,9 @@ constexpr int max_ctas(int rows) { return rows <= 8 ? 3 : 2; }
 // R = query rows of a context as the products have them, U <= R how many the softmax works on (a group of four heads fills half
 // of the narrowest product).
 template <int R, int U>
-__global__ void __launch_bounds__(THREADS, max_ctas(R)) kv8_attend_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(threads(R), max_ctas(R)) kv8_attend_kernel(const __grid_constant__ Params p) {
     constexpr int N = 2 * R;                                  // columns of both products
+    constexpr int SPLIT = split(R), THREADS = threads(R), WORKERS = SPLIT * SOFTMAX, COPIES = WORKERS / 32, PRODUCTS = COPIES + 1;       // the last two: warps
     constexpr int TMEM_COLS = 3 * N <= 64 ? 64 : 3 * N <= 128 ? 128 : 256;     // two score buffers, the accumulator
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     Smem<R> &sm = *reinterpret_cast<Smem<R> *>(smem_raw);
@@ -194,8 +218,8 @@ __global__ void __launch_bounds__(THREADS, max_ctas(R)) kv8_attend_kernel(const 
         return;
     }
     if (threadIdx.x == 0) {
-        mbar_init(bar(B_PFULL), SOFTMAX);
-        mbar_init(bar(B_OFREE), SOFTMAX);
+        mbar_init(bar(B_PFULL), WORKERS);
+        mbar_init(bar(B_OFREE), WORKERS);
         mbar_init(bar(B_NEXT), 1);
         for (int i = 0; i < 2; ++i) {
             mbar_init(bar(B_KFULL + i), 1);
@@ -205,14 +229,14 @@ __global__ void __launch_bounds__(THREADS, max_ctas(R)) kv8_attend_kernel(const 
             mbar_init(bar(B_SFULL + i), 1);
             mbar_init(bar(B_SCALES + i), 1);
             mbar_init(bar(B_CFULL + i), 1);
-            mbar_init(bar(B_CEMPTY + i), 1 + SOFTMAX);        // the last product of scores and the results
+            mbar_init(bar(B_CEMPTY + i), 1 + WORKERS);        // the last product of scores and the results
         }
         sm.abort = 0;
         fence_mbar_init();
         tma_prefetch_desc(&p.tm_k);
         tma_prefetch_desc(&p.tm_v);
     }
-    if (warp == 5) {
+    if (warp == PRODUCTS) {
         tmem_alloc(smem_u32(&sm.tmem), TMEM_COLS);
         tmem_relinquish();
     }
@@ -281,7 +305,7 @@ __global__ void __launch_bounds__(THREADS, max_ctas(R)) kv8_attend_kernel(const 
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(&sm.tmem);
     volatile int *abort_word = &sm.abort;
 
-    if (warp == 4) {
+    if (warp == COPIES) {
         // ================================ copies, queries =======================
         const bool leader = elect_one();
         uint32_t t = 0, contexts = 0; // tiles and contexts started
@@ -477,7 +501,7 @@ __global__ void __launch_bounds__(THREADS, max_ctas(R)) kv8_attend_kernel(const 
             sm.ctx[cs].groups = 0;                            // the end
             mbar_arrive(bar(B_CFULL + cs));
         }
-    } else if (warp == 5) {
+    } else if (warp == PRODUCTS) {
         // ================================ products ==============================
         const bool leader = elect_one();
         constexpr uint32_t idesc_s = idesc_e4m3(128, N);
@@ -534,8 +558,10 @@ __global__ void __launch_bounds__(THREADS, max_ctas(R)) kv8_attend_kernel(const 
         }
     } else {
         // ================================ softmax ===============================
-        const int me = (int)threadIdx.x;                      // token of the tile, lane of tensor memory, dim of the result
-        const uint32_t t_lane = tmem + ((uint32_t)(warp * 32) << 16);
+        constexpr int V = U / SPLIT;
+        const int tid = (int)threadIdx.x, me = tid % SOFTMAX;   // me: token of the tile, lane of tensor memory, dim of the result
+        const int base = tid / SOFTMAX * V, quarter = warp % 4; // the first of this thread's V rows; its warp's place among those of the tokens
+        const uint32_t t_lane = tmem + ((uint32_t)(quarter * 32) << 16);
         const uint32_t t_o = t_lane + 2 * N;
         uint32_t t = 0;
         for (uint32_t contexts = 0;; ++contexts) {
@@ -544,11 +570,11 @@ __global__ void __launch_bounds__(THREADS, max_ctas(R)) kv8_attend_kernel(const 
             const ContextInfo<R> &c = sm.ctx[cs];
             const int n = (c.groups + TILE_GROUPS - 1) / TILE_GROUPS;
             const int pos_lo = c.pos_lo, pos_hi = c.pos_hi;
-            float sum[U];
+            float sum[V];
 #pragma unroll
-            for (int r = 0; r < U; ++r) sum[r] = 0.0f;
-            if (me < U) sm.row[me] = make_float4(kNothing, kNothing, -kNothing, -kNothing);
-            if (any_of_softmax(!ok) || n == 0) break;
+            for (int r = 0; r < V; ++r) sum[r] = 0.0f;
+            if (tid < U) sm.row[tid] = make_float4(kNothing, kNothing, -kNothing, -kNothing);
+            if (any_of_softmax<WORKERS>(!ok) || n == 0) break;
             for (int j = 0; j < n; ++j, ++t) {
                 const int s = (int)(t & 1u);
                 ok = mbar_wait_short(bar(B_SCALES + s), (t >> 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION);
@@ -560,78 +586,78 @@ __global__ void __launch_bounds__(THREADS, max_ctas(R)) kv8_attend_kernel(const 
                 const bool all = there && tok <= pos_lo && (a.window == 0 || pos_hi - tok < a.window || tok < a.sinks);
                 ok = ok && mbar_wait_short(bar(B_SFULL + s), (t >> 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION);
                 tc_fence_after();
-                float x[U];
-                uint32_t raw[N];
-#pragma unroll
-                for (int i = 0; i < N; i += 16) tmem_ld_x16(t_lane + (uint32_t)(s * N + i), *reinterpret_cast<uint32_t(*)[16]>(&raw[i]));
+                float x[V];
+                uint32_t high[V], low[V];
+                load_columns<V>(t_lane + (uint32_t)(s * N + base), high);
+                load_columns<V>(t_lane + (uint32_t)(s * N + R + base), low);
                 tmem_ld_wait();
 #pragma unroll
-                for (int r = 0; r < U; ++r) x[r] = fmaf(__uint_as_float(raw[R + r]), kQLo, __uint_as_float(raw[r])) * (c.qscale[r] * sc.x);
+                for (int r = 0; r < V; ++r) x[r] = fmaf(__uint_as_float(low[r]), kQLo, __uint_as_float(high[r])) * (c.qscale[base + r] * sc.x);
                 if (!there) {
 #pragma unroll
-                    for (int r = 0; r < U; ++r) x[r] = -INFINITY;
+                    for (int r = 0; r < V; ++r) x[r] = -INFINITY;
                 } else if (!all) {
                     // 0 <= p - tok < window as one comparison (a row that does not exist has the position -1)
                     const uint32_t reach = a.window == 0 || tok < a.sinks ? 0x80000000u : (uint32_t)a.window;
 #pragma unroll
-                    for (int r = 0; r < U; ++r)
-                        if ((uint32_t)(c.pos[r] - tok) >= reach) x[r] = -INFINITY;
+                    for (int r = 0; r < V; ++r)
+                        if ((uint32_t)(c.pos[base + r] - tok) >= reach) x[r] = -INFINITY;
                 }
                 bool grown = !ok;
 #pragma unroll
-                for (int r = 0; r < U; ++r) {
-                    const float2 top = *reinterpret_cast<const float2 *>(&sm.row[r].x);
+                for (int r = 0; r < V; ++r) {
+                    const float2 top = *reinterpret_cast<const float2 *>(&sm.row[base + r].x);
                     grown = grown || x[r] > fminf(top.x, top.y - vs);
                 }
-                if (any_of_softmax(grown)) {
+                if (any_of_softmax<WORKERS>(grown)) {
 #pragma unroll
-                    for (int r = 0; r < U; ++r) {
+                    for (int r = 0; r < V; ++r) {
                         const float m = redux_max(fmaxf(x[r], kNothing)), w = redux_max(fmaxf(x[r] + vs, kNothing));
-                        if (lane == 0) *reinterpret_cast<float2 *>(sm.red[warp][r]) = make_float2(m, w);
+                        if (lane == 0) *reinterpret_cast<float2 *>(sm.red[quarter][base + r]) = make_float2(m, w);
                     }
                     // the accumulator is expressed against the new W: the product before has to be complete
                     if (j > 0) ok = ok && mbar_wait_short(bar(B_PVDONE + (int)((t - 1) & 1u)), ((t - 1) >> 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION);
-                    if (any_of_softmax(!ok)) { ok = false; break; }
-                    if (me < U) {
-                        const float4 was = sm.row[me];
-                        const float m = fmaxf(fmaxf(fmaxf(sm.red[0][me][0], sm.red[1][me][0]), fmaxf(sm.red[2][me][0], sm.red[3][me][0])), -was.z);
-                        const float w = fmaxf(fmaxf(fmaxf(sm.red[0][me][1], sm.red[1][me][1]), fmaxf(sm.red[2][me][1], sm.red[3][me][1])), kWeightBase - was.w);
-                        sm.factor[me][0] = ex2(-was.z - m);
-                        sm.factor[me][1] = ex2(kWeightBase - was.w - w);
-                        sm.row[me] = make_float4(m + kTop, w + kWeightTop, -m, kWeightBase - w);
+                    if (any_of_softmax<WORKERS>(!ok)) { ok = false; break; }
+                    if (tid < U) {
+                        const float4 was = sm.row[tid];
+                        const float m = fmaxf(fmaxf(fmaxf(sm.red[0][tid][0], sm.red[1][tid][0]), fmaxf(sm.red[2][tid][0], sm.red[3][tid][0])), -was.z);
+                        const float w = fmaxf(fmaxf(fmaxf(sm.red[0][tid][1], sm.red[1][tid][1]), fmaxf(sm.red[2][tid][1], sm.red[3][tid][1])), kWeightBase - was.w);
+                        sm.factor[tid][0] = ex2(-was.z - m);
+                        sm.factor[tid][1] = ex2(kWeightBase - was.w - w);
+                        sm.row[tid] = make_float4(m + kTop, w + kWeightTop, -m, kWeightBase - w);
                     }
-                    (void)any_of_softmax(false);
+                    (void)any_of_softmax<WORKERS>(false);
                     if (j > 0) {
 #pragma unroll
-                        for (int r = 0; r < U; ++r) sum[r] *= sm.factor[r][0];
+                        for (int r = 0; r < V; ++r) sum[r] *= sm.factor[base + r][0];
                         tc_fence_after();
-#pragma unroll
-                        for (int r0 = 0; r0 < N; r0 += 16) {
-                            uint32_t o[16];
-                            tmem_ld_x16(t_o + (uint32_t)r0, o);
+#pragma unroll 1
+                        for (int part = 0; part < N; part += R) {           // hi, lo
+                            uint32_t o[V];
+                            load_columns<V>(t_o + (uint32_t)(part + base), o);
                             tmem_ld_wait();
 #pragma unroll
-                            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * sm.factor[(r0 + e) % R % U][1]);
-                            tmem_st_x16(t_o + (uint32_t)r0, o);
+                            for (int r = 0; r < V; ++r) o[r] = __float_as_uint(__uint_as_float(o[r]) * sm.factor[base + r][1]);
+                            store_columns<V>(t_o + (uint32_t)(part + base), o);
                         }
                         tmem_st_wait();
                     }
                 }
-                uint32_t w8[N / 4] = {};                      // the token's weights: R codes hi, R codes lo
+                uint32_t w_hi[V / 4] = {}, w_lo[V / 4] = {};  // the token's weights as codes
 #pragma unroll
-                for (int r = 0; r < U; r += 2) {
+                for (int r = 0; r < V; r += 2) {
                     float w[2];
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        const float2 ref = *reinterpret_cast<const float2 *>(&sm.row[r + e].z);
+                        const float2 ref = *reinterpret_cast<const float2 *>(&sm.row[base + r + e].z);
                         sum[r + e] += ex2(x[r + e] + ref.x);
                         // a token that is not seen weighs 0 whatever its block's scale is
                         w[e] = !all && x[r + e] == -INFINITY ? 0.0f : ex2(x[r + e] + (vs + ref.y));
                     }
                     const uint32_t hi = e4m3_split(w[0], w[1]);
                     const uint32_t lo = e4m3x2(w[0] / kPLo, w[1] / kPLo);
-                    w8[r / 4] |= hi << (8 * (r & 2));
-                    w8[(R + r) / 4] |= lo << (8 * (r & 2));
+                    w_hi[r / 4] |= hi << (8 * (r & 2));
+                    w_lo[r / 4] |= lo << (8 * (r & 2));
                 }
                 // the weights of the tile before have been read
                 ok = t == 0 || mbar_wait_short(bar(B_PVDONE + (s ^ 1)), ((t - 1) >> 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION);
@@ -645,10 +671,18 @@ __global__ void __launch_bounds__(THREADS, max_ctas(R)) kv8_attend_kernel(const 
                     }
                 }
                 if (!ok) *abort_word = ST_TIMEOUT_ATTENTION;  // said at the next vote
+                if constexpr (R == 8) {
+                    // all 16 columns; those of rows that do not exist are zero
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(smem_u32(sm.p) + me * 16), "r"(w_hi[0]), "r"(V == 8 ? w_hi[V / 8] : 0u), "r"(w_lo[0]),
+                                 "r"(V == 8 ? w_lo[V / 8] : 0u) : "memory");
+                } else {
 #pragma unroll
-                for (int i = 0; i < N / 16; ++i)
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(smem_u32(sm.p) + i * (16 * SOFTMAX) + me * 16), "r"(w8[4 * i]),
-                                 "r"(w8[4 * i + 1]), "r"(w8[4 * i + 2]), "r"(w8[4 * i + 3]) : "memory");
+                    for (int i = 0; i < V / 4; ++i) {
+                        const int hi = base + 4 * i, lo = R + hi;
+                        *reinterpret_cast<uint32_t *>(sm.p + hi / 16 * (16 * SOFTMAX) + me * 16 + hi % 16) = w_hi[i];
+                        *reinterpret_cast<uint32_t *>(sm.p + lo / 16 * (16 * SOFTMAX) + me * 16 + lo % 16) = w_lo[i];
+                    }
+                }
                 fence_proxy_async_smem();
                 tc_fence_before();
                 mbar_arrive(bar(B_PFULL));
@@ -658,10 +692,10 @@ __global__ void __launch_bounds__(THREADS, max_ctas(R)) kv8_attend_kernel(const 
             ok = ok && mbar_wait_short(bar(B_PVDONE + (int)((t - 1) & 1u)), ((t - 1) >> 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION);
             // sums over the warp's 32 tokens: halves of the rows are exchanged until a lane has one, then the lanes that share it add up
             {
-                constexpr int P2 = U <= 4 ? 4 : U <= 8 ? 8 : U <= 16 ? 16 : 32;
+                constexpr int P2 = V <= 4 ? 4 : V <= 8 ? 8 : 16;
                 float v[P2];
 #pragma unroll
-                for (int r = 0; r < P2; ++r) v[r] = r < U ? sum[r < U ? r : 0] : 0.0f;
+                for (int r = 0; r < P2; ++r) v[r] = r < V ? sum[r < V ? r : 0] : 0.0f;
                 int held = P2;
 #pragma unroll
                 for (int d = 16; d > 0; d >>= 1) {
@@ -678,32 +712,30 @@ __global__ void __launch_bounds__(THREADS, max_ctas(R)) kv8_attend_kernel(const 
                         v[0] += __shfl_xor_sync(0xFFFFFFFFu, v[0], d);
                     }
                 }
-                if ((lane & (32 / P2 - 1)) == 0 && lane / (32 / P2) < U) sm.red[warp][lane / (32 / P2)][0] = v[0];
+                if ((lane & (32 / P2 - 1)) == 0 && lane / (32 / P2) < V) sm.red[quarter][base + lane / (32 / P2)][0] = v[0];
             }
-            if (any_of_softmax(!ok)) break;
-            if (me < c.rows) {
-                const float l = (sm.red[0][me][0] + sm.red[1][me][0]) + (sm.red[2][me][0] + sm.red[3][me][0]);
-                const float4 st = sm.row[me];
-                if (c.slot < 0) sm.factor[me][0] = l == 0.0f ? 0.0f : ex2(st.z - st.w) / l;      // NaN stays NaN
-                else p.part.stats[(size_t)c.slot * U + me] = make_float4(-st.z, l, -st.w, 0.0f);
+            if (any_of_softmax<WORKERS>(!ok)) break;
+            if (tid < c.rows) {
+                const float l = (sm.red[0][tid][0] + sm.red[1][tid][0]) + (sm.red[2][tid][0] + sm.red[3][tid][0]);
+                const float4 st = sm.row[tid];
+                if (c.slot < 0) sm.factor[tid][0] = l == 0.0f ? 0.0f : ex2(st.z - st.w) / l;     // NaN stays NaN
+                else p.part.stats[(size_t)c.slot * U + tid] = make_float4(-st.z, l, -st.w, 0.0f);
             }
             tc_fence_after();
-            uint32_t raw[N];
-#pragma unroll
-            for (int i = 0; i < N; i += 16) tmem_ld_x16(t_o + (uint32_t)i, *reinterpret_cast<uint32_t(*)[16]>(&raw[i]));
+            uint32_t high[V], low[V];
+            load_columns<V>(t_o + (uint32_t)base, high);
+            load_columns<V>(t_o + (uint32_t)(R + base), low);
             tmem_ld_wait();
             tc_fence_before();
             mbar_arrive(bar(B_OFREE));
-            (void)any_of_softmax(false);
-            if (c.slot < 0) {
+            (void)any_of_softmax<WORKERS>(false);
+            float *to = p.part.acc + (size_t)(c.slot < 0 ? 0 : c.slot) * U * kKv8Dim + me;
 #pragma unroll
-                for (int r = 0; r < U; ++r)
-                    if (r < c.rows) c.out[r][me] = __float2bfloat16(fmaf(__uint_as_float(raw[R + r]), kPLo, __uint_as_float(raw[r])) * sm.factor[r][0]);
-            } else {
-                float *to = p.part.acc + (size_t)c.slot * U * kKv8Dim + me;
-#pragma unroll
-                for (int r = 0; r < U; ++r)
-                    if (r < c.rows) to[r * kKv8Dim] = fmaf(__uint_as_float(raw[R + r]), kPLo, __uint_as_float(raw[r]));
+            for (int r = 0; r < V; ++r) {
+                if (base + r >= c.rows) break;
+                const float o = fmaf(__uint_as_float(low[r]), kPLo, __uint_as_float(high[r]));
+                if (c.slot < 0) c.out[base + r][me] = __float2bfloat16(o * sm.factor[base + r][0]);
+                else to[(base + r) * kKv8Dim] = o;
             }
             mbar_arrive(bar(B_CEMPTY + cs));
             // the rows' state and factors are written again after the next context's first vote
@@ -717,7 +749,7 @@ __global__ void __launch_bounds__(THREADS, max_ctas(R)) kv8_attend_kernel(const 
         for (int i = 0; i < 64; ++i) __nanosleep(1000);      // let copies in flight land
         if (threadIdx.x == 0) atomicCAS(&g_kv8_status[0], 0, *abort_word);
     }
-    if (warp == 5) {
+    if (warp == PRODUCTS) {
         __syncwarp();
         tmem_dealloc(tmem, TMEM_COLS);
     }
@@ -791,7 +823,7 @@ bool launch_rows(Params &p, void *workspace, int num_seqs, cudaStream_t st, int 
     grid = num_sms() * ctas_per_sm<R>(num_seqs);
     if (p.whole) grid = num_seqs * p.a.b.kv_heads;
     partial_bytes(grid, U, workspace, &p.part);
-    return launch_chained(kv8_attend_kernel<R, U>, dim3(grid), dim3(THREADS), smem_bytes<R>(num_seqs), st, p) == cudaSuccess;
+    return launch_chained(kv8_attend_kernel<R, U>, dim3(grid), dim3(threads(R)), smem_bytes<R>(num_seqs), st, p) == cudaSuccess;
 }
 
 }  // namespace
@@ -807,33 +839,69 @@ size_t kv8_attention_workspace_bytes() {
 
 // Whole (sequence, kv head) pairs or pieces?  In cycles, from what the phases of the kernel take: a tile's chain 2200, the steps around a
 // context 2600, an SM's share of HBM 1400 a tile; pieces need 2000 for the table of units and 5000 for the join.  The longest
-// context stands for all, which flatters whole pairs where lengths are uneven, hence their limit of 16 tiles.
+// context stands for all, which flatters whole pairs where lengths are uneven, hence their limit of 8 tiles, or 16 if a window makes
+// them even.  Measured, us, whole : pieces (sequences of one new token, four heads a kv head, tokens):
+//   1 x 250        7.0 : 8.6    1 x 900       14 : 9.4    16 x 450      9.6 : 11.1   16 x 900      14 : 12.5    64 x 450      11 : 13
+//   64 x 900        17 : 18     64 x 2000     30 : 37     128 x 900     34 : 30      128 x 2000    61 : 51      256 x 450     29 : 35
+//   64 x 500..2000  25 : 20     128 x 225..900  23 : 21   128 x 500..2000  48 : 36   256 x 112..450  22 : 29    256 x 500..2000  67 : 62
 static bool deal_whole(const Kv8Attend &a, int max_len, int slots) {
     const long long contexts = (long long)a.b.num_seqs * a.b.kv_heads;
     long long tokens = max_len < a.b.max_tokens ? max_len : a.b.max_tokens;
+    long long limit = 8;
     if (a.window > 0) {
         const long long most = (long long)a.window + a.sinks + 2 * kKv8Group;
-        if (most < tokens) tokens = most;
+        if (most < tokens) tokens = most, limit = 16;
     }
     const long long tiles = (tokens + SOFTMAX - 1) / SOFTMAX;
     const long long memory = contexts * tiles * 1400 / num_sms();
     const long long whole = (contexts + slots - 1) / slots * (2600 + tiles * 2200);
     const long long pieces = (contexts * tiles * 2200 + contexts * 2600) / slots + 2200 + 2600;
-    return tiles <= 16 && (whole > memory ? whole : memory) <= 7000 + (pieces > memory ? pieces : memory);
+    return tiles <= limit && (whole > memory ? whole : memory) <= 7000 + (pieces > memory ? pieces : memory);
+}
+
+// Rows of a row tile of this kernel for so many query rows of a sequence.
+static int tile_rows(long long want) {
+    if (want <= 4) return 4;
+    const long long tiles = (want + 31) / 32, each = (want + tiles - 1) / tiles;
+    return (int)((each + 7) / 8 * 8);
+}
+
+// This kernel, or the one for many queries (128 rows of a (sequence, kv head) to a CTA, no splitting of long contexts)?  In cycles, two CTAs
+// per SM.  This one: 17000 around it all, 10000 for a tile of 128 tokens and up to 32 rows; lengths are taken to be uneven, half of the
+// longest on average, with a tile's worth for each context.  The other: 10000 for an item, and 2100 for 64 keys, 2700 when two
+// items share an SM.  Measured, us, this one : the other (sequences x new tokens of four heads a kv head, context):
+//   64 x 8, 200..2000    50 : 50     256 x 8, 200..450   62 : 64     19 x 8, 40..4450   36 : 80     4 x 8, 8000     33 : 139
+//   64 x 16, 200..2000   96 : 55     256 x 16, 200..450  121 : 68    19 x 12, 40..4450  43 : 80     2 x 16, 30000   57 : 498
+//   1 x 16, 200          20 : 10     1 x 32, 200         33 : 10     19 x 24, 40..4450  67 : 80     64 x 4, 200..2000  33 : 49
+// Up to 16 rows it is always this one.
+static bool few_rows(const Kv8Attend &a, long long want, int max_len) {
+    if (a.b.num_seqs > MAX_SEQS) return false;
+    // units are counted in 32 bits
+    const long long groups = (long long)a.b.max_tokens / kKv8Group + 2 * TILE_GROUPS;
+    const long long most = ((long long)a.b.total_new * a.group / tile_rows(want) + a.b.num_seqs) * a.b.kv_heads;
+    if (most > 0x7FFFFFFFLL / groups) return false;
+    if (want <= 16) return true;
+    const long long contexts = (long long)a.b.num_seqs * a.b.kv_heads, slots = 2LL * num_sms();
+    long long tokens = max_len < a.b.max_tokens ? max_len : a.b.max_tokens, few_tokens = tokens;
+    if (a.window > 0) {
+        const long long seen = (long long)a.window + a.sinks + 2 * kKv8Group;
+        if (seen + 128 / a.group < tokens) tokens = seen + 128 / a.group;
+        if (seen + want / a.group < few_tokens) few_tokens = seen + want / a.group;      // a row tile reads what any row of the sequence sees
+    }
+    const long long units = contexts * ((want + 31) / 32) * ((few_tokens + SOFTMAX - 1) / SOFTMAX + 2) / 2;
+    const long long few = 17000 + (units + slots - 1) / slots * 10000;
+    const long long items = contexts * ((want + 127) / 128), steps = (tokens + 63) / 64;
+    const long long many = (items + slots - 1) / slots * (10000 + steps * (items > slots / 2 ? 2700 : 2100));
+    return few <= many;
 }
 
 bool kv8_attention_launch(const Kv8Attend &a, int max_new, int max_len, void *workspace, cudaStream_t st, int &launches) {
     const long long want = (long long)max_new * a.group;
-    if (want > 32) {
+    if (!few_rows(a, want, max_len)) {
         launches = 1;
         return kv8_prefill_launch(a, st);
     }
-    if (a.b.num_seqs > MAX_SEQS) return false;
-    const int rows = want <= 4 ? 4 : (int)(want + 7) / 8 * 8;
-    // units are counted in 32 bits
-    const long long groups = (long long)a.b.max_tokens / kKv8Group + 2 * TILE_GROUPS;
-    const long long most = ((long long)a.b.total_new * a.group / rows + a.b.num_seqs) * a.b.kv_heads;
-    if (most > 0x7FFFFFFFLL / groups) return false;
+    const int rows = tile_rows(want);
     Params p;
     memset(&p, 0, sizeof(p));
     const uint64_t pool_rows = (uint64_t)a.b.num_blocks * a.b.kv_heads * a.b.block_size;

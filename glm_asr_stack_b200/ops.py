@@ -371,7 +371,7 @@ def kv8_attention(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
 
     query [tokens, q_heads, 128] bf16; the rest as in kv8_append.  The query at position p sees the positions j <= p with
     window == 0, or p - j < window, or j < sinks; one that sees nothing gets zeros.  max_new / max_len: the most new tokens and
-    the longest sequence to expect -- they choose kernels, not results (default: all rows / the table's width).  scale defaults to
+    the longest sequence to expect -- they choose kernels, not results (default: the mean / the table's width).  scale defaults to
     128 ** -0.5.  Rows behind cu_new[num_seqs] are left as they are.  out must not overlap query."""
     cache, device, kv_heads, block_size = _kv8_cache(k_cache, v_cache, k_scale, v_scale)
     n, max_blocks = _kv8_batch(block_tables, seq_lens, cu_new, device)
@@ -394,7 +394,7 @@ def kv8_attention(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
         size = _kv8_workspace_bytes[device] = lib.glmasr_kv8_attention_workspace()
     workspace = torch.empty(size, dtype=torch.uint8, device=query.device)
     if lib.glmasr_kv8_attention(o, ldo, q, ldq, cache, block_tables.data_ptr(), max_blocks, seq_lens.data_ptr(), cu_new.data_ptr(), n, tokens, q_heads,
-                                tokens if max_new is None else max_new, max_blocks * block_size if max_len is None else max_len, window, sinks,
+                                (tokens + n - 1) // n if max_new is None else max_new, max_blocks * block_size if max_len is None else max_len, window, sinks,
                                 _KV8_SCALE if scale is None else scale, workspace.data_ptr(), size) != 0:
         raise ValueError("glmasr_kv8_attention rejected the arguments")
     used = 0 if _stream is None else _stream.cuda_stream
