@@ -207,7 +207,7 @@ def test_a_few_queries_each(new, ctx, kv_heads, group, window, sinks):
     b = Batch(new, ctx, kv_heads, group, 16)
     q = b.rows(b.heads, extra=2)
     # max_new below what comes: several tiles of rows; right; far above: the kernel for many queries
-    for max_new, max_len in ((1, 2000), (max(new), 600), (max(new), 50_000), (200, 600)):
+    for max_new, max_len in ((1, 2000), (max(new), 600), (max(new), 50_000), (100_000, 600)):
         out = attend(b, q, window, sinks, max_new=max_new, max_len=max_len)
         check_attention(b, q, out, window, sinks)
         assert torch.all(out[b.total:] == 7)
@@ -219,9 +219,74 @@ def test_a_few_queries_each(new, ctx, kv_heads, group, window, sinks):
 def test_many_queries_each(new, ctx, kv_heads, group, page, window, sinks):
     b = Batch(new, ctx, kv_heads, group, page)
     q = b.rows(b.heads, extra=1)
-    out = attend(b, q, window, sinks)
-    check_attention(b, q, out, window, sinks, rows=[0, 1, 2, 31, 32, 33, 41, 69, 127, 128, 131, 171, 299])
-    assert torch.all(out[b.total:] == 7)
+    for more in ({}, {"max_new": 100_000}):
+        out = attend(b, q, window, sinks, **more)
+        check_attention(b, q, out, window, sinks, rows=[0, 1, 2, 31, 32, 33, 41, 69, 127, 128, 131, 171, 299])
+        assert torch.all(out[b.total:] == 7)
+
+
+def test_short_and_long_sequences_together():
+    """Contexts of a tile or less between long ones, cut into pieces that begin and end anywhere."""
+    rng = np.random.default_rng(8)
+    ctx = [int(n) for n in np.where(rng.random(60) < 0.8, rng.integers(0, 140, 60), rng.integers(2000, 5000, 60))]
+    for new, group in ((1, 4), (1, 8), (4, 8)):
+        b = Batch([new] * 60, ctx, 2, group, 16, missing=[(5, 0)])
+        b.lens[7] = b.lens[40] = 0                            # nothing to see
+        q = b.rows(b.heads)
+        check_attention(b, q, attend(b, q, max_new=new, max_len=5000))
+
+
+def test_rows_of_a_projection_and_into_wider_rows():
+    b = Batch([3, 0, 70], [20, 4, 9], 2, 4, 16)
+    q = b.rows(b.heads + 4)
+    pool, tables, lens, cu = b.device()
+    for max_new in (3, 100_000):
+        out = torch.full((b.total + 2, 2 * b.heads, 128), 7.0, dtype=torch.bfloat16, device="cuda")
+        got = ops.kv8_attention(dev(q)[:, 2:2 + b.heads], *pool, tables, lens, cu, max_new=max_new, out=out[:b.total, b.heads:])
+        check_attention(b, q[:, 2:2 + b.heads], got, rows=[0, 1, 2, 33, 69])
+        assert torch.all(out[:, :b.heads] == 7) and torch.all(out[b.total:] == 7)
+
+
+def test_a_prefix_that_sequences_share():
+    b = Batch([1, 2, 1], [200, 150, 90], 2, 4, 16)
+    b.tables[1, :6], b.tables[2, :5] = b.tables[0, :6], b.tables[0, :5]
+    q = b.rows(b.heads)
+    for max_new, max_len in ((2, 300), (2, 50_000), (100_000, 300)):
+        check_attention(b, q, attend(b, q, max_new=max_new, max_len=max_len))
+
+
+@pytest.mark.parametrize("new,ctx", [(1, 40), (2, 7)])
+def test_more_sequences_than_one_line_of_work_has(new, ctx):
+    n = 4500
+    b = Batch([new] * n, [ctx + i % 30 for i in range(n)], 1, 2, 16)
+    q, k, v = b.rows(2), b.rows(1), b.rows(1)
+    out = attend(b, q, max_new=new, max_len=80)
+    pool, tables, lens, cu = b.device()
+    for i in range(0, n, 113):
+        r = slice(int(b.cu[i]), int(b.cu[i]) + new)
+        for t in range(new):
+            want, tol = ref.attend(q[r][t:t + 1], b.codes[0], b.scales[0], b.codes[1], b.scales[1], b.tables[i], b.lens[i] - new + t + 1)
+            assert np.all(np.abs(out[r][t:t + 1].float().cpu().numpy() - want) <= tol)
+    ops.kv8_append(*pool, dev(k), dev(v), tables, lens, cu)
+    check_append(b, k, v, 10000.0, pool=pool)
+
+
+def test_a_pool_of_more_than_4_gib():
+    """Pages whose byte offset in the pool does not fit 32 bits."""
+    b = Batch([1, 20, 90], [70, 33, 5], 1, 4, 16)
+    first = (1 << 32) // (16 * 128) + 7
+    small, tables, lens, cu = b.device()
+    big = tuple(torch.empty((first + b.blocks,) + t.shape[1:], dtype=t.dtype, device="cuda") for t in small)
+    for x, t in zip(big, small):
+        x[first:].view(torch.uint8).copy_(t.view(torch.uint8))
+    tables = torch.where(tables >= 0, tables + first, tables)
+    q, k, v = b.rows(4), b.rows(1), b.rows(1)
+    for max_new in (1, 100_000):
+        out = ops.kv8_attention(dev(q), *big, tables, lens, cu, max_new=max_new)
+        check_attention(b, q, out, rows=[0, 1, 19, 77, 89])
+    ops.kv8_append(*big, dev(k), dev(v), tables, lens, cu)
+    check_append(b, k, v, 10000.0, pool=tuple(t[first:] for t in big))
+    assert ops.status() == 0
 
 
 @pytest.mark.parametrize("new", [1, 3, 70])
