@@ -14,14 +14,15 @@
 // Bound: the two products are 2 x 128 x 64 x 128 multiply-adds a step, 512 cycles at the tensor cores' nominal rate, and the exponentials 512
 // of the special-function units.  The softmax of a step is a chain of some 2000 cycles, so two CTAs share an SM, and a CTA's scores of
 // the next step are computed under its softmax: tensor memory has two of S and one of O.  (128 keys per step with one S: 382 us
-// where this takes 335, two sequences of 2000 new tokens behind 5000; 128 columns of S are all that O leaves of the half of
-// tensor memory that a CTA has.  Two threads per row, eight warps of softmax: 386 there, and 63 us instead of 71 for 25 prompts of 400.)
+// where this takes 345, two sequences of 2000 new tokens behind 5000; 128 columns of S are all that O leaves of the half of
+// tensor memory that a CTA has.  Two threads per row, eight warps of softmax: 386.)
 //   warp 8      producer: the work items, K and V tiles (a TMA box of 2 KB per group of 16 keys), scales of each step; places in the pool are
 //               looked up 8 steps ahead, which is worth 60 us there
 //   warp 9      products; scores [0, 64) and [64, 128), output [128, 256) of tensor memory, P as f16 over the scores it was made from
 //   warps 4-7   V of a step as f16 (or bf16)
-//   warps 0-3   softmax: thread = row = lane of tensor memory; it also splits its row of queries, which for the next item are on their way
-//               while the last sum of the present one is waited for, and brings out its row of the output
+//   warps 0-3   softmax: thread = row = lane of tensor memory; it also splits its row of queries and brings out its row of the output.  The
+//               queries of the next item are asked for under its last softmax and split before its output goes out, so that the
+//               products of the next item run meanwhile (25 prompts of 400 tokens: 61.5 us, 71 one after the other)
 // (warps 10 and 11 only give their registers to the softmax.)  The loops are kept rolled up: fully unrolled, the kernel was 92 KB of code
 // and its softmax waited for instructions, 30 cycles a key instead of 21.
 // The grid has a CTA for every work item there could be; those that run take over the items of those that have not started.
@@ -68,7 +69,7 @@ struct StepInfo {
     uint32_t poisoned;                        // groups whose V scale is not a number
 };
 struct Smem {
-    uint8_t q[2][QT * kKv8Dim];               // hi, lo; before that the row as it came, dims 0..63 and 64..127
+    uint8_t q[2][QT * kKv8Dim];               // hi, lo; before that the row as it came, even and odd eights of its dims
     uint8_t k[2][KT * kKv8Dim], raw[2][KT * kKv8Dim];       // codes of K and V
     uint8_t v[2][2][KT * 128];                // f16, two boxes of 64 dims
     uint8_t stage[4][32 * 64];                // 32 columns of a warp's output rows on their way out
@@ -437,51 +438,56 @@ __global__ void __launch_bounds__(THREADS, 2) kv8_prefill_kernel(const __grid_co
 #pragma unroll 4
             for (int i = 0; i < 32; i += 2) {
                 const int r = warp * 32 + i + (lane >> 4), row = min(r, next.rows - 1) + next.row0, tok = a.by_group.div(row);
-                cp_async16_zfill(smem_u32(sm.q[part >> 3]) + swizzled(r, (part & 7) * 16),
+                cp_async16_zfill(smem_u32(sm.q[part & 1]) + swizzled(r, (part >> 1) * 16),
                         a.query + (long long)(next.first_token + tok) * a.ldq + (size_t)(next.head * a.group + row - tok * a.group) * kKv8Dim + part * 8, r < next.rows);
             }
             cp_async_commit();
             return true;
         };
+        // Queries of the next item: 2^shift brings the largest element to [2^7, 2^8) (one below 2^-119 less far); a row that is not finite
+        // gets NaN scores by its scale.  16 dims of this thread's row are split into the 32 bytes they came in.
+        float next_qs = 0.0f;
+        auto split_queries = [&]() {
+            if (next.rows == 0 || next.steps == 0) return;
+            cp_async_wait<0>();
+            __syncwarp();
+            uint32_t big = 0u;
+#pragma unroll 2
+            for (int i = 0; i < 16; ++i) {
+                const uint4 q = *reinterpret_cast<const uint4 *>(sm.q[i & 1] + swizzled(me, (i >> 1) * 16));
+                big = __vmaxu2(big, __vmaxu2(__vmaxu2(q.x & 0x7FFF7FFFu, q.y & 0x7FFF7FFFu), __vmaxu2(q.z & 0x7FFF7FFFu, q.w & 0x7FFF7FFFu)));
+            }
+            big = max(big >> 16, big & 0xFFFFu);
+            const int expo = (int)(big >> 7), shift = expo == 255 ? 0 : min(7 + 127 - expo, 126);
+            const float up = pow2(shift);
+            next_qs = expo == 255 ? __int_as_float(0x7FFFFFFF) : a.scale_log2 * pow2(-shift);
+#pragma unroll 1
+            for (int c = 0; c < 8; ++c) {
+                uint4 *first = reinterpret_cast<uint4 *>(sm.q[0] + swizzled(me, c * 16)), *second = reinterpret_cast<uint4 *>(sm.q[1] + swizzled(me, c * 16));
+                const uint4 q0 = *first, q1 = *second;
+                const uint32_t w[8] = {q0.x, q0.y, q0.z, q0.w, q1.x, q1.y, q1.z, q1.w};
+                uint32_t hi[4] = {0u, 0u, 0u, 0u}, lo[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    float x0 = __uint_as_float(w[e] << 16) * up, x1 = __uint_as_float(w[e] & 0xFFFF0000u) * up;
+                    hi[e >> 1] |= e4m3_split(x0, x1) << (16 * (e & 1));
+                    lo[e >> 1] |= e4m3x2(x0, x1) << (16 * (e & 1));
+                }
+                *first = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                *second = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            }
+            fence_proxy_async_smem();
+            arrive_warp(bar(B_QFULL));
+        };
         bool ok = look_ahead();
+        if (ok) split_queries();
         while (ok && next.rows > 0) {
             info = next;
             const int row = info.row0 + me, tok = a.by_group.div(row);
             const int pos = me < info.rows ? info.start + tok : -1;
-            float m = kNothing, l = 0.0f, qs = 0.0f, vref = 1.0f;
-            if (info.steps > 0) {
-                // 2^shift brings the largest element to [2^7, 2^8) (one below 2^-119 less far); a row that is not finite gets NaN
-                // scores by its scale.
-                cp_async_wait<0>();
-                __syncwarp();
-                uint4 q[16];
-                uint32_t big = 0u;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    q[i] = *reinterpret_cast<const uint4 *>(sm.q[i >> 3] + swizzled(me, (i & 7) * 16));
-                    big = __vmaxu2(big, __vmaxu2(__vmaxu2(q[i].x & 0x7FFF7FFFu, q[i].y & 0x7FFF7FFFu), __vmaxu2(q[i].z & 0x7FFF7FFFu, q[i].w & 0x7FFF7FFFu)));
-                }
-                big = max(big >> 16, big & 0xFFFFu);
-                const int expo = (int)(big >> 7), shift = expo == 255 ? 0 : min(7 + 127 - expo, 126);
-                const float up = pow2(shift);
-                qs = expo == 255 ? __int_as_float(0x7FFFFFFF) : a.scale_log2 * pow2(-shift);
-#pragma unroll
-                for (int c = 0; c < 8; ++c) {                 // 16 dims
-                    uint32_t hi[4] = {0u, 0u, 0u, 0u}, lo[4] = {0u, 0u, 0u, 0u};
-                    const uint32_t w[8] = {q[2 * c].x, q[2 * c].y, q[2 * c].z, q[2 * c].w, q[2 * c + 1].x, q[2 * c + 1].y, q[2 * c + 1].z, q[2 * c + 1].w};
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        float x0 = __uint_as_float(w[e] << 16) * up, x1 = __uint_as_float(w[e] & 0xFFFF0000u) * up;
-                        hi[e >> 1] |= e4m3_split(x0, x1) << (16 * (e & 1));
-                        lo[e >> 1] |= e4m3x2(x0, x1) << (16 * (e & 1));
-                    }
-                    const uint32_t at = swizzled(me, c * 16);
-                    *reinterpret_cast<uint4 *>(sm.q[0] + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                    *reinterpret_cast<uint4 *>(sm.q[1] + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-                }
-                fence_proxy_async_smem();
-                arrive_warp(bar(B_QFULL));
-            }
+            const float qs = next_qs;
+            float m = kNothing, l = 0.0f, vref = 1.0f;
+            if (info.steps == 0) ok = look_ahead();
             for (int j = 0; j < info.steps; ++j, ++t) {
                 const int s = (int)(t & 1u);
                 ok = wait(B_STEP + (int)(t % STEPS), t / STEPS) && wait(B_SFULL + s, t >> 1);
@@ -498,6 +504,10 @@ __global__ void __launch_bounds__(THREADS, 2) kv8_prefill_kernel(const __grid_co
                 float factor = j > 0 ? st.vstep : 1.0f;
                 vref = st.vref;
                 tmem_ld_wait();
+                if (j == info.steps - 1) {                        // the last scores: the queries are done with
+                    ok = look_ahead();
+                    if (!ok) break;
+                }
                 if (st.plain == 0) {
                     // scores times their scales here, -inf for keys that this row does not see
 #pragma unroll
@@ -570,8 +580,7 @@ __global__ void __launch_bounds__(THREADS, 2) kv8_prefill_kernel(const __grid_co
                 arrive_warp(bar(B_PFULL + s));
             }
             if (!ok) break;
-            ok = look_ahead();
-            if (!ok) break;
+            split_queries();                                      // so that the next item's scores come while this one's output goes
             if (info.steps > 0) {
                 ok = wait_sum(t - 1);
                 if (!ok) break;
