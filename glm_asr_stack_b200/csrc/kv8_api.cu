@@ -84,7 +84,6 @@ extern "C" int glmasr_kv8_attention(uint16_t *out, long long ldo, const uint16_t
     if ((long long)total_new * q_heads > 0x7FFFFF00LL) return -1;                // rows are numbered in 32 bits
     a.group = q_heads / a.b.kv_heads;
     a.by_group = FastDiv(a.group);
-    a.by_q_heads = FastDiv(q_heads);
     a.window = window >= a.b.max_tokens ? 0 : window;              // one that reaches past the table leaves nothing out
     a.sinks = sinks < a.b.max_tokens ? sinks : a.b.max_tokens;
     a.scale_log2 = scale * 1.4426950408889634f;

@@ -16,7 +16,7 @@ struct Kv8Attend {
     long long ldq, ldo;
     Kv8Batch b;
     int group;                    // query heads per kv head
-    FastDiv by_group, by_q_heads;
+    FastDiv by_group;
     int window, sinks;            // window 0: no limit
     float scale_log2;             // softmax scale * log2(e)
 };

@@ -430,9 +430,10 @@ int glmasr_kv8_append(const glmasr_kv8_cache *cache, const uint16_t *key, long l
  * position p sees the positions j <= p with window == 0, or p - j < window, or j < sinks.  A query that sees nothing gets zeros.
  * out, query: bf16 [total_new, q_heads * 128] with row pitches ldo, ldq (multiples of 8; 16-byte aligned); q_heads a multiple of
  * kv_heads.  scale: of the scores, before the softmax.  max_new (new tokens of a sequence) and max_len (tokens of a sequence)
- * say what to expect: they choose kernels and never change what is computed.
- * workspace: glmasr_kv8_attention_workspace() bytes (of the current device's kind) of device memory, 16-byte aligned, contents irrelevant, not shared
- * with a call that may run at the same time.  num_seqs <= 4096.  Returns 0, or -1 on bad arguments or a launch failure. */
+ * say what to expect: they choose kernels (which differ in the order of sums and in rounding), never what is seen or computed.
+ * workspace: glmasr_kv8_attention_workspace() bytes (for the current device) of device memory, 16-byte aligned, contents irrelevant,
+ * not shared with a call that may run at the same time.  out must not overlap query.  Returns 0, or -1 on bad arguments or a
+ * launch failure. */
 long long glmasr_kv8_attention_workspace(void);
 int glmasr_kv8_attention(uint16_t *out, long long ldo, const uint16_t *query, long long ldq, const glmasr_kv8_cache *cache,
                          const int *block_tables, int max_blocks, const int *seq_lens, const int *cu_new, int num_seqs,
