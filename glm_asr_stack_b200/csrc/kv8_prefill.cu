@@ -50,7 +50,7 @@ constexpr float kF16Range = 1.0f / 32.0f;     // of V scales
 static_assert(GROUPS == 4, "a step's K scales are read as one float4");
 constexpr int STEPS = 4;                      // steps whose scales and lengths are kept
 
-enum : int { B_QFULL = 0, B_OFREE, B_NEXT, B_KFULL, B_KEMPTY = B_KFULL + 2, B_RFULL = B_KEMPTY + 2, B_REMPTY = B_RFULL + 2, B_VFULL = B_REMPTY + 2, B_SFULL = B_VFULL + 2,
+enum : int { B_QFULL = 0, B_OFREE, B_NEXT, B_KFULL, B_RFULL = B_KFULL + 2, B_REMPTY = B_RFULL + 2, B_VFULL = B_REMPTY + 2, B_SFULL = B_VFULL + 2,
              B_PFULL = B_SFULL + 2, B_INFO = B_PFULL + 2, B_INFOFREE = B_INFO + 2, B_STEP = B_INFOFREE + 2, B_PVDONE = B_STEP + STEPS, B_COUNT = B_PVDONE + STEPS };
 
 struct ItemInfo {
@@ -140,7 +140,6 @@ __global__ void __launch_bounds__(THREADS, 2) kv8_prefill_kernel(const __grid_co
         mbar_init(bar(B_NEXT), 1);
         for (int i = 0; i < 2; ++i) {
             mbar_init(bar(B_KFULL + i), 1);
-            mbar_init(bar(B_KEMPTY + i), 1);
             mbar_init(bar(B_RFULL + i), 1);
             mbar_init(bar(B_REMPTY + i), 4);
             mbar_init(bar(B_VFULL + i), 4);
@@ -220,7 +219,7 @@ __global__ void __launch_bounds__(THREADS, 2) kv8_prefill_kernel(const __grid_co
                         const int s = (int)(t & 1u), slot = lane % GROUPS;
                         const bool mine = lane / GROUPS == g % 32 / GROUPS, load = mine && place >= 0;
                         const uint32_t bytes = (uint32_t)__popc(__ballot_sync(0xFFFFFFFFu, load)) * GROUP_BYTES;
-                        ok = wait(B_KEMPTY + s, (t >> 1) ^ 1u);
+                        ok = wait(B_SFULL + s, (t >> 1) ^ 1u);       // the scores of the keys before, in their place, are there
                         if (!ok) break;
                         if (leader) mbar_expect_tx(bar(B_KFULL + s), bytes);
                         __syncwarp();
@@ -336,7 +335,6 @@ __global__ void __launch_bounds__(THREADS, 2) kv8_prefill_kernel(const __grid_co
 #pragma unroll
                             for (int k = 0; k < 8; ++k)
                                 umma_f8(tmem + (uint32_t)(s * KT), smem_desc_sw128(smem_u32(sm.q[k >> 2])) + (uint64_t)(((k & 3) * 32) >> 4), bd + (uint64_t)(((k & 3) * 32) >> 4), idesc_s, k > 0 ? 1u : 0u);
-                            umma_commit(bar(B_KEMPTY + s));
                             umma_commit(bar(B_SFULL + s));
                         }
                         __syncwarp();
@@ -367,7 +365,10 @@ __global__ void __launch_bounds__(THREADS, 2) kv8_prefill_kernel(const __grid_co
     } else if (warp >= 4) {
         // ================================ V ================================
         fewer_registers<REGS_VALUES>();
-        const int w4 = warp - 4, chunk = lane & 7, in_group = w4 * 4 + (lane >> 3);       // a thread has 16 dims of one key of each group
+        // A thread has 16 dims of one key of each group.  Eight threads that access shared memory together have four chunks of a key a and
+        // the same of key a ^ 5: eight different places among the 128 bytes of a row, of codes as well as of the result.
+        const int pair = (threadIdx.x >> 4) & 7, a_key = (pair & 3) + (pair >> 2) * 8, in_group = (lane & 4) != 0 ? a_key ^ 5 : a_key;
+        const int chunk = (lane & 3) + ((lane >> 3) & 1) * 4;
         const uint32_t src0 = smem_u32(sm.raw[0]) + (uint32_t)(in_group * kKv8Dim + ((chunk ^ (in_group & 7)) << 4));
         // the 16-byte chunks 2 (chunk % 4) and the next of the row, swizzled: they differ in the lowest bit
         const uint32_t dst0 = smem_u32(sm.v[0][chunk >> 2]) + (uint32_t)(in_group * 128 + ((((chunk & 3) * 2) ^ (in_group & 7)) << 4));
