@@ -289,6 +289,35 @@ def test_a_pool_of_more_than_4_gib():
     assert ops.status() == 0
 
 
+def test_a_batch_without_a_new_token():
+    """All of the packed rows lie behind the last sequence: nothing is read, written or appended."""
+    b = Batch([0, 0, 0], [5, 0, 40], 2, 4, 16)
+    pool, tables, lens, cu = b.device()
+    before = [t.clone() for t in pool]
+    q, kv = (torch.full((9, h, 128), float("nan"), dtype=torch.bfloat16, device="cuda") for h in (8, 2))
+    for max_new, max_len in ((1, 100), (1, 50_000), (100_000, 100)):
+        out = torch.full_like(q, 7.0)
+        ops.kv8_attention(q, *pool, tables, lens, cu, max_new=max_new, max_len=max_len, out=out)
+        assert torch.all(out == 7)
+    qo = torch.full_like(q, 7.0)
+    ops.kv8_append(*pool, kv, kv, tables, lens, cu, query=q, query_out=qo)
+    assert torch.all(qo == 7) and all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(before, pool))
+    assert ops.status() == 0
+
+
+@pytest.mark.parametrize("new", [1, 7, 90])
+def test_pages_a_window_has_left_behind(new):
+    b = Batch([new, new], [400, 333], 2, 4, 16)
+    for i in range(2):
+        for j in range(2, (b.ctx[i] - 60 + 1) // 16):         # no query sees them; the first two have the first tokens
+            b.tables[i, j] = -1 if j % 2 else b.blocks + 9
+    q = b.rows(b.heads)
+    full = Batch([new, new], [400, 333], 2, 4, 16)
+    for max_new, max_len in ((new, 500), (new, 50_000), (100_000, 500)):
+        out = attend(b, q, 60, 20, max_new=max_new, max_len=max_len)
+        check_attention(full, q, out, 60, 20, rows=[0, 1, 6, 31, 60, 89])
+
+
 @pytest.mark.parametrize("new", [1, 3, 70])
 def test_what_is_not_there(new):
     """Missing pages, lengths below the number of new tokens, positions behind the table: not seen, and what lies in unused
