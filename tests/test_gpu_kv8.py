@@ -236,6 +236,28 @@ def test_short_and_long_sequences_together():
         check_attention(b, q, attend(b, q, max_new=new, max_len=5000))
 
 
+@pytest.mark.parametrize("kv_heads,group", [(4, 4), (4, 8), (2, 16)])
+def test_more_contexts_than_places_for_them(kv_heads, group):
+    """CTAs take over further contexts, the longest first: each is worked on once, whatever the lengths and the hints."""
+    rng = np.random.default_rng(9)
+    n = 330
+    new = (rng.random(n) < 0.9).astype(int).tolist()
+    b = Batch(new, rng.integers(0, 420, n).tolist(), kv_heads, group, 16)
+    b.lens[3] = b.lens[200] = 0
+    q = b.rows(b.heads)
+    for max_len in (1, 500):
+        check_attention(b, q, attend(b, q, max_new=1, max_len=max_len))
+    more = Batch([3] * 150, rng.integers(0, 2500, 150).tolist(), kv_heads, group, 16)      # longer, and more rows, than said
+    q = more.rows(more.heads)
+    out = attend(more, q, max_new=1, max_len=100)
+    for i in range(0, 150, 7):
+        for t in range(3):
+            r = slice(3 * i + t, 3 * i + t + 1)
+            want, tol = ref.attend(q[r], more.codes[0], more.scales[0], more.codes[1], more.scales[1], more.tables[i], more.lens[i] - 2 + t)
+            assert np.all(np.abs(out[r].float().cpu().numpy() - want) <= tol)
+    assert not torch.any(torch.all(out[:more.total] == 0, dim=2))
+
+
 def test_rows_of_a_projection_and_into_wider_rows():
     b = Batch([3, 0, 70], [20, 4, 9], 2, 4, 16)
     q = b.rows(b.heads + 4)
