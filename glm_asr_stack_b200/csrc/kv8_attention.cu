@@ -113,7 +113,7 @@ __device__ __forceinline__ void store_columns(uint32_t t, const uint32_t (&r)[V]
 // The line of work.  rows = query rows (new token, head of the group) a context has at most; a sequence with more of them has
 // several row tiles.  Units of (sequence, row tile, kv head), in that order: its visible groups of 16 tokens, and behind them as many
 // empty ones as its last tile lacks and one more tile has, for what a context costs by itself.  (Without those a piece of
-// short contexts takes twice as long as the others: 47 us instead of 29 for 19 sequences of 40 to 4450 tokens, 5 new.)
+// short contexts takes twice as long as the others: 47 us instead of 31 for 19 sequences of 40 to 4450 tokens, 5 new.)
 struct SeqWork {
     int row0, n, len, start, tiles;   // first packed row, new tokens, tokens in all, position of the first new one, row tiles
     Kv8Span span;                     // what any of its queries sees
