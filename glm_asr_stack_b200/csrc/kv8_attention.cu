@@ -13,7 +13,7 @@
 //            beside the running maximum m of the softmax: W, the running maximum of x_j + log2 v_scale_j.  The weight
 //            2^(x_j + log2 v_scale_j - W + 6), at most 2^8, is split as p = hi + 2^-4 lo: off by 6.6e-4 of its size (rms; bf16: 1.6e-3) or 2^-20
 //            of the largest, whichever is more.
-//   lazily   m and W are touched when a term has grown past 2^8 m or 2^2 W: an ordinary tile needs one vote of its four warps.
+//   lazily   m and W are touched when a term has grown past 2^8 m or 2^2 W: an ordinary tile needs one vote of the softmax's warps.
 //   split    Two ways to deal out the work, chosen on the host (see deal_whole()).  Whole: one CTA of the grid for each (sequence, kv
 //            head); those that run take over the work of those that have not started, and there is nothing to join.  Pieces: all
 //            visible groups of 16 tokens of all (sequence, kv head) pairs form one line, cut into equal pieces, one per CTA, so that
@@ -218,8 +218,8 @@ __global__ void __launch_bounds__(threads(R), max_ctas(R)) kv8_attend_kernel(con
         return;
     }
     if (threadIdx.x == 0) {
-        mbar_init(bar(B_PFULL), WORKERS);
-        mbar_init(bar(B_OFREE), WORKERS);
+        mbar_init(bar(B_PFULL), WORKERS / 32);
+        mbar_init(bar(B_OFREE), WORKERS / 32);
         mbar_init(bar(B_NEXT), 1);
         for (int i = 0; i < 2; ++i) {
             mbar_init(bar(B_KFULL + i), 1);
@@ -229,7 +229,7 @@ __global__ void __launch_bounds__(threads(R), max_ctas(R)) kv8_attend_kernel(con
             mbar_init(bar(B_SFULL + i), 1);
             mbar_init(bar(B_SCALES + i), 1);
             mbar_init(bar(B_CFULL + i), 1);
-            mbar_init(bar(B_CEMPTY + i), 1 + WORKERS);        // the last product of scores and the results
+            mbar_init(bar(B_CEMPTY + i), 1 + WORKERS / 32);        // the last product of scores and the results
         }
         sm.abort = 0;
         fence_mbar_init();
@@ -685,7 +685,7 @@ __global__ void __launch_bounds__(threads(R), max_ctas(R)) kv8_attend_kernel(con
                 }
                 fence_proxy_async_smem();
                 tc_fence_before();
-                mbar_arrive(bar(B_PFULL));
+                mbar_arrive_warp(bar(B_PFULL));
             }
 
             // ---- the result of these groups ----
@@ -727,7 +727,7 @@ __global__ void __launch_bounds__(threads(R), max_ctas(R)) kv8_attend_kernel(con
             load_columns<V>(t_o + (uint32_t)(R + base), low);
             tmem_ld_wait();
             tc_fence_before();
-            mbar_arrive(bar(B_OFREE));
+            mbar_arrive_warp(bar(B_OFREE));
             (void)any_of_softmax<WORKERS>(false);
             float *to = p.part.acc + (size_t)(c.slot < 0 ? 0 : c.slot) * U * kKv8Dim + me;
 #pragma unroll
@@ -737,7 +737,7 @@ __global__ void __launch_bounds__(threads(R), max_ctas(R)) kv8_attend_kernel(con
                 if (c.slot < 0) c.out[base + r][me] = __float2bfloat16(o * sm.factor[base + r][0]);
                 else to[(base + r) * kKv8Dim] = o;
             }
-            mbar_arrive(bar(B_CEMPTY + cs));
+            mbar_arrive_warp(bar(B_CEMPTY + cs));
             // the rows' state and factors are written again after the next context's first vote
         }
     }

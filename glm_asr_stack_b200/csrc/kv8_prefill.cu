@@ -114,11 +114,6 @@ __device__ __forceinline__ void scale_columns(uint32_t t_o, float f) {
     }
 }
 
-// One arrival for the 32 threads of a warp, each of which is done.
-__device__ __forceinline__ void arrive_warp(uint32_t bar) {
-    __syncwarp();
-    if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
-}
 template <int N>
 __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N>
@@ -380,7 +375,7 @@ __global__ void __launch_bounds__(THREADS, 2) kv8_prefill_kernel(const __grid_co
             const int rows = sm.item[is].rows, steps = sm.item[is].steps;
             if (rows == 0) break;
             ++items;
-            arrive_warp(bar(B_INFOFREE + is));
+            mbar_arrive_warp(bar(B_INFOFREE + is));
             for (int j = 0; j < steps; ++j, ++t) {
                 const int s = (int)(t & 1u);
                 const StepInfo &st = sm.step[t % STEPS];
@@ -414,9 +409,9 @@ __global__ void __launch_bounds__(THREADS, 2) kv8_prefill_kernel(const __grid_co
                     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
                     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at ^ 16u), "r"(h[4]), "r"(h[5]), "r"(h[6]), "r"(h[7]) : "memory");
                 }
-                arrive_warp(bar(B_REMPTY + s));
+                mbar_arrive_warp(bar(B_REMPTY + s));
                 fence_proxy_async_smem();
-                arrive_warp(bar(B_VFULL + s));
+                mbar_arrive_warp(bar(B_VFULL + s));
             }
         }
     } else {
@@ -433,7 +428,7 @@ __global__ void __launch_bounds__(THREADS, 2) kv8_prefill_kernel(const __grid_co
             next = sm.item[is];
             ++items;
             if (next.rows == 0) return true;
-            arrive_warp(bar(B_INFOFREE + is));
+            mbar_arrive_warp(bar(B_INFOFREE + is));
             if (next.steps == 0) return true;
             const int part = lane & 15;
 #pragma unroll 4
@@ -478,7 +473,7 @@ __global__ void __launch_bounds__(THREADS, 2) kv8_prefill_kernel(const __grid_co
                 *second = make_uint4(lo[0], lo[1], lo[2], lo[3]);
             }
             fence_proxy_async_smem();
-            arrive_warp(bar(B_QFULL));
+            mbar_arrive_warp(bar(B_QFULL));
         };
         bool ok = look_ahead();
         if (ok) split_queries();
@@ -578,7 +573,7 @@ __global__ void __launch_bounds__(THREADS, 2) kv8_prefill_kernel(const __grid_co
                 l += s0 + s1;
                 tmem_st_wait();
                 tc_fence_before();
-                arrive_warp(bar(B_PFULL + s));
+                mbar_arrive_warp(bar(B_PFULL + s));
             }
             if (!ok) break;
             split_queries();                                      // so that the next item's scores come while this one's output goes
@@ -622,7 +617,7 @@ __global__ void __launch_bounds__(THREADS, 2) kv8_prefill_kernel(const __grid_co
             }
             if (info.steps > 0) {
                 tc_fence_before();
-                arrive_warp(bar(B_OFREE));
+                mbar_arrive_warp(bar(B_OFREE));
             }
         }
         cp_async_wait<0>();
