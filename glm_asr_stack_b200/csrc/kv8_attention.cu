@@ -48,7 +48,7 @@ constexpr int MAX_SEQS = 4096;                                // the line's tabl
 constexpr float kTop = 8.0f, kWeightTop = 2.0f, kWeightBase = 6.0f;
 constexpr float kQLo = 1.0f / 32.0f, kPLo = 1.0f / 16.0f;
 
-enum : int { B_KFULL = 0, B_KEMPTY = 2, B_VFULL = 4, B_PVDONE = 6, B_SFULL = 8, B_SCALES = 10, B_CFULL = 12, B_CEMPTY = 14, B_PFULL = 16, B_OFREE = 17, B_NEXT = 18, B_COUNT = 19 };
+enum : int { B_KFULL = 0, B_KEMPTY = 2, B_VFULL = 4, B_PVDONE = 6, B_SFULL = 8, B_SCALES = 10, B_CFULL = 12, B_CEMPTY = 14, B_PFULL = 16, B_OFREE = 17, B_NEXT = 18, B_FIRST = 19, B_COUNT = 20 };
 
 // What the products and the softmax have to know of a context.
 template <int R>
@@ -74,6 +74,7 @@ struct Smem {
     float2 scales[2][TILE_GROUPS];        // K, V
     int tokens[2][TILE_GROUPS];           // of each group that exist
     uint4 next;                           // answer to the question for more work
+    struct { int row0, head, first_token, start; } begin;      // whose queries the CTA's first context has: see split_row
     unsigned long long bars[B_COUNT];
     uint32_t tmem;
     int abort, warp_sum[threads(R) / 32];
@@ -91,6 +92,51 @@ __device__ __forceinline__ bool any_of_softmax(bool x) {
         "selp.u32 %0, 1, 0, q;\n\t}"
         : "=r"(r) : "r"(x ? 1u : 0u), "n"(COUNT) : "memory");
     return r != 0;
+}
+// Query rows are split by QL lanes each (all rows of a small tile at a time, or eight): a lane has dims 8 QL i + 8 (lane % QL) .. + 7.
+constexpr int query_lanes(int rows) { return rows <= 4 ? 8 : 4; }
+// Row r of context cs, which is row `row` of its sequence.
+template <int QL, int R>
+__device__ __forceinline__ void split_row(const Kv8Attend &a, Smem<R> &sm, int cs, int r, bool exists, const uint4 (&q)[16 / QL], int row, int head, int first_token, int start) {
+    const int part = (int)threadIdx.x % QL;
+    uint32_t most = 0u;
+#pragma unroll
+    for (int i = 0; i < 16 / QL; ++i)
+        most = __vmaxu2(most, __vmaxu2(__vmaxu2(q[i].x & 0x7FFF7FFFu, q[i].y & 0x7FFF7FFFu), __vmaxu2(q[i].z & 0x7FFF7FFFu, q[i].w & 0x7FFF7FFFu)));
+#pragma unroll
+    for (int d = 1; d < QL; d <<= 1) most = __vmaxu2(most, __shfl_xor_sync(0xFFFFFFFFu, most, d));
+    most = max(most >> 16, most & 0xFFFFu);
+    // 2^shift brings the largest element to [2^7, 2^8) (one below 2^-119 less far); a row that is not finite gets NaN scores by its scale
+    const int expo = (int)(most >> 7), shift = expo == 255 ? 0 : min(7 + 127 - expo, 126);
+    const float up = pow2(shift);
+#pragma unroll
+    for (int i = 0; i < 16 / QL; ++i) {
+        const uint32_t w[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
+        uint32_t hi[2] = {0u, 0u}, lo[2] = {0u, 0u};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            float x0 = __uint_as_float(w[e] << 16) * up, x1 = __uint_as_float(w[e] & 0xFFFF0000u) * up;
+            hi[e >> 1] |= e4m3_split(x0, x1) << (16 * (e & 1));
+            lo[e >> 1] |= e4m3x2(x0 / kQLo, x1 / kQLo) << (16 * (e & 1));
+        }
+        const int b = i * 8 * QL + part * 8;
+        *reinterpret_cast<uint2 *>(sm.q[cs] + swizzled(r, b)) = make_uint2(hi[0], hi[1]);
+        *reinterpret_cast<uint2 *>(sm.q[cs] + swizzled(R + r, b)) = make_uint2(lo[0], lo[1]);
+    }
+    if (part == 0) {
+        const int tok = a.by_group.div(row);
+        ContextInfo<R> &info = sm.ctx[cs];
+        info.qscale[r] = expo == 255 ? __int_as_float(0x7FFFFFFF) : a.scale_log2 * pow2(-shift);
+        info.pos[r] = exists ? start + tok : -1;
+        info.out[r] = a.out + (long long)(first_token + tok) * a.ldo + (size_t)(head * a.group + row - tok * a.group) * kKv8Dim;
+    }
+}
+template <int QL>
+__device__ __forceinline__ void load_row(const Kv8Attend &a, bool exists, uint4 (&q)[16 / QL], int row, int head, int first_token) {
+    const int tok = a.by_group.div(row);
+    const __nv_bfloat16 *src = a.query + (long long)(first_token + tok) * a.ldq + (size_t)(head * a.group + row - tok * a.group) * kKv8Dim + threadIdx.x % QL * 8;
+#pragma unroll
+    for (int i = 0; i < 16 / QL; ++i) q[i] = exists ? *reinterpret_cast<const uint4 *>(src + i * 8 * QL) : make_uint4(0u, 0u, 0u, 0u);
 }
 // V columns of tensor memory, 32 bits of this lane each
 template <int V>
@@ -113,7 +159,7 @@ __device__ __forceinline__ void store_columns(uint32_t t, const uint32_t (&r)[V]
 // The line of work.  rows = query rows (new token, head of the group) a context has at most; a sequence with more of them has
 // several row tiles.  Units of (sequence, row tile, kv head), in that order: its visible groups of 16 tokens, and behind them as many
 // empty ones as its last tile lacks and one more tile has, for what a context costs by itself.  (Without those a piece of
-// short contexts takes twice as long as the others: 47 us instead of 31 for 19 sequences of 40 to 4450 tokens, 5 new.)
+// short contexts takes twice as long as the others: 47 us instead of 29 for 19 sequences of 40 to 4450 tokens, 5 new.)
 struct SeqWork {
     int row0, n, len, start, tiles;   // first packed row, new tokens, tokens in all, position of the first new one, row tiles
     Kv8Span span;                     // what any of its queries sees
@@ -221,6 +267,7 @@ __global__ void __launch_bounds__(threads(R), max_ctas(R)) kv8_attend_kernel(con
         mbar_init(bar(B_PFULL), WORKERS / 32);
         mbar_init(bar(B_OFREE), WORKERS / 32);
         mbar_init(bar(B_NEXT), 1);
+        mbar_init(bar(B_FIRST), 1);
         for (int i = 0; i < 2; ++i) {
             mbar_init(bar(B_KFULL + i), 1);
             mbar_init(bar(B_KEMPTY + i), 1);
@@ -354,20 +401,14 @@ __global__ void __launch_bounds__(threads(R), max_ctas(R)) kv8_attend_kernel(con
         // of the coming tile, by lane: place in the pool in groups (-1: none) and existing tokens of a group, its scales
         int place = -1, tokens = 0;
         float2 scale = make_float2(0.0f, 0.0f);
-        // queries: QL lanes per row, all rows of a small tile or eight at a time; the first are asked for when a context is entered
-        constexpr int QL = U <= 4 ? 8 : 4, QROWS = 32 / QL, QI = 16 / QL;
-        uint4 q[QI];                                          // dims 8 QL i + 8 (lane % QL) .. + 7
+        // Queries of a context: the softmax's warps split those of the first, all at once; this warp those of the next under the tiles before.
+        // The first rows are asked for when a context is entered.
+        constexpr int QL = query_lanes(U), QROWS = 32 / QL, QI = 16 / QL;
+        uint4 q[QI];
         auto place_of = [&](int r, int &tok) {                // first element of the row's head in a packed row, and the row
             const int row = c.row_tile * U + r;
             tok = a.by_group.div(row);
             return (size_t)(c.head * a.group + row - tok * a.group) * kKv8Dim;
-        };
-        auto ask_queries = [&](int r, uint4 (&q)[QI]) {
-            int tok;
-            const size_t col = place_of(r, tok);
-            const __nv_bfloat16 *src = a.query + (long long)(c.w.row0 + tok) * a.ldq + col + (lane % QL) * 8;
-#pragma unroll
-            for (int i = 0; i < QI; ++i) q[i] = r < rows ? *reinterpret_cast<const uint4 *>(src + i * 8 * QL) : make_uint4(0u, 0u, 0u, 0u);
         };
         for (;;) {
             have = false;
@@ -379,7 +420,7 @@ __global__ void __launch_bounds__(threads(R), max_ctas(R)) kv8_attend_kernel(con
                     rows = min(U, c.w.n * a.group - c.row_tile * U);
                     join.rows = rows;
                     g = c.from;
-                    ask_queries(lane / QL, q);
+                    if (contexts > 0) load_row<QL>(a, lane / QL < rows, q, c.row_tile * U + lane / QL, c.head, c.w.row0);
                 }
                 if (g == c.to) {                              // empty units, or a context in which nothing is visible
                     if (c.w.span.count > 0 || (!p.whole && first_unit != c.unit0)) continue;
@@ -446,45 +487,21 @@ __global__ void __launch_bounds__(threads(R), max_ctas(R)) kv8_attend_kernel(con
                 info.pos_hi = c.w.start + a.by_group.div(c.row_tile * U + rows - 1);
                 info.slot = p.whole || (first_unit == c.unit0 && at >= c.real1) ? -1 : 2 * (int)blockIdx.x + (c.unit0 > begin ? 1 : 0);
             }
+            __syncwarp();
+            if (contexts == 1) {                              // the first
+                if (leader) {
+                    sm.begin = {c.row_tile * U, c.head, c.w.row0, c.w.start};
+                    mbar_arrive(bar(B_FIRST));
+                }
+                __syncwarp();
+                if (!put_v()) break;
+                continue;
+            }
 #pragma unroll 1
             for (int r = lane / QL; r < U; r += QROWS) {
                 uint4 next[QI];
-                if (r + QROWS < U) ask_queries(r + QROWS, next);
-                uint32_t most = 0u;
-#pragma unroll
-                for (int i = 0; i < QI; ++i) {
-                    const uint32_t high = __vmaxu2(__vmaxu2(q[i].x & 0x7FFF7FFFu, q[i].y & 0x7FFF7FFFu), __vmaxu2(q[i].z & 0x7FFF7FFFu, q[i].w & 0x7FFF7FFFu));
-                    most = __vmaxu2(most, high);
-                }
-#pragma unroll
-                for (int d = 1; d < QL; d <<= 1) most = __vmaxu2(most, __shfl_xor_sync(0xFFFFFFFFu, most, d));
-                most = max(most >> 16, most & 0xFFFFu);
-                // 2^shift brings the largest element to [2^7, 2^8) (one below 2^-119 less far); a row that is not finite gets NaN
-                // scores by its scale
-                const int expo = (int)(most >> 7);
-                const int shift = expo == 255 ? 0 : min(7 + 127 - expo, 126);
-                const float up = pow2(shift);
-#pragma unroll
-                for (int i = 0; i < QI; ++i) {
-                    const uint32_t w[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
-                    uint32_t hi[2] = {0u, 0u}, lo[2] = {0u, 0u};
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        float x0 = __uint_as_float(w[e] << 16) * up, x1 = __uint_as_float(w[e] & 0xFFFF0000u) * up;
-                        hi[e >> 1] |= e4m3_split(x0, x1) << (16 * (e & 1));
-                        lo[e >> 1] |= e4m3x2(x0 / kQLo, x1 / kQLo) << (16 * (e & 1));
-                    }
-                    const int b = i * 8 * QL + (lane % QL) * 8;
-                    *reinterpret_cast<uint2 *>(sm.q[cs] + swizzled(r, b)) = make_uint2(hi[0], hi[1]);
-                    *reinterpret_cast<uint2 *>(sm.q[cs] + swizzled(R + r, b)) = make_uint2(lo[0], lo[1]);
-                }
-                if (lane % QL == 0) {
-                    int tok;
-                    const size_t col = place_of(r, tok);
-                    info.qscale[r] = expo == 255 ? __int_as_float(0x7FFFFFFF) : a.scale_log2 * pow2(-shift);
-                    info.pos[r] = r < rows ? c.w.start + tok : -1;
-                    info.out[r] = a.out + (long long)(c.w.row0 + tok) * a.ldo + col;
-                }
+                if (r + QROWS < U) load_row<QL>(a, r + QROWS < rows, next, c.row_tile * U + r + QROWS, c.head, c.w.row0);
+                split_row<QL>(a, sm, cs, r, r < rows, q, c.row_tile * U + r, c.head, c.w.row0, c.w.start);
                 if (r + QROWS < U) {
 #pragma unroll
                     for (int i = 0; i < QI; ++i) q[i] = next[i];
@@ -500,6 +517,7 @@ __global__ void __launch_bounds__(threads(R), max_ctas(R)) kv8_attend_kernel(con
         if (ok && mbar_wait_short(bar(B_CEMPTY + cs), ((contexts >> 1) & 1u) ^ 1u, abort_word, ST_TIMEOUT_ATTENTION) && leader) {
             sm.ctx[cs].groups = 0;                            // the end
             mbar_arrive(bar(B_CFULL + cs));
+            if (contexts == 0) mbar_arrive(bar(B_FIRST));
         }
     } else if (warp == PRODUCTS) {
         // ================================ products ==============================
@@ -563,6 +581,22 @@ __global__ void __launch_bounds__(threads(R), max_ctas(R)) kv8_attend_kernel(con
         const int base = tid / SOFTMAX * V, quarter = warp % 4; // the first of this thread's V rows; its warp's place among those of the tokens
         const uint32_t t_lane = tmem + ((uint32_t)(quarter * 32) << 16);
         const uint32_t t_o = t_lane + 2 * N;
+        {
+            // the queries of the first context, all rows at once
+            constexpr int QL = query_lanes(U);
+            static_assert(U * QL <= WORKERS && U * QL % 32 == 0, "a row for QL lanes, whole warps");
+            const bool ok = mbar_wait_short(bar(B_FIRST), 0u, abort_word, ST_TIMEOUT_ATTENTION);
+            const bool any = sm.ctx[0].groups != 0;
+            if (ok && any && tid < U * QL) {
+                const int r = tid / QL;
+                const bool exists = r < sm.ctx[0].rows;
+                uint4 q[16 / QL];
+                load_row<QL>(a, exists, q, sm.begin.row0 + r, sm.begin.head, sm.begin.first_token);
+                split_row<QL>(a, sm, 0, r, exists, q, sm.begin.row0 + r, sm.begin.head, sm.begin.first_token, sm.begin.start);
+                fence_proxy_async_smem();
+            }
+            if (!any_of_softmax<WORKERS>(!ok) && any && tid == 0) mbar_arrive(bar(B_CFULL));
+        }
         uint32_t t = 0;
         for (uint32_t contexts = 0;; ++contexts) {
             const int cs = (int)(contexts & 1u);
