@@ -297,7 +297,7 @@ def _kv8_cache(k_cache, v_cache, k_scale, v_scale):
     if (len(shape) == 4 and v_cache.shape == shape and k_cache.dtype in _KV8_CODES and v_cache.dtype in _KV8_CODES
             and k_cache.is_contiguous() and v_cache.is_contiguous() and k_scale.dtype is torch.float32 and v_scale.dtype is torch.float32
             and k_scale.shape == v_scale.shape == (shape[0], shape[1], shape[2] // 16) and k_scale.is_contiguous() and v_scale.is_contiguous()
-            and device >= 0 and device == v_cache.get_device() == k_scale.get_device() == v_scale.get_device() == torch.cuda.current_device()):
+            and device >= 0 and device == v_cache.get_device() == k_scale.get_device() == v_scale.get_device() == torch._C._cuda_getDevice()):
         return _KV8_STRUCT.pack(k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), shape[0], shape[2], shape[1],
                                 shape[3]), device, shape[1], shape[2]
     if device < 0:
@@ -392,7 +392,7 @@ def kv8_attention(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
     size = _kv8_workspace_bytes.get(device)
     if size is None:
         size = _kv8_workspace_bytes[device] = lib.glmasr_kv8_attention_workspace()
-    workspace = torch.empty(size, dtype=torch.uint8, device=query.device)
+    workspace = seq_lens.new_empty(size // 4)       # a multiple of 256 bytes; cheaper than torch.empty
     if lib.glmasr_kv8_attention(o, ldo, q, ldq, cache, block_tables.data_ptr(), max_blocks, seq_lens.data_ptr(), cu_new.data_ptr(), n, tokens, q_heads,
                                 (tokens + n - 1) // n if max_new is None else max_new, max_blocks * block_size if max_len is None else max_len, window, sinks,
                                 _KV8_SCALE if scale is None else scale, workspace.data_ptr(), size) != 0:
