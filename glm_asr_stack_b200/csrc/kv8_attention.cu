@@ -252,6 +252,9 @@ template <int R, int U>
 __global__ void __launch_bounds__(threads(R), max_ctas(R)) kv8_attend_kernel(const __grid_constant__ Params p) {
     constexpr int N = 2 * R;                                  // columns of both products
     constexpr int SPLIT = split(R), THREADS = threads(R), WORKERS = SPLIT * SOFTMAX, COPIES = WORKERS / 32, PRODUCTS = COPIES + 1;       // the last two: warps
+    // The softmax's warps split the queries of the first context, all rows at once (19 sequences with 4 new tokens behind 300, 16 rows:
+    // 12.1 -> 11.4 us).  Up to 8 rows the copying warp is as quick, and nobody has to be told (6.3 us, 6.6 for one of 60 tokens).
+    constexpr bool SHARED_FIRST = U > 8;
     constexpr int TMEM_COLS = 3 * N <= 64 ? 64 : 3 * N <= 128 ? 128 : 256;     // two score buffers, the accumulator
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     Smem<R> &sm = *reinterpret_cast<Smem<R> *>(smem_raw);
@@ -401,8 +404,7 @@ __global__ void __launch_bounds__(threads(R), max_ctas(R)) kv8_attend_kernel(con
         // of the coming tile, by lane: place in the pool in groups (-1: none) and existing tokens of a group, its scales
         int place = -1, tokens = 0;
         float2 scale = make_float2(0.0f, 0.0f);
-        // Queries of a context: the softmax's warps split those of the first, all at once; this warp those of the next under the tiles before.
-        // The first rows are asked for when a context is entered.
+        // Queries of a context, under the tiles of the one before; the first rows are asked for when it is entered.
         constexpr int QL = query_lanes(U), QROWS = 32 / QL, QI = 16 / QL;
         uint4 q[QI];
         auto place_of = [&](int r, int &tok) {                // first element of the row's head in a packed row, and the row
@@ -420,7 +422,7 @@ __global__ void __launch_bounds__(threads(R), max_ctas(R)) kv8_attend_kernel(con
                     rows = min(U, c.w.n * a.group - c.row_tile * U);
                     join.rows = rows;
                     g = c.from;
-                    if (contexts > 0) load_row<QL>(a, lane / QL < rows, q, c.row_tile * U + lane / QL, c.head, c.w.row0);
+                    if (!SHARED_FIRST || contexts > 0) load_row<QL>(a, lane / QL < rows, q, c.row_tile * U + lane / QL, c.head, c.w.row0);
                 }
                 if (g == c.to) {                              // empty units, or a context in which nothing is visible
                     if (c.w.span.count > 0 || (!p.whole && first_unit != c.unit0)) continue;
@@ -488,7 +490,7 @@ __global__ void __launch_bounds__(threads(R), max_ctas(R)) kv8_attend_kernel(con
                 info.slot = p.whole || (first_unit == c.unit0 && at >= c.real1) ? -1 : 2 * (int)blockIdx.x + (c.unit0 > begin ? 1 : 0);
             }
             __syncwarp();
-            if (contexts == 1) {                              // the first
+            if (SHARED_FIRST && contexts == 1) {
                 if (leader) {
                     sm.begin = {c.row_tile * U, c.head, c.w.row0, c.w.start};
                     mbar_arrive(bar(B_FIRST));
@@ -517,7 +519,7 @@ __global__ void __launch_bounds__(threads(R), max_ctas(R)) kv8_attend_kernel(con
         if (ok && mbar_wait_short(bar(B_CEMPTY + cs), ((contexts >> 1) & 1u) ^ 1u, abort_word, ST_TIMEOUT_ATTENTION) && leader) {
             sm.ctx[cs].groups = 0;                            // the end
             mbar_arrive(bar(B_CFULL + cs));
-            if (contexts == 0) mbar_arrive(bar(B_FIRST));
+            if (SHARED_FIRST && contexts == 0) mbar_arrive(bar(B_FIRST));
         }
     } else if (warp == PRODUCTS) {
         // ================================ products ==============================
@@ -581,8 +583,7 @@ __global__ void __launch_bounds__(threads(R), max_ctas(R)) kv8_attend_kernel(con
         const int base = tid / SOFTMAX * V, quarter = warp % 4; // the first of this thread's V rows; its warp's place among those of the tokens
         const uint32_t t_lane = tmem + ((uint32_t)(quarter * 32) << 16);
         const uint32_t t_o = t_lane + 2 * N;
-        {
-            // the queries of the first context, all rows at once
+        if constexpr (SHARED_FIRST) {
             constexpr int QL = query_lanes(U);
             static_assert(U * QL <= WORKERS && U * QL % 32 == 0, "a row for QL lanes, whole warps");
             const bool ok = mbar_wait_short(bar(B_FIRST), 0u, abort_word, ST_TIMEOUT_ATTENTION);
