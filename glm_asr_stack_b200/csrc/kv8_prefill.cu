@@ -9,8 +9,9 @@
 //                     above 2^8, and only then is O touched.
 //   O += P V          f16 x f16: weights have 11 bits down to 2^-14 of the largest, and are off by 2^-25 of it below.  V's codes become
 //                     f16, times the scale of their block over the largest scale of the item so far (exact: a power of two),
-//                     which O is expressed against.  From the first block on whose scale is 2^5 below that one, small weights
-//                     on large values may be what counts: P and V are bf16, 8 bits of any size (a block of zeros does not count).
+//                     which O is expressed against.  Once the scales of an item's blocks, in whatever order they come, are more than 2^5
+//                     apart (a block of zeros has the smallest one there is), small weights on large values may be what counts: from
+//                     that step on P and V are bf16, 8 bits of any size.
 // Bound: the two products are 2 x 128 x 64 x 128 multiply-adds a step, 512 cycles at the tensor cores' nominal rate, and the exponentials 512
 // of the special-function units.  The softmax of a step is a chain of some 2000 cycles, so two CTAs share an SM, and a CTA's scores of
 // the next step are computed under its softmax: tensor memory has two of S and one of O.  (128 keys per step with one S: 382 us
@@ -45,7 +46,7 @@ constexpr int REGS_SOFTMAX = 128, REGS_VALUES = 56, REGS_REST = 56;
 constexpr int GROUPS = KT / kKv8Group, GROUP_BYTES = kKv8Group * kKv8Dim;
 constexpr int TMEM_COLS = 256, COL_O = 128;
 constexpr float kLazy = 8.0f;                 // log2: the reference moves when a weight would be above 2^8
-constexpr float kF16Range = 1.0f / 32.0f;     // of V scales
+constexpr float kF16Range = 1.0f / 32.0f;     // smallest over largest V scale of an item's steps so far that f16 weights are taken for
 
 static_assert(GROUPS == 4, "a step's K scales are read as one float4");
 constexpr int STEPS = 4;                      // steps whose scales and lengths are kept
@@ -198,6 +199,7 @@ __global__ void __launch_bounds__(THREADS, 2) kv8_prefill_kernel(const __grid_co
                 int next_seq = -1, next_head = 0, next_len = 0, next_lo = 0, next_hi = 0;
                 Kv8Span next_span = {0, 0, 0};
                 float vref = 0.0f;
+                uint32_t vlow = 0x7F7FFFFFu;                      // the smallest V scale so far: bits of floats >= 0 are in their order
                 bool wide = false, looked = false;
                 int g = 0;
                 place_ahead = place_of(lane);
@@ -232,7 +234,8 @@ __global__ void __launch_bounds__(THREADS, 2) kv8_prefill_kernel(const __grid_co
                         const float vmul = number && most > 0.0f ? vs / most : 0.0f;
                         const bool plain_here = tokens == kKv8Group && key + kKv8Group - 1 <= pos_lo &&
                                                 (a.window == 0 || pos_hi - key < a.window || key + kKv8Group <= a.sinks);
-                        wide = __any_sync(0xFFFFFFFFu, mine && vs > 0x1p-126f && vmul < kF16Range && number) || wide;
+                        vlow = min(vlow, __reduce_min_sync(0xFFFFFFFFu, mine && tokens > 0 && number ? __float_as_uint(vs) : 0x7F7FFFFFu));
+                        wide = wide || __uint_as_float(vlow) < most * kF16Range;
                         const uint32_t poisoned = __ballot_sync(0xFFFFFFFFu, mine && !number) >> (g % 32);
                         const bool plain = !__any_sync(0xFFFFFFFFu, mine && !plain_here);
                         // the step whose place this is has been summed: softmax and V are done with it

@@ -1,0 +1,82 @@
+"""The 8-bit paged cache where its numbers, streams and forms of work reach their limits, against kv8_reference.py."""
+import numpy as np
+import pytest
+import torch
+
+import kv8_reference as ref
+from glm_asr_stack_b200 import ops
+from test_gpu_kv8 import Batch, dev
+
+pytestmark = pytest.mark.gpu
+
+LN2 = float(np.float32(np.log(2.0)))
+STRETCH = 1 + 2.0 ** -5
+
+
+def ladder(steps, tokens, new, seed=0):
+    """One sequence whose i-th run of 64 keys has the score STRETCH * steps[i][0] (log2, under the scale ln 2: no power of two, which
+    any format holds) and the V scale steps[i][1]; the score and scale of the last run last to the end."""
+    b = Batch([new], [tokens - new], 1, 4, 16, seed=seed)
+    k, v, ks, vs = b.codes[0], b.codes[1], b.scales[0], b.scales[1]
+    k[...], ks[...] = 0, 1.0
+    for g in range(-(-tokens // 16)):
+        score, scale = steps[min(g // 4, len(steps) - 1)]
+        blk = b.tables[0, g]
+        k[blk, 0, :, 0] = ref.e4m3(np.array([float(score)]))[0]
+        assert ref.VALUE[k[blk, 0, 0, 0]] == score
+        vs[blk] = scale
+        if scale in (0.0, 2.0 ** -126):
+            v[blk] = 0
+    q = np.zeros((new, b.heads, ref.DIM))
+    q[:, :, 0] = STRETCH
+    return b, q
+
+
+def bound(b, q, row):
+    """The result, and how far a kernel may be from it: weights off by 2^-8 of themselves (twice, above and below the line), scores
+    exact here but for 2^-20, the bf16 result by half a step.  Small weights may be off by 2^-20 of the largest PRODUCT of weight
+    and V scale, or by 2^-25 of the largest weight under the V scales within 2^5 of the smallest that a key here has: neither
+    lets a small weight on a large value go."""
+    want, _ = ref.attend(q[row:row + 1], b.codes[0], b.scales[0], b.codes[1], b.scales[1], b.tables[0], b.lens[0] - b.new[0] + row + 1, scale=LN2)
+    length = b.lens[0] - b.new[0] + row + 1
+    at = np.arange(length)
+    blk = b.tables[0, at // 16]
+    x = STRETCH * ref.VALUE[b.codes[0][blk, 0, at % 16, 0]]
+    w = np.exp((x - x.max()) * LN2)
+    w /= w.sum()
+    vs = b.scales[1][blk, 0, 0].astype(np.float64)
+    codes = np.abs(ref.VALUE[b.codes[1][blk, 0, at % 16]])
+    small = 2.0 ** -20 * (w * vs).max() + 2.0 ** -25 * w.max() * min(vs.max(), vs.min() * 2.0 ** 5)
+    return want, 2.0 ** -8 * np.abs(want) + (2.0 ** -8 + 2.0 ** -19) * 2 * ((w * vs) @ codes)[None, None] + small * codes.sum(0)[None, None] + 1e-37
+
+
+LADDERS = {
+    "up 2^16": [(16, 1.0), (0, 2.0 ** 16)],
+    "up 2^20": [(20, 1.0), (0, 2.0 ** 20)],
+    "up 2^24": [(24, 1.0), (0, 2.0 ** 24)],
+    "up 2^30": [(30, 1.0), (0, 2.0 ** 30)],
+    "down 2^24": [(0, 2.0 ** 24), (24, 1.0)],
+    "up 2^4 eleven times": [(4 * (11 - i), 2.0 ** (4 * i)) for i in range(12)],
+    "up 2^2 fourteen times": [(2 * (14 - i), 2.0 ** (2 * i)) for i in range(15)],
+    "up, down and up": [(24, 1.0), (0, 2.0 ** 24), (24, 1.0), (0, 2.0 ** 24)],
+    "zeros first": [(26, 2.0 ** -126), (0, 1.0)],
+    "never written first": [(26, 0.0), (0, 1.0)],
+    "zeros last": [(0, 1.0), (26, 2.0 ** -126)],
+    "far out": [(30, 2.0 ** -60), (0, 2.0 ** -30), (-30, 1.0)],
+}
+
+
+@pytest.mark.parametrize("name", LADDERS)
+@pytest.mark.parametrize("new", [1, 40])
+def test_v_scales_that_change_along_the_context(name, new):
+    """Small weights on large values, in every order, by both kernels: the hint chooses between them and not the result."""
+    steps = LADDERS[name]
+    tokens = 64 * len(steps) + 70 + new
+    b, q = ladder(steps, tokens, new)
+    pool, tables, lens, cu = b.device()
+    for max_new in (1, 100_000):
+        out = ops.kv8_attention(dev(q), *pool, tables, lens, cu, max_new=max_new, scale=LN2).float().cpu().numpy()
+        for row in {0, new // 2, new - 1}:
+            want, tol = bound(b, q, row)
+            assert np.all(np.abs(out[row:row + 1] - want) <= tol), (max_new, row, (np.abs(out[row:row + 1] - want) / tol).max())
+    assert ops.status() == 0
