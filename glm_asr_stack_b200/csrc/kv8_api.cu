@@ -43,6 +43,19 @@ bool rows_ok(const void *p, long long ld, int heads, int rows) {
     return p != nullptr && aligned16(p) && ld % 8 == 0 && (rows <= 1 || ld >= (long long)heads * kKv8Dim);
 }
 
+// Whether two sets of `rows` rows (of heads_a and heads_b heads) have an element in common.  At one pitch, rows i of the one and j of the other are
+// (b - a) + (j - i) * pitch apart, of which only the two next to zero matter; rows of different pitches count as one piece each.
+bool rows_overlap(const void *a, long long lda, int heads_a, const void *b, long long ldb, int heads_b, int rows) {
+    const long long wa = (long long)heads_a * kKv8Dim, wb = (long long)heads_b * kKv8Dim;
+    const long long apart = ((long long)(uintptr_t)b - (long long)(uintptr_t)a) / 2;          // elements; both are 16-byte aligned
+    if (rows <= 1) lda = ldb = 0;
+    if (apart >= (rows - 1) * lda + wa || -apart >= (rows - 1) * ldb + wb) return false;
+    if (lda != ldb || rows <= 1) return true;
+    long long j = -apart / lda;                               // apart + j * lda is the first that is not below zero
+    if (apart + j * lda < 0) ++j;
+    return (j < rows && -j < rows && apart + j * lda < wa) || (j - 1 < rows && 1 - j < rows && -(apart + (j - 1) * lda) < wb);
+}
+
 }  // namespace
 
 extern "C" int glmasr_kv8_append(const glmasr_kv8_cache *cache, const uint16_t *key, long long ldk, const uint16_t *value, long long ldv,
@@ -54,7 +67,12 @@ extern "C" int glmasr_kv8_append(const glmasr_kv8_cache *cache, const uint16_t *
     if (!isfinite(theta) || theta < 0.0 || (query != nullptr && q_heads <= 0) || (query == nullptr) != (query_out == nullptr)) return -1;
     if (num_seqs == 0 || total_new == 0) return 0;
     if (!rows_ok(key, ldk, b.kv_heads, total_new) || !rows_ok(value, ldv, b.kv_heads, total_new)) return -1;
-    if (query != nullptr && (!rows_ok(query, ldq, q_heads, total_new) || !rows_ok(query_out, ldqo, q_heads, total_new))) return -1;
+    if (query != nullptr) {
+        if (!rows_ok(query, ldq, q_heads, total_new) || !rows_ok(query_out, ldqo, q_heads, total_new)) return -1;
+        const bool in_place = query_out == query && (ldqo == ldq || total_new == 1);
+        if (!in_place && rows_overlap(query_out, ldqo, q_heads, query, ldq, q_heads, total_new)) return -1;
+        if (rows_overlap(query_out, ldqo, q_heads, key, ldk, b.kv_heads, total_new) || rows_overlap(query_out, ldqo, q_heads, value, ldv, b.kv_heads, total_new)) return -1;
+    }
     if (!kv8_append_launch(cache->k, cache->v, cache->k_scale, cache->v_scale, (const __nv_bfloat16 *)key, ldk, (const __nv_bfloat16 *)value, ldv,
                            (const __nv_bfloat16 *)query, ldq, (__nv_bfloat16 *)query_out, ldqo, b, theta, current_stream())) {
         (void)cudaGetLastError();
@@ -75,6 +93,7 @@ extern "C" int glmasr_kv8_attention(uint16_t *out, long long ldo, const uint16_t
     if (q_heads <= 0 || q_heads % a.b.kv_heads != 0 || window < 0 || sinks < 0 || max_new < 0 || max_len < 0 || !(scale >= 0.0f) || !isfinite(scale)) return -1;
     if (num_seqs == 0 || total_new == 0) return 0;
     if (!rows_ok(query, ldq, q_heads, total_new) || !rows_ok(out, ldo, q_heads, total_new)) return -1;
+    if (rows_overlap(out, ldo, q_heads, query, ldq, q_heads, total_new)) return -1;
     if (workspace == nullptr || !aligned16(workspace) || workspace_bytes < glmasr_kv8_attention_workspace()) return -1;
     a.k_cache = cache->k, a.v_cache = cache->v;
     a.k_scale = cache->k_scale, a.v_scale = cache->v_scale;

@@ -335,7 +335,8 @@ def kv8_append(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tens
     k_cache, v_cache [num_blocks, kv_heads, block_size, 128] (float8_e4m3fn or uint8), k_scale, v_scale float32
     [num_blocks, kv_heads, block_size / 16]; key, value [tokens, kv_heads, 128], query [tokens, q_heads, 128] bf16, row slices
     of a fused projection included.  Sequence s owns the rows cu_new[s] .. cu_new[s + 1] and has seq_lens[s] tokens WITH them
-    (device int32).  theta = 0: no rotation.  Returns the rotated queries (query_out, which may be query itself), or None."""
+    (device int32).  theta = 0: no rotation.  Returns the rotated queries (query_out, which may be query itself and must not overlap the
+    inputs otherwise), or None."""
     cache, device, kv_heads, _ = _kv8_cache(k_cache, v_cache, k_scale, v_scale)
     n, max_blocks = _kv8_batch(block_tables, seq_lens, cu_new, device)
     k, ldk, tokens = _kv8_rows(key, "key", device, kv_heads)

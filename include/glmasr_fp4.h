@@ -419,7 +419,8 @@ typedef struct {
  * no rotation) and write keys and values to the cache: per block of 16 positions the scale is that of its new tokens, or the
  * one it had where that is larger and the block holds earlier tokens; their codes are rescaled when it grows.  Two sequences
  * must not append to the same block in one call.  key, value, query, query_out: bf16 rows of kv_heads (q_heads) * 128 elements, row
- * pitches in elements, multiples of 8, 16-byte aligned.  query and query_out may both be NULL, and may be the same rows.
+ * pitches in elements, multiples of 8, 16-byte aligned.  query and query_out may both be NULL, and may be the same rows; else query_out
+ * must not overlap query, key or value (columns of one array at one pitch may lie side by side).
  * Returns 0, or -1 on bad arguments or a launch failure. */
 int glmasr_kv8_append(const glmasr_kv8_cache *cache, const uint16_t *key, long long ldk, const uint16_t *value, long long ldv,
                       const uint16_t *query, long long ldq, uint16_t *query_out, long long ldqo, int q_heads,
@@ -432,8 +433,8 @@ int glmasr_kv8_append(const glmasr_kv8_cache *cache, const uint16_t *key, long l
  * kv_heads.  scale: of the scores, before the softmax.  max_new (new tokens of a sequence) and max_len (tokens of a sequence)
  * say what to expect: they choose kernels (which differ in the order of sums and in rounding), never what is seen or computed.
  * workspace: glmasr_kv8_attention_workspace() bytes (for the current device) of device memory, 16-byte aligned, contents irrelevant,
- * not shared with a call that may run at the same time.  out must not overlap query.  Returns 0, or -1 on bad arguments or a
- * launch failure. */
+ * not shared with a call that may run at the same time.  out must not overlap query (columns of one array at one pitch may lie side by
+ * side).  Returns 0, or -1 on bad arguments or a launch failure. */
 long long glmasr_kv8_attention_workspace(void);
 int glmasr_kv8_attention(uint16_t *out, long long ldo, const uint16_t *query, long long ldq, const glmasr_kv8_cache *cache,
                          const int *block_tables, int max_blocks, const int *seq_lens, const int *cu_new, int num_seqs,

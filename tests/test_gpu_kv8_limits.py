@@ -80,3 +80,24 @@ def test_v_scales_that_change_along_the_context(name, new):
             want, tol = bound(b, q, row)
             assert np.all(np.abs(out[row:row + 1] - want) <= tol), (max_new, row, (np.abs(out[row:row + 1] - want) / tol).max())
     assert ops.status() == 0
+
+
+def test_slices_that_overlap_are_refused():
+    b = Batch([3, 2], [20, 4], 2, 4, 16)
+    pool, tables, lens, cu = b.device()
+    buf = dev(b.rows(3 * b.heads, extra=1))
+    h, n = b.heads, b.total
+    before = [buf.clone()] + [t.clone() for t in pool]
+    for out in (buf[:n, 1:1 + h], buf[1:, :h], buf[1:, h - 1:2 * h - 1], buf[:n, :h]):
+        with pytest.raises(ValueError):
+            ops.kv8_attention(buf[:n, :h], *pool, tables, lens, cu, out=out)
+    kv = buf[:n, 2 * h:2 * h + 2]
+    for query, out, key, value in ((0, 1, kv, kv), (0, h, buf[:n, h:h + 2], kv), (0, h, kv, buf[:n, 2 * h - 2:2 * h]), (0, h, kv, buf[1:, h + 1:h + 3])):
+        with pytest.raises(ValueError):
+            ops.kv8_append(*pool, key, value, tables, lens, cu, query=buf[:n, query:query + h], query_out=buf[:n, out:out + h])
+    torch.cuda.synchronize()
+    assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(before, [buf, *pool]))
+    # side by side in one array
+    apart = ops.kv8_attention(buf[:n, :h].clone(), *pool, tables, lens, cu)
+    assert torch.equal(ops.kv8_attention(buf[:n, :h], *pool, tables, lens, cu, out=buf[:n, h:2 * h]), apart)
+    assert torch.equal(buf[:, :h], before[0][:, :h]) and torch.equal(buf[:, 2 * h:], before[0][:, 2 * h:])

@@ -1,0 +1,102 @@
+"""The C entry points of the 8-bit paged cache without a GPU: kv8_api.cu is host code, compiled here against launches that only
+count, so that a call with good arguments returns 0 and every refusal shows the check it is for."""
+import ctypes
+import os
+import random
+import subprocess
+
+import pytest
+
+from conftest import ROOT
+from glm_asr_stack_b200 import _lib
+
+CSRC = os.path.join(ROOT, "glm_asr_stack_b200", "csrc")
+FAKES = r"""
+#include "kv8_attention.cuh"
+#include "runtime.cuh"
+namespace glmasr {
+static int launched = 0;
+static Kv8Attend last;
+cudaStream_t current_stream() { return nullptr; }
+void note_launches(int) {}
+size_t kv8_attention_workspace_bytes() { return 4096; }
+bool kv8_append_launch(uint8_t *, uint8_t *, float *, float *, const __nv_bfloat16 *, long long, const __nv_bfloat16 *, long long, const __nv_bfloat16 *,
+                       long long, __nv_bfloat16 *, long long, const Kv8Batch &, double, cudaStream_t) { ++launched; return true; }
+bool kv8_attention_launch(const Kv8Attend &a, int, int, void *, cudaStream_t, int &n) { ++launched; last = a; n = 1; return true; }
+}
+extern "C" cudaError_t cudaGetLastError() { return cudaSuccess; }
+extern "C" int launches() { return glmasr::launched; }
+"""
+A = 1 << 20            # addresses that nothing follows
+
+
+@pytest.fixture(scope="module")
+def lib(tmp_path_factory):
+    tmp = tmp_path_factory.mktemp("kv8_entry")
+    (tmp / "fakes.cpp").write_text(FAKES)
+    cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
+    subprocess.run(["g++", "-std=c++17", "-shared", "-fPIC", "-Wl,-Bsymbolic", "-I", CSRC, "-I", os.path.join(cuda, "include"), "-o", str(tmp / "e.so"),
+                    str(tmp / "fakes.cpp"), "-x", "c++", os.path.join(CSRC, "kv8_api.cu")], check=True, capture_output=True)
+    dll = ctypes.CDLL(str(tmp / "e.so"))
+    for name in ("glmasr_kv8_append", "glmasr_kv8_attention"):
+        getattr(dll, name).restype, getattr(dll, name).argtypes = _lib.SIGNATURES[name]
+    return dll
+
+
+CACHE = {"k": A, "v": A, "k_scale": A, "v_scale": A, "num_blocks": 4, "block_size": 16, "kv_heads": 2, "head_dim": 128}
+APPEND = dict(key=A, ldk=256, value=A, ldv=256, query=2 * A, ldq=1024, out=3 * A, ldo=1024, heads=8, tables=A, max_blocks=4, lens=A, cu=A, seqs=1,
+              rows=2, theta=1e4)
+ATTEND = dict(out=A, ldo=1024, query=2 * A, ldq=1024, tables=A, max_blocks=4, lens=A, cu=A, seqs=1, rows=2, heads=8, max_new=2, max_len=9, window=0,
+              sinks=0, scale=0.1, ws=A, ws_bytes=4096)
+
+
+def append(lib, cache=CACHE, **change):
+    f = {**APPEND, **change}
+    c = ctypes.byref(_lib.Kv8Cache(*[cache[n] for n, _ in _lib.Kv8Cache._fields_])) if cache is not None else None
+    before = lib.launches()
+    code = lib.glmasr_kv8_append(c, *f.values())
+    assert (code == 0 and lib.launches() == before + 1) or lib.launches() == before
+    return code
+
+
+def attend(lib, cache=CACHE, **change):
+    f = {**ATTEND, **change}
+    c = ctypes.byref(_lib.Kv8Cache(*[cache[n] for n, _ in _lib.Kv8Cache._fields_])) if cache is not None else None
+    before = lib.launches()
+    code = lib.glmasr_kv8_attention(f["out"], f["ldo"], f["query"], f["ldq"], c, *list(f.values())[4:])
+    assert (code == 0 and lib.launches() == before + 1) or lib.launches() == before
+    return code
+
+
+def elements(address, ld, heads, rows):
+    return {address // 2 + r * ld + i for r in range(rows) for i in range(0, heads * 128, 8)}
+
+
+def test_outputs_that_overlap_inputs_are_refused(lib):
+    """Against the sets of elements, for rows at one pitch; shifted by rows, by heads and by 16 bytes."""
+    rng = random.Random(0)
+    refused = 0
+    for _ in range(4000):
+        heads, rows, ld = 8, rng.randint(1, 5), rng.choice([1024, 1032, 1536, 2048, 4096])
+        shift = 2 * rng.choice([rng.randint(-6, 6) * ld, rng.randint(-6, 6) * ld + rng.choice([-1, 1]) * rng.choice([8, 128, 512, 1016, 1024, ld - 1024]),
+                                8 * rng.randint(-4000, 4000)])
+        want = bool(elements(A, ld, heads, rows) & elements(A + shift, ld, heads, rows))
+        assert attend(lib, out=A, ldo=ld, query=A + shift, ldq=ld, rows=rows) == (-1 if want else 0), (rows, ld, shift)
+        far = {"key": 64 * A, "value": 64 * A}
+        assert append(lib, query=A + shift, ldq=ld, out=A, ldo=ld, rows=rows, **far) == (-1 if want and shift != 0 else 0), (rows, ld, shift)
+        for which, pitch in (("key", "ldk"), ("value", "ldv")):
+            hit = bool(elements(A, ld, heads, rows) & elements(A + shift, ld, 2, rows))
+            assert append(lib, **{**far, "query": 32 * A, "ldq": ld, "out": A, "ldo": ld, "rows": rows, which: A + shift, pitch: ld}) == (-1 if hit else 0)
+        refused += want
+    assert 500 < refused < 3500
+
+
+def test_outputs_at_another_pitch_have_to_lie_apart(lib):
+    assert attend(lib, out=A, ldo=1024, query=A, ldq=2048) == -1
+    assert attend(lib, out=A, ldo=2048, query=A + 2048, ldq=1024) == -1         # between the rows, but for one array's sake
+    assert attend(lib, out=A, ldo=1024, query=A + 4 * 1024, ldq=2048) == 0
+    assert attend(lib, out=A + 2 * (2048 + 1024), ldo=1024, query=A, ldq=2048) == 0
+    assert attend(lib, out=A, ldo=8, query=A + 2048, ldq=16, rows=1) == 0       # one row has no pitch
+    assert append(lib, query=A, ldq=1024, out=A, ldo=2048) == -1
+    assert append(lib, query=A, ldq=1024, out=A, ldo=2048, rows=1, key=64 * A, value=64 * A) == 0
+    assert append(lib, query=A, ldq=1536, out=A, ldo=1536, key=A + 2048, ldk=1536, value=A + 2560, ldv=1536) == 0       # one fused projection
