@@ -325,6 +325,25 @@ def _kv8_batch(block_tables, seq_lens, cu_new, device: int):
     raise ValueError("expected block_tables [num_seqs, max_blocks], seq_lens [num_seqs], cu_new [num_seqs + 1] on the cache's device")
 
 
+def _kv8_launch_stream(device: int):
+    """The stream of set_stream(), or None where it is torch's current one."""
+    if (0 if _stream is None else _stream.cuda_stream) == torch._C._cuda_getCurrentRawStream(device):
+        return None
+    return torch.cuda.default_stream(device) if _stream is None else _stream
+
+
+def _kv8_rows_like(query: torch.Tensor, device: int) -> torch.Tensor:
+    """An array for a call's result.  Where launches go to another stream than torch's current one it is made on that one: a block of the
+    current stream's pool may still be in use there, and one that is given back goes to whoever asks next."""
+    stream = _kv8_launch_stream(device)
+    if stream is None:
+        return torch.empty(query.shape, dtype=torch.bfloat16, device=query.device)
+    with torch.cuda.stream(stream):
+        out = torch.empty(query.shape, dtype=torch.bfloat16, device=query.device)
+    out.record_stream(torch.cuda.current_stream(device))       # where the caller reads it
+    return out
+
+
 def kv8_append(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, key: torch.Tensor,
                value: torch.Tensor, block_tables: torch.Tensor, seq_lens: torch.Tensor, cu_new: torch.Tensor,
                query: Optional[torch.Tensor] = None, query_out: Optional[torch.Tensor] = None,
@@ -349,7 +368,7 @@ def kv8_append(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tens
         q, ldq, q_tokens = _kv8_rows(query, "query", device)
         q_heads = query.shape[1]
         if query_out is None:
-            query_out = torch.empty(query.shape, dtype=torch.bfloat16, device=query.device)
+            query_out = _kv8_rows_like(query, device)
         qo, ldqo, o_tokens = _kv8_rows(query_out, "query_out", device, q_heads)
         if q_tokens != tokens or o_tokens != tokens:
             raise ValueError("query, query_out: not as many rows as key")
@@ -381,7 +400,7 @@ def kv8_attention(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
     if q_heads == 0 or q_heads % kv_heads != 0:
         raise ValueError("query: the head count must be a multiple of the cache's")
     if out is None:
-        out = torch.empty((tokens, q_heads, 128), dtype=torch.bfloat16, device=query.device)
+        out = _kv8_rows_like(query, device)
     o, ldo, o_tokens = _kv8_rows(out, "out", device, q_heads)
     if o_tokens != tokens:
         raise ValueError("out: not as many rows as query")
@@ -393,15 +412,16 @@ def kv8_attention(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
     size = _kv8_workspace_bytes.get(device)
     if size is None:
         size = _kv8_workspace_bytes[device] = lib.glmasr_kv8_attention_workspace()
-    workspace = seq_lens.new_empty(size // 4)       # a multiple of 256 bytes; cheaper than torch.empty
+    stream = _kv8_launch_stream(device)
+    if stream is None:
+        workspace = seq_lens.new_empty(size // 4)   # a multiple of 256 bytes; cheaper than torch.empty
+    else:
+        with torch.cuda.stream(stream):             # of the pool of the stream that works on it
+            workspace = seq_lens.new_empty(size // 4)
     if lib.glmasr_kv8_attention(o, ldo, q, ldq, cache, block_tables.data_ptr(), max_blocks, seq_lens.data_ptr(), cu_new.data_ptr(), n, tokens, q_heads,
                                 (tokens + n - 1) // n if max_new is None else max_new, max_blocks * block_size if max_len is None else max_len, window, sinks,
                                 _KV8_SCALE if scale is None else scale, workspace.data_ptr(), size) != 0:
         raise ValueError("glmasr_kv8_attention rejected the arguments")
-    used = 0 if _stream is None else _stream.cuda_stream
-    if used != torch._C._cuda_getCurrentRawStream(device):
-        # the workspace came from another stream than the one that works on it
-        workspace.record_stream(torch.cuda.default_stream(device) if _stream is None else _stream)
     return out
 
 

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import kv8_reference as ref
-from glm_asr_stack_b200 import ops
+from glm_asr_stack_b200 import _lib, ops
 from test_gpu_kv8 import Batch, dev
 
 pytestmark = pytest.mark.gpu
@@ -101,3 +101,45 @@ def test_slices_that_overlap_are_refused():
     apart = ops.kv8_attention(buf[:n, :h].clone(), *pool, tables, lens, cu)
     assert torch.equal(ops.kv8_attention(buf[:n, :h], *pool, tables, lens, cu, out=buf[:n, h:2 * h]), apart)
     assert torch.equal(buf[:, :h], before[0][:, :h]) and torch.equal(buf[:, 2 * h:], before[0][:, 2 * h:])
+
+
+@pytest.mark.parametrize("own_stream", [False, True])
+def test_what_a_call_allocates_belongs_to_the_stream_that_works_on_it(own_stream):
+    """torch's current stream is another one than the launches'.  Blocks that the current stream's pool has back are still in use on it,
+    and a result that is dropped at once is still being written: no call may touch the one or give the other away."""
+    b = Batch([1] * 3, [5000, 17, 90], 2, 4, 16)
+    pool, tables, lens, cu = b.device()
+    q, k = dev(b.rows(b.heads)), dev(b.rows(2))
+    want_q = ops.kv8_append(*pool, k, k, tables, lens, cu, query=q)
+    want = ops.kv8_attention(want_q, *pool, tables, lens, cu, max_new=1)
+    size = _lib.load().glmasr_kv8_attention_workspace()
+    other = torch.cuda.Stream()
+    current, launch = (torch.cuda.default_stream(), other) if own_stream else (other, torch.cuda.default_stream())
+    rest = lambda s: s.synchronize() or torch.cuda._sleep(40_000_000)  # noqa: E731  about 20 ms
+    torch.cuda.synchronize()
+    if own_stream:
+        ops.set_stream(other)
+    try:
+        with torch.cuda.stream(current):
+            for nbytes in (size, q.numel() * 2):
+                used = torch.full((nbytes,), 7, dtype=torch.uint8, device="cuda")
+                rest(current)
+                copy = used.clone()                           # when the current stream gets to it
+                del used
+                q2 = ops.kv8_append(*pool, k, k, tables, lens, cu, query=q)
+                got = ops.kv8_attention(want_q, *pool, tables, lens, cu, max_new=1)
+                torch.cuda.synchronize()
+                assert torch.all(copy == 7)
+                assert torch.equal(got, want) and torch.equal(q2, want_q)
+                del copy, q2, got
+            for call in (lambda: ops.kv8_append(*pool, k, k, tables, lens, cu, query=q), lambda: ops.kv8_attention(want_q, *pool, tables, lens, cu, max_new=1)):
+                with torch.cuda.stream(launch):
+                    rest(launch)
+                call()                                        # its result is dropped while the launch stream is still asleep
+                after = torch.full_like(q, 5.0)
+                torch.cuda.synchronize()
+                assert torch.all(after == 5)
+                del after
+    finally:
+        ops.set_stream(None)
+    assert ops.status() == 0
