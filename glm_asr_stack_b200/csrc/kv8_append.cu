@@ -41,7 +41,7 @@ struct AppendParams {
     __nv_bfloat16 *query_out;
     long long ldq, ldqo;
     Kv8Batch b;
-    double turns[HALF];           // theta^(-d / 64) / (2 pi)
+    double turns[HALF];           // theta^(-d / 64) / (2 pi); zeros: no rotation
 };
 
 // 64 bits -> 32 bits, cut towards zero, the last bit set if anything was cut ("round to odd").
@@ -248,6 +248,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) kv8_append_kernel(const __grid_
     };
     load_heads(head);
     find_angles();
+    const bool rotated = p.turns[0] != 0.0;                      // else as they are: 0 * inf is not 0, and -0 + 0 not -0
     float2 cs[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -259,13 +260,15 @@ __global__ void __launch_bounds__(THREADS, CTAS) kv8_append_kernel(const __grid_
 #pragma unroll
         for (int u = 0; u < STEPS; ++u) {
             uint32_t own[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
+            if (rotated) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint32_t other = __shfl_xor_sync(0xFFFFFFFFu, own[j], 8);
-                const float y0 = fmaf(bf16_lo(own[j]), cs[2 * j].x, cs[2 * j].y * bf16_lo(other));
-                const float y1 = fmaf(bf16_hi(own[j]), cs[2 * j + 1].x, cs[2 * j + 1].y * bf16_hi(other));
-                const __nv_bfloat162 b = __floats2bfloat162_rn(y0, y1);
-                own[j] = *reinterpret_cast<const uint32_t *>(&b);
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t other = __shfl_xor_sync(0xFFFFFFFFu, own[j], 8);
+                    const float y0 = fmaf(bf16_lo(own[j]), cs[2 * j].x, cs[2 * j].y * bf16_lo(other));
+                    const float y1 = fmaf(bf16_hi(own[j]), cs[2 * j + 1].x, cs[2 * j + 1].y * bf16_hi(other));
+                    const __nv_bfloat162 b = __floats2bfloat162_rn(y0, y1);
+                    own[j] = *reinterpret_cast<const uint32_t *>(&b);
+                }
             }
             y[u] = make_uint4(own[0], own[1], own[2], own[3]);
         }

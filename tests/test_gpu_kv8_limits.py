@@ -143,3 +143,21 @@ def test_what_a_call_allocates_belongs_to_the_stream_that_works_on_it(own_stream
     finally:
         ops.set_stream(None)
     assert ops.status() == 0
+
+
+@pytest.mark.parametrize("new,ctx", [([1], [0]), ([1, 5], [7, 300]), ([40, 2], [3, 15])])
+def test_no_rotation_leaves_every_bit_of_the_queries(new, ctx):
+    """theta = 0: a dim has nothing from its partner, be that infinite or no number, and a zero keeps its sign."""
+    b = Batch(new, ctx, 2, 4, 16)
+    q, k = dev(b.rows(b.heads)), dev(b.rows(2))
+    flat = q.view(b.total, -1)
+    for i, x in enumerate((np.inf, -np.inf, np.nan, -0.0, 3e38)):
+        flat[:, 7 + 65 * i] = x
+    q = flat.view(q.shape)
+    pool, tables, lens, cu = b.device()
+    want = q.clone()
+    got = ops.kv8_append(*pool, k, k, tables, lens, cu, query=q, theta=0.0)
+    assert torch.equal(got.view(torch.int16), want.view(torch.int16))
+    wide = torch.cat([q, q], dim=1)                           # in place, into rows of a wider pitch
+    ops.kv8_append(*pool, k, k, tables, lens, cu, query=wide[:, :b.heads], query_out=wide[:, :b.heads], theta=0.0)
+    assert torch.equal(wide.view(torch.int16), torch.cat([want, want], dim=1).view(torch.int16))
