@@ -31,6 +31,10 @@ constexpr int THREADS = 256, CTAS = 3;     // per SM
 constexpr int QUERY_HEADS = 16;            // of a CTA that has queries
 constexpr size_t SPREAD = 64 * 1024;       // of shared memory: with it two CTAs fit an SM, not three
 constexpr int HALF = kKv8Dim / 2;
+// Keys are computed times 2^40, which their angles bring along: numbers below 2^-126, where 32 bits have fewer digits, are then below
+// 2^-166, and the smallest one with a code other than 0 is 2^-136.  At the other end 448 * 2^60 still has 2^19 above it.
+constexpr int KEY_EXP = 40;
+constexpr double KEY_UNIT = (double)(1ull << KEY_EXP);
 
 struct AppendParams {
     uint8_t *cache[2];            // K, V
@@ -48,7 +52,7 @@ struct AppendParams {
 __device__ __forceinline__ float cut_odd(double x) {
     const uint32_t hi = (uint32_t)__double2hiint(x), lo = (uint32_t)__double2loint(x);
     const uint32_t mag = hi & 0x7FFFFFFFu;
-    if (mag < 0x38100000u || mag >= 0x47F00000u) return (float)x;        // below 2^-126 (nothing there is near a border), or not finite
+    if (mag < 0x38100000u || mag >= 0x47F00000u) return (float)x;        // below 2^-126 (there is no border there: see KEY_UNIT), or not finite
     const uint32_t r = __funnelshift_l(lo, hi, 3) - (384u << 23);        // nine exponent bits and 23 of the mantissa, exponent re-biased
     return __uint_as_float((hi & 0x80000000u) | (r & 0x7FFFFFFFu) | ((lo & 0x1FFFFFFFu) != 0u ? 1u : 0u));
 }
@@ -66,9 +70,10 @@ __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
 // an e4m3 code's value times 2^-120: its bits are those of a bf16 number with another exponent bias
 __device__ __forceinline__ float e4m3_value(uint32_t c) { return __uint_as_float(((c & 0x7Fu) << 20) | ((c & 0x80u) << 24)) * 0x1p120f; }
 
-// Exponent of the scale for a block whose largest absolute value has the given bits (finite, at most 448 * 2^60): 448 = 1.75 * 2^8.
-__device__ __forceinline__ int scale_exponent(uint32_t amax) {
-    const int e = (int)(amax >> 23) - 127 - 8 + ((amax & 0x7FFFFFu) > 0x600000u ? 1 : 0);
+// Exponent of the scale for a block whose largest absolute value, times 2^unit, has the given bits (finite, at most 448 * 2^60 without the
+// unit): 448 = 1.75 * 2^8.
+__device__ __forceinline__ int scale_exponent(uint32_t amax, int unit) {
+    const int e = (int)(amax >> 23) - 127 - 8 - unit + ((amax & 0x7FFFFFu) > 0x600000u ? 1 : 0);
     return max(e, -126);
 }
 __device__ __forceinline__ float pow2f(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }     // e in [-126, 127]
@@ -103,6 +108,7 @@ __device__ __forceinline__ void meet(int pair) { asm volatile("barrier.cta.sync 
 template <bool KEY>
 __device__ __forceinline__ void quantise_head(const AppendParams &p, const Part &b, long long row, const uint4 (&w)[STEPS], const double2 *angles, volatile uint32_t *shared_max) {
     constexpr int which = KEY ? 0 : 1;
+    constexpr float unit = KEY ? (float)KEY_UNIT : 1.0f;         // that x is taken times
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = lane & 15, sub = lane >> 4;
     float *scale = p.scale[which] + row / kKv8Group;
     const float old = b.first > 0 && row >= 0 ? *scale : 0.0f;
@@ -142,13 +148,14 @@ __device__ __forceinline__ void quantise_head(const AppendParams &p, const Part 
     // every lane has the old scale
     if (row < 0) return;                                         // no page: nowhere to write
     uint8_t *dst = p.cache[which] + row * kKv8Dim;
-    const bool poisoned = amax > __float_as_uint(448.0f * 0x1p60f) || (b.first > 0 && !(old >= 0.0f && old <= pow2f(kKv8MaxExp)));
+    const bool poisoned = amax > __float_as_uint(448.0f * 0x1p60f * unit) || (b.first > 0 && !(old >= 0.0f && old <= pow2f(kKv8MaxExp)));
     float now = 0.0f, inv = 0.0f;
     if (!poisoned) {
-        now = pow2f(scale_exponent(amax));
+        now = pow2f(scale_exponent(amax, KEY ? KEY_EXP : 0));
         if (old > now) now = old;
         inv = 1.0f / now;                                        // exact: a power of two, at most 2^126
     }
+    const float quantum = inv / unit;
     if (b.from == 0) {
         if (lane == 0) *scale = poisoned ? __uint_as_float(0x7FFFFFFFu) : now;
         if (b.first > 0 && (poisoned || now != old)) {           // the earlier tokens of the block, under the new scale
@@ -173,8 +180,8 @@ __device__ __forceinline__ void quantise_head(const AppendParams &p, const Part 
         if (t >= b.n || r < 0 || r >= p.b.total_new) continue;
         uint2 codes = make_uint2(0u, 0u);
         if (!poisoned)
-            codes = make_uint2(e4m3x4(x[i][0] * inv, x[i][1] * inv, x[i][2] * inv, x[i][3] * inv),
-                               e4m3x4(x[i][4] * inv, x[i][5] * inv, x[i][6] * inv, x[i][7] * inv));
+            codes = make_uint2(e4m3x4(x[i][0] * quantum, x[i][1] * quantum, x[i][2] * quantum, x[i][3] * quantum),
+                               e4m3x4(x[i][4] * quantum, x[i][5] * quantum, x[i][6] * quantum, x[i][7] * quantum));
         *reinterpret_cast<uint2 *>(dst + (b.first + t) * kKv8Dim + c * 8) = codes;
     }
 }
@@ -200,13 +207,13 @@ __global__ void __launch_bounds__(THREADS, CTAS) kv8_append_kernel(const __grid_
     // tokens that were in the block before: with a start inside the block they are the places below `first`
     Part part = {row0 + (pos - start), n, pos & (kKv8Group - 1), 0};
 
-    auto find_angles = [&]() {
+    auto find_angles = [&](double unit) {
 #pragma unroll 1                     // two at once take registers from the rest: 28.4 us instead of 27.9
         for (int i = threadIdx.x; i < n * HALF; i += THREADS) {
             const double turn = (double)(pos + i / HALF) * p.turns[i % HALF];
             double s, c;
             sincospi(2.0 * (turn - rint(turn)), &s, &c);
-            angles[angle_at(i / HALF, i % HALF)] = make_double2(c, s);
+            angles[angle_at(i / HALF, i % HALF)] = make_double2(c * unit, s * unit);
         }
         __syncthreads();
     };
@@ -219,7 +226,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) kv8_append_kernel(const __grid_
         if (shared) part.from = (warp & 1) * 2 * STEPS;
         auto is_value = [&](int i) { return (i ^ (i / units)) & 1; };
         if (task < 2 * heads) load_rows(p, part, is_value(task), task >> 1, w);  // on their way under the angles
-        find_angles();
+        find_angles(KEY_UNIT);
         for (int round = 0; task < 2 * heads; task += units, ++round) {
             const long long row = kv8_group_row(p.b, seq, task >> 1, group);
             volatile uint32_t *max_here = shared ? shared_max[round & 1] : nullptr;
@@ -247,7 +254,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) kv8_append_kernel(const __grid_
         }
     };
     load_heads(head);
-    find_angles();
+    find_angles(1.0);
     const bool rotated = p.turns[0] != 0.0;                      // else as they are: 0 * inf is not 0, and -0 + 0 not -0
     float2 cs[8];
 #pragma unroll

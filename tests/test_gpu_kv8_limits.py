@@ -5,7 +5,7 @@ import torch
 
 import kv8_reference as ref
 from glm_asr_stack_b200 import _lib, ops
-from test_gpu_kv8 import Batch, dev
+from test_gpu_kv8 import Batch, check_append, dev
 
 pytestmark = pytest.mark.gpu
 
@@ -161,3 +161,23 @@ def test_no_rotation_leaves_every_bit_of_the_queries(new, ctx):
     wide = torch.cat([q, q], dim=1)                           # in place, into rows of a wider pitch
     ops.kv8_append(*pool, k, k, tables, lens, cu, query=wide[:, :b.heads], query_out=wide[:, :b.heads], theta=0.0)
     assert torch.equal(wide.view(torch.int16), torch.cat([want, want], dim=1).view(torch.int16))
+
+
+# Keys below 2^-126 whose rotation lies within 2^-150 of the middle between two codes: position, dim, and the two elements in
+# units of 2^-133
+NEXT_TO_A_BORDER = [(2783, 28, 101, -94), (344, 42, -79, -51), (220, 38, 46, 34), (2835, 43, -49, 105), (1625, 38, -89, -114), (1199, 49, -36, 67),
+                    (3258, 55, -71, -78), (1235, 62, 46, 45), (1550, 53, 58, 54), (3907, 7, -39, -90), (4773, 63, -39, -115), (1646, 23, -35, -78)]
+
+
+def test_keys_below_the_smallest_normal_number_next_to_a_border():
+    n = len(NEXT_TO_A_BORDER)
+    b = Batch([1] * n, [p for p, *_ in NEXT_TO_A_BORDER], 1, 2, 16)
+    for i, (p, *_) in enumerate(NEXT_TO_A_BORDER):            # earlier tokens of the block: scale 2^-126 as well
+        b.scales[0][b.tables[i, p // 16]] = 2.0 ** -126
+    k = np.zeros((n, 1, ref.DIM))
+    for i, (_, d, x, y) in enumerate(NEXT_TO_A_BORDER):
+        k[i, 0, d], k[i, 0, d + 64] = x * 2.0 ** -133, y * 2.0 ** -133
+    v = b.rows(1)
+    pool, tables, lens, cu = b.device()
+    ops.kv8_append(*pool, dev(k), dev(v), tables, lens, cu)
+    check_append(b, k, v, 10000.0, pool=pool)
