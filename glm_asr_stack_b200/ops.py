@@ -272,6 +272,7 @@ def paged_decode_attention(query, k_cache, v_cache, block_tables, seq_lens, num_
 _KV8_STRUCT = struct.Struct("@QQQQiiii")        # glmasr_kv8_cache
 _KV8_SCALE = 128 ** -0.5
 _KV8_CODES = (torch.float8_e4m3fn, torch.uint8)
+_INT_MAX = 2 ** 31 - 1             # what the C calls take: lengths and counts beyond it are as good as this one
 _kv8_workspace_bytes = {}          # by device: a constant of the device's size
 
 
@@ -408,6 +409,12 @@ def kv8_attention(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
         raise ValueError("out must not overlap query")
     if n == 0 or tokens == 0:
         return out
+    max_new = (tokens + n - 1) // n if max_new is None else max_new
+    max_len = max_blocks * block_size if max_len is None else max_len
+    if (max_new | max_len | window | sinks) >> 31 != 0:         # a negative one, or one that does not fit 32 bits
+        if min(max_new, max_len, window, sinks) < 0:
+            raise ValueError("max_new, max_len, window and sinks must not be negative")
+        max_new, max_len, window, sinks = (min(x, _INT_MAX) for x in (max_new, max_len, window, sinks))
     lib = _lib.load()
     size = _kv8_workspace_bytes.get(device)
     if size is None:
@@ -419,8 +426,7 @@ def kv8_attention(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
         with torch.cuda.stream(stream):             # of the pool of the stream that works on it
             workspace = seq_lens.new_empty(size // 4)
     if lib.glmasr_kv8_attention(o, ldo, q, ldq, cache, block_tables.data_ptr(), max_blocks, seq_lens.data_ptr(), cu_new.data_ptr(), n, tokens, q_heads,
-                                (tokens + n - 1) // n if max_new is None else max_new, max_blocks * block_size if max_len is None else max_len, window, sinks,
-                                _KV8_SCALE if scale is None else scale, workspace.data_ptr(), size) != 0:
+                                max_new, max_len, window, sinks, _KV8_SCALE if scale is None else scale, workspace.data_ptr(), size) != 0:
         raise ValueError("glmasr_kv8_attention rejected the arguments")
     return out
 

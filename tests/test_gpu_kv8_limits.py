@@ -5,7 +5,7 @@ import torch
 
 import kv8_reference as ref
 from glm_asr_stack_b200 import _lib, ops
-from test_gpu_kv8 import Batch, check_append, dev
+from test_gpu_kv8 import Batch, check_append, check_attention, dev
 
 pytestmark = pytest.mark.gpu
 
@@ -181,3 +181,20 @@ def test_keys_below_the_smallest_normal_number_next_to_a_border():
     pool, tables, lens, cu = b.device()
     ops.kv8_append(*pool, dev(k), dev(v), tables, lens, cu)
     check_append(b, k, v, 10000.0, pool=pool)
+
+
+def test_numbers_that_do_not_fit_32_bits():
+    """A window, first tokens and expectations beyond every length there is: no limit, as 2^31 - 1 is, and not their low 32 bits."""
+    b = Batch([2, 1], [100, 50], 2, 4, 16)
+    q = b.rows(b.heads)
+    pool, tables, lens, cu = b.device()
+    want = ops.kv8_attention(dev(q), *pool, tables, lens, cu)
+    check_attention(b, q, want)
+    for far in (2 ** 31 - 1, 2 ** 31, 2 ** 32 + 16, 2 ** 40 + 3):
+        assert torch.equal(ops.kv8_attention(dev(q), *pool, tables, lens, cu, window=far), want), far
+        assert torch.equal(ops.kv8_attention(dev(q), *pool, tables, lens, cu, window=5, sinks=far), want), far
+        out = ops.kv8_attention(dev(q), *pool, tables, lens, cu, max_new=far, max_len=far)
+        check_attention(b, q, out)
+    for bad in ({"window": -2 ** 32 + 5}, {"window": 5, "sinks": -2 ** 32}, {"max_new": -2 ** 32 + 1}, {"max_len": -2 ** 32 + 1}):
+        with pytest.raises(ValueError):
+            ops.kv8_attention(dev(q), *pool, tables, lens, cu, **bad)
