@@ -286,12 +286,13 @@ __global__ void __launch_bounds__(threads(R), max_ctas(R)) kv8_attend_kernel(con
         tma_prefetch_desc(&p.tm_k);
         tma_prefetch_desc(&p.tm_v);
     }
+    // Tensor memory is asked for, without a limit to the wait, when no earlier kernel can be about to, and later ones start when this one
+    // has it: two kernels that each have a part and wait for the other cannot come about.
+    pdl_wait();
     if (warp == PRODUCTS) {
         tmem_alloc(smem_u32(&sm.tmem), TMEM_COLS);
         tmem_relinquish();
     }
-    pdl_wait();
-    pdl_launch_dependents();          // after the wait: the join may look at the batch before its own
 
     // rows of the queries' operand that no row of a context fills stay zero
     if constexpr (U < R) {
@@ -352,6 +353,7 @@ __global__ void __launch_bounds__(threads(R), max_ctas(R)) kv8_attend_kernel(con
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    pdl_launch_dependents();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(&sm.tmem);
     volatile int *abort_word = &sm.abort;
 

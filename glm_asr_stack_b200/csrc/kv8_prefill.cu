@@ -153,6 +153,8 @@ __global__ void __launch_bounds__(THREADS, 2) kv8_prefill_kernel(const __grid_co
         tma_prefetch_desc(&p.tm_k);
         tma_prefetch_desc(&p.tm_v);
     }
+    // as in the kernel for few queries: tensor memory after every earlier kernel, later ones when this one has it
+    pdl_wait();
     if (warp == 9) {
         tmem_alloc(smem_u32(&sm.tmem), TMEM_COLS);
         tmem_relinquish();
@@ -160,10 +162,9 @@ __global__ void __launch_bounds__(THREADS, 2) kv8_prefill_kernel(const __grid_co
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    pdl_launch_dependents();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(&sm.tmem);
     volatile int *abort_word = &sm.abort;
-    pdl_wait();                                               // nothing above touched global memory
-    pdl_launch_dependents();
 
     auto wait = [&](int i, uint32_t parity) { return mbar_wait_short(bar(i), parity & 1u, abort_word, ST_TIMEOUT_ATTENTION); };
     // the weighted sum of step t, the (t / STEPS)-th of its barrier, is done

@@ -100,3 +100,21 @@ def test_outputs_at_another_pitch_have_to_lie_apart(lib):
     assert append(lib, query=A, ldq=1024, out=A, ldo=2048) == -1
     assert append(lib, query=A, ldq=1024, out=A, ldo=2048, rows=1, key=64 * A, value=64 * A) == 0
     assert append(lib, query=A, ldq=1536, out=A, ldo=1536, key=A + 2048, ldk=1536, value=A + 2560, ldv=1536) == 0       # one fused projection
+
+
+def test_tensor_memory_is_asked_for_between_the_wait_and_the_signal():
+    """An allocation of tensor memory waits without a limit: only when all earlier kernels are done, and later ones may not start before
+    every warp of the block knows that it has come."""
+    kernels = 0
+    for name in sorted(os.listdir(CSRC)):
+        if not name.startswith("kv8_") or not name.endswith(".cu"):
+            continue
+        for body in open(os.path.join(CSRC, name)).read().split("__global__")[1:]:
+            if "tmem_alloc(" not in body:
+                continue
+            kernels += 1
+            alloc = body.index("tmem_alloc(")
+            assert body.count("tmem_alloc(") == 1 and body.count("pdl_launch_dependents();") == 1 and "pdl_wait();" in body[:alloc], name
+            signal = body.index("pdl_launch_dependents();")
+            assert "__syncthreads();" in body[alloc:signal], name
+    assert kernels == 2
