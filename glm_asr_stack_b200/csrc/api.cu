@@ -1651,7 +1651,7 @@ extern "C" int glmasr_fp4_status(void) {
         if (host[0] != 0) cudaMemset(g_noalloc_status_ptr[dev], 0, sizeof(host));
         if (code == 0) code = host[0];
     }
-    const int kv8 = kv8_take_status();
+    const int kv8 = kv8_status();
     return code != 0 ? code : kv8;
 }
 

@@ -81,6 +81,7 @@ __device__ __forceinline__ int warp_last_not_above(int n, long long x, Key key) 
 #endif
 
 int kv8_take_status();             // first status code of these kernels on the current device, cleared; 0 if none
+int kv8_status();                  // the same, without asking a device that none of them was launched on
 
 bool kv8_append_launch(uint8_t *k_cache, uint8_t *v_cache, float *k_scale, float *v_scale, const __nv_bfloat16 *key, long long ldk,
                        const __nv_bfloat16 *value, long long ldv, const __nv_bfloat16 *query, long long ldq, __nv_bfloat16 *query_out,

@@ -7,6 +7,13 @@
 
 using namespace glmasr;
 
+// two copies to the host and their module's load, which a program without this cache should not pay for
+static PerDevice<bool> g_attention_used;
+int glmasr::kv8_status() {
+    const bool *used = g_attention_used.here();
+    return used != nullptr && *used ? kv8_take_status() : 0;
+}
+
 namespace {
 
 bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
@@ -107,6 +114,7 @@ extern "C" int glmasr_kv8_attention(uint16_t *out, long long ldo, const uint16_t
     a.sinks = sinks < a.b.max_tokens ? sinks : a.b.max_tokens;
     a.scale_log2 = scale * 1.4426950408889634f;
     int launches = 0;
+    if (bool *used = g_attention_used.here()) *used = true;
     if (!kv8_attention_launch(a, max_new, max_len, workspace, current_stream(), launches)) {
         (void)cudaGetLastError();
         return -1;

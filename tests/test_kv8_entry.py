@@ -25,6 +25,11 @@ bool kv8_append_launch(uint8_t *, uint8_t *, float *, float *, const __nv_bfloat
 bool kv8_attention_launch(const Kv8Attend &a, int, int, void *, cudaStream_t, int &n) { ++launched; last = a; n = 1; return true; }
 }
 extern "C" cudaError_t cudaGetLastError() { return cudaSuccess; }
+int kv8_looks = 0, device = 0;
+namespace glmasr { int kv8_take_status() { ++kv8_looks; return 5; } }
+extern "C" cudaError_t cudaGetDevice(int *d) { *d = device; return cudaSuccess; }
+extern "C" int status(int on) { device = on; return glmasr::kv8_status(); }
+extern "C" int looks() { return kv8_looks; }
 extern "C" int launches() { return glmasr::launched; }
 """
 A = 1 << 20            # addresses that nothing follows
@@ -118,3 +123,13 @@ def test_tensor_memory_is_asked_for_between_the_wait_and_the_signal():
             signal = body.index("pdl_launch_dependents();")
             assert "__syncthreads();" in body[alloc:signal], name
     assert kernels == 2
+
+
+def test_the_status_of_a_device_without_such_a_launch_is_not_asked_for(lib):
+    assert attend(lib) == 0 and lib.status(0) == 5            # this device has one
+    before = lib.looks()
+    assert lib.status(1) == 0 and lib.status(2) == 0 and lib.looks() == before
+    assert append(lib) == 0 and lib.status(2) == 0            # an append waits for nothing
+    assert attend(lib, ws=0) == -1 and lib.status(2) == 0 and lib.looks() == before
+    assert attend(lib) == 0 and lib.status(2) == 5 and lib.status(1) == 0 and lib.looks() == before + 1
+    lib.status(0)
