@@ -198,11 +198,12 @@ __global__ void __launch_bounds__(THREADS, CTAS) kv8_append_kernel(const __grid_
     const int seq = warp_last_not_above(p.b.num_seqs, (long long)blockIdx.x, [&](int s) { return (long long)(cu[s] >> 4) + 2LL * s; });
     if (seq < 0) return;
     const int row0 = cu[seq], n_new = cu[seq + 1] - row0;
-    const int start = p.b.seq_lens[seq] - n_new;                 // position of the sequence's first new token
+    const int len = p.b.seq_lens[seq];
+    const int start = len - n_new;                               // position of the sequence's first new token
     const int group = (start >> 4) + ((int)blockIdx.x - (row0 >> 4) - 2 * seq);
-    if (n_new <= 0 || group < 0) return;
+    if (n_new <= 0 || len <= 0 || (uint32_t)group >= 1u << 27) return;           // before the first position, or behind the last there is
     const int pos = max(start, group * kKv8Group);               // first new token in this block
-    const int n = min(start + n_new, (group + 1) * kKv8Group) - pos;
+    const int n = min(len - group * kKv8Group, kKv8Group) - (pos - group * kKv8Group);
     if (n <= 0) return;
     // tokens that were in the block before: with a start inside the block they are the places below `first`
     Part part = {row0 + (pos - start), n, pos & (kKv8Group - 1), 0};

@@ -198,3 +198,25 @@ def test_numbers_that_do_not_fit_32_bits():
     for bad in ({"window": -2 ** 32 + 5}, {"window": 5, "sinks": -2 ** 32}, {"max_new": -2 ** 32 + 1}, {"max_len": -2 ** 32 + 1}):
         with pytest.raises(ValueError):
             ops.kv8_attention(dev(q), *pool, tables, lens, cu, **bad)
+
+
+@pytest.mark.parametrize("length", [2 ** 31 - 1, 2 ** 31 - 2, 2 ** 31 - 16, 2 ** 31 - 17, -1, -2 ** 31, -2 ** 31 + 1])
+def test_a_length_that_cannot_be_is_its_own_sequence_s_concern(length):
+    """Behind every table, or below zero: nothing of it is written, and the sequences around it are as without it."""
+    b = Batch([2, 1, 3, 1], [40, 50, 20, 7], 2, 4, 16)
+    q, k, v = b.rows(b.heads), b.rows(2), b.rows(2)
+    pool, tables, lens, cu = b.device()
+    lens[1] = length
+    qo = torch.full((b.total, b.heads, 128), 7.0, dtype=torch.bfloat16, device="cuda")
+    ops.kv8_append(*pool, dev(k), dev(v), tables, lens, cu, query=dev(q), query_out=qo)
+    around = [0, 1, 3, 4, 5, 6]
+    got = qo[around]
+    b.new[1], b.tables[1] = 0, -1                             # the same batch without it
+    keep = np.array(around)
+    b.cu, b.total = np.array([0, 2, 2, 5, 6], dtype=np.int32), 6
+    check_append(b, k[keep], v[keep], 10000.0, q[keep], got, pool)
+    for max_new in (1, 100_000):
+        out = ops.kv8_attention(qo, *pool, tables, lens, cu, max_new=max_new)
+        check_attention(b, got.double().cpu().numpy(), out[around])
+        assert length > 0 or not torch.any(out[2])
+    assert ops.status() == 0
