@@ -55,21 +55,21 @@ ATTEND = dict(out=A, ldo=1024, query=2 * A, ldq=1024, tables=A, max_blocks=4, le
               sinks=0, scale=0.1, ws=A, ws_bytes=4096)
 
 
-def append(lib, cache=CACHE, **change):
+def append(lib, cache=CACHE, launches=1, **change):
     f = {**APPEND, **change}
     c = ctypes.byref(_lib.Kv8Cache(*[cache[n] for n, _ in _lib.Kv8Cache._fields_])) if cache is not None else None
     before = lib.launches()
     code = lib.glmasr_kv8_append(c, *f.values())
-    assert (code == 0 and lib.launches() == before + 1) or lib.launches() == before
+    assert lib.launches() - before == (launches if code == 0 else 0)
     return code
 
 
-def attend(lib, cache=CACHE, **change):
+def attend(lib, cache=CACHE, launches=1, **change):
     f = {**ATTEND, **change}
     c = ctypes.byref(_lib.Kv8Cache(*[cache[n] for n, _ in _lib.Kv8Cache._fields_])) if cache is not None else None
     before = lib.launches()
     code = lib.glmasr_kv8_attention(f["out"], f["ldo"], f["query"], f["ldq"], c, *list(f.values())[4:])
-    assert (code == 0 and lib.launches() == before + 1) or lib.launches() == before
+    assert lib.launches() - before == (launches if code == 0 else 0)
     return code
 
 
@@ -133,3 +133,47 @@ def test_the_status_of_a_device_without_such_a_launch_is_not_asked_for(lib):
     assert attend(lib, ws=0) == -1 and lib.status(2) == 0 and lib.looks() == before
     assert attend(lib) == 0 and lib.status(2) == 5 and lib.status(1) == 0 and lib.looks() == before + 1
     lib.status(0)
+
+
+BAD_CACHES = [{"k": 0}, {"v": 0}, {"k_scale": 0}, {"v_scale": 0}, {"k": A + 4}, {"v": A + 8}, {"k_scale": A + 2}, {"v_scale": A + 1}, {"num_blocks": 0}, {"num_blocks": -1},
+              {"block_size": 0}, {"block_size": -16}, {"block_size": 24}, {"kv_heads": 0}, {"kv_heads": -2}, {"head_dim": 64}, {"head_dim": 256},
+              {"num_blocks": 1 << 26}, {"num_blocks": 1 << 16, "block_size": 1 << 14}]
+BAD_BATCHES = [{"tables": 0}, {"tables": A + 2}, {"lens": 0}, {"lens": A + 1}, {"cu": 0}, {"cu": A + 3}, {"seqs": -1}, {"rows": -1}, {"max_blocks": 0}, {"max_blocks": -1}]
+
+
+def test_good_calls_are_launched(lib):
+    assert append(lib) == 0 and attend(lib) == 0
+    assert append(lib, query=None, out=None, heads=0, ldq=0, ldo=0) == 0
+    assert append(lib, theta=0.0) == 0 and append(lib, ldk=256 + 8, ldv=512, ldq=1032) == 0
+    assert attend(lib, window=1 << 30, sinks=1 << 30, max_new=0, max_len=0, scale=0.0) == 0
+    largest = {**CACHE, "num_blocks": (1 << 26) - 1}         # 2^31 - 32 rows of codes
+    assert append(lib, largest) == 0 and attend(lib, largest) == 0
+    nothing = dict(launches=0, query=None, out=None)          # to do: no error, whatever the rows are
+    assert append(lib, rows=0, key=0, value=0, **nothing) == 0 and append(lib, seqs=0, key=0, value=0, **nothing) == 0
+    assert attend(lib, rows=0, ws=0, **nothing) == 0 and attend(lib, seqs=0, ws=0, **nothing) == 0
+
+
+@pytest.mark.parametrize("change", BAD_CACHES)
+def test_a_bad_cache_is_refused(lib, change):
+    assert append(lib, {**CACHE, **change}) == -1 and attend(lib, {**CACHE, **change}) == -1
+    assert append(lib, None) == -1 and attend(lib, None) == -1
+
+
+@pytest.mark.parametrize("change", BAD_BATCHES)
+def test_a_bad_batch_is_refused(lib, change):
+    assert append(lib, **change) == -1 and attend(lib, **change) == -1
+
+
+@pytest.mark.parametrize("change", [{"key": 0}, {"key": A + 2}, {"ldk": 252}, {"ldk": 128}, {"ldk": -256}, {"value": 0}, {"value": A + 8}, {"ldv": 255}, {"ldv": 248},
+                                    {"theta": -1.0}, {"theta": float("nan")}, {"theta": float("inf")}, {"query": None}, {"out": None}, {"heads": 0}, {"heads": -8},
+                                    {"query": 2 * A + 8}, {"ldq": 1020}, {"ldq": 512}, {"out": 3 * A + 4}, {"ldo": 1028}, {"ldo": 1016}])
+def test_append_refuses(lib, change):
+    assert append(lib, **change) == -1
+
+
+@pytest.mark.parametrize("change", [{"out": 0}, {"out": A + 8}, {"ldo": 1020}, {"ldo": 1016}, {"query": 0}, {"query": 2 * A + 2}, {"ldq": 1028}, {"ldq": 512}, {"heads": 0},
+                                    {"heads": 7}, {"heads": -2}, {"max_new": -1}, {"max_len": -1}, {"window": -1}, {"sinks": -1}, {"scale": float("nan")},
+                                    {"scale": -1.0}, {"scale": float("inf")}, {"ws": 0}, {"ws": A + 8}, {"ws_bytes": 4095}, {"ws_bytes": 0}, {"ws_bytes": -1},
+                                    {"rows": 1 << 28, "ldq": 1024, "query": 1 << 50}])
+def test_attention_refuses(lib, change):
+    assert attend(lib, **change) == -1
