@@ -263,7 +263,11 @@ __global__ void __launch_bounds__(threads(R), max_ctas(R)) kv8_attend_kernel(con
     const uint32_t sbase = smem_u32(smem_raw);
     auto bar = [&](int i) { return smem_u32(&sm.bars[i]); };
     if ((sbase & 1023u) != 0) {                               // the swizzled tiles need a 1024-byte aligned base
-        if (threadIdx.x == 0) atomicCAS(&g_kv8_status[0], 0, ST_BAD_LAYOUT);
+        pdl_wait();
+        if (threadIdx.x == 0) {
+            atomicCAS(&g_kv8_status[0], 0, ST_BAD_LAYOUT);
+            if (!p.whole) p.part.join[blockIdx.x].last = -1;      // else the join would take what lies there for work
+        }
         return;
     }
     if (threadIdx.x == 0) {

@@ -177,3 +177,13 @@ def test_append_refuses(lib, change):
                                     {"rows": 1 << 28, "ldq": 1024, "query": 1 << 50}])
 def test_attention_refuses(lib, change):
     assert attend(lib, **change) == -1
+
+
+def test_a_block_that_gives_up_leaves_nothing_to_join():
+    """The second launch reads each block's word on what to join, whatever became of the block: written on every way out."""
+    body = open(os.path.join(CSRC, "kv8_attention.cu")).read().split("__global__")[1]
+    ways_out = [body[:i] for i in range(len(body)) if body.startswith("        return;\n", i) and "mbar_init" not in body[:i]]
+    assert len(ways_out) == 1
+    for way in ways_out:
+        assert "p.part.join[blockIdx.x].last = -1" in way and way.index("pdl_wait();") < way.index("p.part.join")
+    assert "if (leader && !p.whole) p.part.join[blockIdx.x] = join;" in body
