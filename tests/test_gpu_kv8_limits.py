@@ -220,3 +220,188 @@ def test_a_length_that_cannot_be_is_its_own_sequence_s_concern(length):
         check_attention(b, got.double().cpu().numpy(), out[around])
         assert length > 0 or not torch.any(out[2])
     assert ops.status() == 0
+
+
+def in_pieces(b, q, columns, **more):
+    """The attention of a batch whose table has room for so many pages that a context is cut into pieces, which a second launch joins."""
+    pool, tables, lens, cu = b.device()
+    tables = torch.nn.functional.pad(tables, (0, max(0, columns - tables.shape[1])), value=-1)
+    out = torch.full((q.shape[0], b.heads, 128), 7.0, dtype=torch.bfloat16, device="cuda")
+    before = ops.launch_count()
+    ops.kv8_attention(dev(q), *pool, tables, lens, cu, max_len=50_000, out=out, **more)
+    assert ops.launch_count() - before == 2
+    assert ops.status() == 0
+    return out
+
+
+LENGTHS = [1, 2, 15, 16, 17, 33, 127, 128, 129, 300, 513, 2049, 2500]
+
+
+@pytest.mark.parametrize("kv_heads,group,page", [(4, 4, 16), (2, 1, 48), (1, 8, 64), (1, 20, 32), (2, 3, 16)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (2100, 0), (2100, 40), (2200, 2300), (5000, 4)])
+def test_pieces_of_contexts(kv_heads, group, page, window, sinks):
+    """One query each; a window of more than 16 tiles, so that pieces begin and end before, in and behind what it leaves out."""
+    b = Batch([1] * len(LENGTHS), [n - 1 for n in LENGTHS], kv_heads, group, page)
+    q = b.rows(b.heads)
+    check_attention(b, q, in_pieces(b, q, 5120 // page, max_new=1, window=window, sinks=sinks), window, sinks)
+
+
+@pytest.mark.parametrize("new", [1, 2, 4, 7])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (2100, 100), (2100, 1)])
+def test_pieces_with_a_gap_between_the_first_tokens_and_the_window(new, window, sinks):
+    b = Batch([new] * 3, [4100, 3333, 2101], 1, 4, 16)
+    q = b.rows(b.heads, extra=2)
+    out = in_pieces(b, q, 320, max_new=new, window=window, sinks=sinks)
+    check_attention(b, q, out, window, sinks)
+    assert torch.all(out[b.total:] == 7)
+
+
+def test_pieces_of_few_units_over_all_blocks():
+    """Fewer groups than blocks, more sequences than blocks, and sequences without any."""
+    for ctx in ([700], [3000, 0], [17] * 500, [0] * 30 + [2600] + [0] * 30):
+        b = Batch([1] * len(ctx), ctx, 2, 4, 16)
+        q = b.rows(b.heads)
+        check_attention(b, q, in_pieces(b, q, 400, max_new=1))
+
+
+def test_pieces_of_a_batch_without_a_new_token():
+    b = Batch([0, 0, 0], [5, 0, 40], 2, 4, 16)
+    out = in_pieces(b, np.full((9, 8, 128), np.nan), 400, max_new=1)
+    assert torch.all(out == 7)
+
+
+@pytest.mark.parametrize("new", [1, 3])
+def test_pieces_of_a_prefix_that_sequences_share(new):
+    b = Batch([new, 2, 1], [2000, 1500, 900], 2, 4, 16)
+    b.tables[1, :60], b.tables[2, :50] = b.tables[0, :60], b.tables[0, :50]
+    q = b.rows(b.heads)
+    check_attention(b, q, in_pieces(b, q, 400, max_new=new))
+
+
+@pytest.mark.parametrize("new", [1, 3, 7])
+def test_pieces_with_pages_that_are_not_there(new):
+    """Missing pages from the first to the last, a whole piece of them, none at all; lengths below the new tokens; and what lies in places
+    that nothing is in does not matter."""
+    b = Batch([new] * 5, [2500, 700, 1900, 9, 40], 2, 4, 16, missing=[(0, 0), (0, 3), (2, 1), (2, 110), (1, 20)] + [(0, j) for j in range(30, 90)])
+    b.tables[3, :] = -1
+    b.tables[2, 60:70] = b.blocks + 5
+    b.lens[4] = new - 1
+    used = np.zeros((b.blocks, 16), dtype=bool)
+    for i in range(5):
+        for p in range(b.lens[i]):
+            if 0 <= b.tables[i, p // 16] < b.blocks:
+                used[b.tables[i, p // 16], p % 16] = True
+    for c, s in zip(b.codes, b.scales):
+        c[np.broadcast_to(~used[:, None, :, None], c.shape)] = 0x7F
+        s[np.broadcast_to(~used.any(1)[:, None, None], s.shape)] = np.nan
+    q = b.rows(b.heads)
+    out = in_pieces(b, q, 400, max_new=new)
+    check_attention(b, q, out)
+    assert torch.all(out[3 * new:4 * new] == 0)
+
+
+@pytest.mark.parametrize("new", [1, 4])
+def test_pieces_of_pages_a_window_has_left_behind(new):
+    b = Batch([new, new], [4000, 3333], 2, 4, 16)
+    for i in range(2):
+        for j in range(2, (b.ctx[i] - 2200 + 1) // 16):
+            b.tables[i, j] = -1 if j % 2 else b.blocks + 9
+    q = b.rows(b.heads)
+    full = Batch([new, new], [4000, 3333], 2, 4, 16)
+    check_attention(full, q, in_pieces(b, q, 400, max_new=new, window=2200, sinks=20), 2200, 20)
+
+
+@pytest.mark.parametrize("new", [1, 4])
+@pytest.mark.parametrize("which", [0, 1])
+def test_pieces_with_a_poisoned_block(new, which):
+    """In the first, a middle and the last piece of a context: every query that sees it, and no other."""
+    for place in (0, 60, (2000 + new - 1) // 16):
+        b = Batch([new, new], [2000, 2000], 2, 2, 16)
+        b.scales[which][b.tables[0, place], 1], b.codes[which][b.tables[0, place], 1] = np.nan, 0
+        q = b.rows(b.heads)
+        got = torch.isnan(in_pieces(b, q, 400, max_new=new)).cpu().numpy()
+        want = np.zeros((2 * new, 4), dtype=bool)
+        for t in range(new):
+            want[t, 2:] = 2000 + t >= place * 16
+        assert np.array_equal(got.all(2), want) and np.array_equal(got.any(2), want)
+        # a window that has left it behind
+        if place == 60:
+            assert not torch.any(torch.isnan(in_pieces(b, q, 400, max_new=new, window=1000)))
+
+
+@pytest.mark.parametrize("new", [1, 4])
+@pytest.mark.parametrize("span", [8, 30, 60])
+def test_pieces_of_scales_far_apart(new, span):
+    """The parts of a context have references far from each other."""
+    b = Batch([new, new], [2000, 1077], 1, 4, 16, seed=span)
+    run = np.repeat(b.rng.integers(-span, 1, -(-b.blocks // 7)), 7)[:b.blocks]
+    for i in range(2):                                        # some 110 tokens in a row under one scale
+        n = (b.tables[i] >= 0).sum()
+        b.scales[1][b.tables[i, :n]] = (2.0 ** run[:n].astype(np.float64))[:, None, None]
+    b.scales[0] *= (2.0 ** b.rng.integers(-6, 3, b.scales[0].shape)).astype(np.float32)
+    q = b.rows(4)
+    q[0] *= 2.0 ** -100
+    q[-1] = 0
+    check_attention(b, q, in_pieces(b, q, 400, max_new=new))
+
+
+@pytest.mark.parametrize("name", LADDERS)
+def test_pieces_of_v_scales_that_change_along_the_context(name):
+    """As whole contexts have them: a part's small weights on large values count in the whole."""
+    steps = LADDERS[name]
+    b, q = ladder(steps, 64 * len(steps) + 70 + 3, 3)
+    out = in_pieces(b, q, 400, max_new=3, scale=LN2).float().cpu().numpy()
+    for row in range(3):
+        want, tol = bound(b, q, row)
+        assert np.all(np.abs(out[row:row + 1] - want) <= tol), (row, (np.abs(out[row:row + 1] - want) / tol).max())
+
+
+@pytest.mark.parametrize("new", [1, 6])
+def test_pieces_captured_replayed_and_on_two_streams(new):
+    """Two graphs of an append and an attention in pieces, each with a workspace of its own, replayed at once on two streams with other
+    lengths than they were captured with: as the eager calls."""
+    b = Batch([new] * 3, [2000, 17, 900], 2, 4, 16)
+    q, k, v = dev(b.rows(b.heads)), dev(b.rows(2)), dev(b.rows(2))
+    wide = lambda t: torch.nn.functional.pad(t, (0, 400 - t.shape[1]), value=-1)  # noqa: E731
+    graphs = []
+    for g in range(2):
+        pool, tables, lens, cu = b.device()
+        tables = wide(tables)
+        out = torch.zeros_like(q)
+        s = torch.cuda.Stream()
+        torch.cuda.synchronize()
+        ops.set_stream(s)
+        try:
+            with torch.cuda.stream(s):
+                def run():
+                    r = ops.kv8_append(*pool, k, v, tables, lens, cu, query=q)
+                    ops.kv8_attention(r, *pool, tables, lens, cu, max_new=new, max_len=50_000, out=out)
+                before = ops.launch_count()
+                run()
+                assert ops.launch_count() - before == 3
+                torch.cuda.synchronize()
+                graph = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(graph, stream=s):
+                    run()
+        finally:
+            ops.set_stream(None)
+        graphs.append((graph, s, pool, lens, out, tables, cu))
+    for shift in (0, 3, -9, -900):
+        fresh = b.device()
+        for (graph, s, pool, lens, out, _, _), d in zip(graphs, (shift, shift + 1)):
+            for t, f in zip(pool, fresh[0]):
+                t.copy_(f)
+            lens.copy_(torch.clamp(fresh[2] + d, min=new))
+        torch.cuda.synchronize()
+        for _ in range(3):                                    # the same tokens again leave the cache as it is
+            for graph, s, *_ in graphs:
+                with torch.cuda.stream(s):
+                    graph.replay()
+        torch.cuda.synchronize()
+        for graph, s, pool, lens, out, tables, cu in graphs:
+            eager = b.device()[0]
+            r = ops.kv8_append(*eager, k, v, tables, lens, cu, query=q)
+            want = ops.kv8_attention(r, *eager, tables, lens, cu, max_new=new, max_len=50_000)
+            assert torch.equal(out, want)
+            assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(pool, eager))
+    assert ops.status() == 0
