@@ -89,7 +89,11 @@ extern "C" int glmasr_kv8_append(const glmasr_kv8_cache *cache, const uint16_t *
     return 0;
 }
 
-extern "C" long long glmasr_kv8_attention_workspace(void) { return (long long)kv8_attention_workspace_bytes(); }
+extern "C" long long glmasr_kv8_attention_workspace(void) {
+    if (g_attention_used.here() != nullptr) return (long long)kv8_attention_workspace_bytes();
+    (void)cudaGetLastError();                                 // no device: what asks for its size would end the process
+    return 0;
+}
 
 extern "C" int glmasr_kv8_attention(uint16_t *out, long long ldo, const uint16_t *query, long long ldq, const glmasr_kv8_cache *cache,
                                     const int *block_tables, int max_blocks, const int *seq_lens, const int *cu_new, int num_seqs,
@@ -101,7 +105,8 @@ extern "C" int glmasr_kv8_attention(uint16_t *out, long long ldo, const uint16_t
     if (num_seqs == 0 || total_new == 0) return 0;
     if (!rows_ok(query, ldq, q_heads, total_new) || !rows_ok(out, ldo, q_heads, total_new)) return -1;
     if (rows_overlap(out, ldo, q_heads, query, ldq, q_heads, total_new)) return -1;
-    if (workspace == nullptr || !aligned16(workspace) || workspace_bytes < glmasr_kv8_attention_workspace()) return -1;
+    const long long needed = glmasr_kv8_attention_workspace();
+    if (needed == 0 || workspace == nullptr || !aligned16(workspace) || workspace_bytes < needed) return -1;
     a.k_cache = cache->k, a.v_cache = cache->v;
     a.k_scale = cache->k_scale, a.v_scale = cache->v_scale;
     a.query = (const __nv_bfloat16 *)query;
@@ -114,7 +119,7 @@ extern "C" int glmasr_kv8_attention(uint16_t *out, long long ldo, const uint16_t
     a.sinks = sinks < a.b.max_tokens ? sinks : a.b.max_tokens;
     a.scale_log2 = scale * 1.4426950408889634f;
     int launches = 0;
-    if (bool *used = g_attention_used.here()) *used = true;
+    *g_attention_used.here() = true;
     if (!kv8_attention_launch(a, max_new, max_len, workspace, current_stream(), launches)) {
         (void)cudaGetLastError();
         return -1;

@@ -432,7 +432,7 @@ int glmasr_kv8_append(const glmasr_kv8_cache *cache, const uint16_t *key, long l
  * out, query: bf16 [total_new, q_heads * 128] with row pitches ldo, ldq (multiples of 8; 16-byte aligned); q_heads a multiple of
  * kv_heads.  scale: of the scores, before the softmax.  max_new (new tokens of a sequence) and max_len (tokens of a sequence)
  * say what to expect: they choose kernels (which differ in the order of sums and in rounding), never what is seen or computed.
- * workspace: glmasr_kv8_attention_workspace() bytes (for the current device) of device memory, 16-byte aligned, contents irrelevant,
+ * workspace: glmasr_kv8_attention_workspace() bytes (for the current device; 0 without one) of device memory, 16-byte aligned, contents irrelevant,
  * not shared with a call that may run at the same time.  out must not overlap query (columns of one array at one pitch may lie side by
  * side).  Returns 0, or -1 on bad arguments or a launch failure. */
 long long glmasr_kv8_attention_workspace(void);

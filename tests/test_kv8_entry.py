@@ -4,6 +4,7 @@ import ctypes
 import os
 import random
 import subprocess
+import sys
 
 import pytest
 
@@ -27,7 +28,7 @@ bool kv8_attention_launch(const Kv8Attend &a, int, int, void *, cudaStream_t, in
 extern "C" cudaError_t cudaGetLastError() { return cudaSuccess; }
 int kv8_looks = 0, device = 0;
 namespace glmasr { int kv8_take_status() { ++kv8_looks; return 5; } }
-extern "C" cudaError_t cudaGetDevice(int *d) { *d = device; return cudaSuccess; }
+extern "C" cudaError_t cudaGetDevice(int *d) { *d = device; return device < 0 ? cudaErrorNoDevice : cudaSuccess; }
 extern "C" int status(int on) { device = on; return glmasr::kv8_status(); }
 extern "C" int looks() { return kv8_looks; }
 extern "C" int launches() { return glmasr::launched; }
@@ -43,7 +44,7 @@ def lib(tmp_path_factory):
     subprocess.run(["g++", "-std=c++17", "-shared", "-fPIC", "-Wl,-Bsymbolic", "-I", CSRC, "-I", os.path.join(cuda, "include"), "-o", str(tmp / "e.so"),
                     str(tmp / "fakes.cpp"), "-x", "c++", os.path.join(CSRC, "kv8_api.cu")], check=True, capture_output=True)
     dll = ctypes.CDLL(str(tmp / "e.so"))
-    for name in ("glmasr_kv8_append", "glmasr_kv8_attention"):
+    for name in ("glmasr_kv8_append", "glmasr_kv8_attention", "glmasr_kv8_attention_workspace"):
         getattr(dll, name).restype, getattr(dll, name).argtypes = _lib.SIGNATURES[name]
     return dll
 
@@ -187,3 +188,22 @@ def test_a_block_that_gives_up_leaves_nothing_to_join():
     for way in ways_out:
         assert "p.part.join[blockIdx.x].last = -1" in way and way.index("pdl_wait();") < way.index("p.part.join")
     assert "if (leader && !p.whole) p.part.join[blockIdx.x] = join;" in body
+
+
+def test_without_a_device_the_calls_return(lib):
+    """-1, and a workspace of 0 bytes; what asks for the device's size ends the process where there is none."""
+    lib.status(-1)
+    assert lib.glmasr_kv8_attention_workspace() == 0 and attend(lib) == -1 and lib.status(-1) == 0
+    lib.status(0)
+    assert lib.glmasr_kv8_attention_workspace() == 4096 and attend(lib) == 0
+    code = """if True:
+        import ctypes, sys
+        sys.path[:0] = [%r, %r]
+        from glm_asr_stack_b200 import _lib
+        import test_kv8_host as t
+        size = _lib.load().glmasr_kv8_attention_workspace()
+        print(size, t._append(t._c_cache()), t._attend(t._c_cache(), ws_bytes=1 << 40))
+    """ % (ROOT, os.path.join(ROOT, "tests"))
+    env = {**os.environ, "CUDA_VISIBLE_DEVICES": ""}
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, env=env)
+    assert r.returncode == 0 and r.stdout.split() == ["0", "-1", "-1"], (r.stdout, r.stderr)
