@@ -105,8 +105,9 @@ extern "C" int glmasr_kv8_attention(uint16_t *out, long long ldo, const uint16_t
     if (num_seqs == 0 || total_new == 0) return 0;
     if (!rows_ok(query, ldq, q_heads, total_new) || !rows_ok(out, ldo, q_heads, total_new)) return -1;
     if (rows_overlap(out, ldo, q_heads, query, ldq, q_heads, total_new)) return -1;
-    const long long needed = glmasr_kv8_attention_workspace();
-    if (needed == 0 || workspace == nullptr || !aligned16(workspace) || workspace_bytes < needed) return -1;
+    bool *used = g_attention_used.here();
+    if (used == nullptr) (void)cudaGetLastError();
+    if (used == nullptr || workspace == nullptr || !aligned16(workspace) || workspace_bytes < (long long)kv8_attention_workspace_bytes()) return -1;
     a.k_cache = cache->k, a.v_cache = cache->v;
     a.k_scale = cache->k_scale, a.v_scale = cache->v_scale;
     a.query = (const __nv_bfloat16 *)query;
@@ -119,7 +120,7 @@ extern "C" int glmasr_kv8_attention(uint16_t *out, long long ldo, const uint16_t
     a.sinks = sinks < a.b.max_tokens ? sinks : a.b.max_tokens;
     a.scale_log2 = scale * 1.4426950408889634f;
     int launches = 0;
-    *g_attention_used.here() = true;
+    *used = true;
     if (!kv8_attention_launch(a, max_new, max_len, workspace, current_stream(), launches)) {
         (void)cudaGetLastError();
         return -1;

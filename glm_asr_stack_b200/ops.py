@@ -272,6 +272,7 @@ def paged_decode_attention(query, k_cache, v_cache, block_tables, seq_lens, num_
 _KV8_STRUCT = struct.Struct("@QQQQiiii")        # glmasr_kv8_cache
 _KV8_SCALE = 128 ** -0.5
 _KV8_CODES = (torch.float8_e4m3fn, torch.uint8)
+_current_device, _current_raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 _INT_MAX = 2 ** 31 - 1             # what the C calls take: lengths and counts beyond it are as good as this one
 _kv8_workspace_bytes = {}          # by device: a constant of the device's size
 
@@ -298,7 +299,7 @@ def _kv8_cache(k_cache, v_cache, k_scale, v_scale):
     if (len(shape) == 4 and v_cache.shape == shape and k_cache.dtype in _KV8_CODES and v_cache.dtype in _KV8_CODES
             and k_cache.is_contiguous() and v_cache.is_contiguous() and k_scale.dtype is torch.float32 and v_scale.dtype is torch.float32
             and k_scale.shape == v_scale.shape == (shape[0], shape[1], shape[2] // 16) and k_scale.is_contiguous() and v_scale.is_contiguous()
-            and device >= 0 and device == v_cache.get_device() == k_scale.get_device() == v_scale.get_device() == torch._C._cuda_getDevice()):
+            and device >= 0 and device == v_cache.get_device() == k_scale.get_device() == v_scale.get_device() == _current_device()):
         return _KV8_STRUCT.pack(k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), shape[0], shape[2], shape[1],
                                 shape[3]), device, shape[1], shape[2]
     if device < 0:
@@ -328,7 +329,7 @@ def _kv8_batch(block_tables, seq_lens, cu_new, device: int):
 
 def _kv8_launch_stream(device: int):
     """The stream of set_stream(), or None where it is torch's current one."""
-    if (0 if _stream is None else _stream.cuda_stream) == torch._C._cuda_getCurrentRawStream(device):
+    if (0 if _stream is None else _stream.cuda_stream) == _current_raw_stream(device):
         return None
     return torch.cuda.default_stream(device) if _stream is None else _stream
 
@@ -419,11 +420,10 @@ def kv8_attention(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
     size = _kv8_workspace_bytes.get(device)
     if size is None:
         size = _kv8_workspace_bytes[device] = lib.glmasr_kv8_attention_workspace()
-    stream = _kv8_launch_stream(device)
-    if stream is None:
+    if (0 if _stream is None else _stream.cuda_stream) == _current_raw_stream(device):
         workspace = seq_lens.new_empty(size // 4)   # a multiple of 256 bytes; cheaper than torch.empty
     else:
-        with torch.cuda.stream(stream):             # of the pool of the stream that works on it
+        with torch.cuda.stream(_kv8_launch_stream(device)):     # of the pool of the stream that works on it
             workspace = seq_lens.new_empty(size // 4)
     if lib.glmasr_kv8_attention(o, ldo, q, ldq, cache, block_tables.data_ptr(), max_blocks, seq_lens.data_ptr(), cu_new.data_ptr(), n, tokens, q_heads,
                                 max_new, max_len, window, sinks, _KV8_SCALE if scale is None else scale, workspace.data_ptr(), size) != 0:
