@@ -10,9 +10,9 @@
 // shared memory, while its first rows are on their way.
 //
 // Bound: the rows' bytes for many tokens, but every CTA is a chain (its sequence, lengths, rows, angles, scale, stores), so there are
-// three CTAs per SM (80 registers, eight tokens of a head per warp): 10000 tokens of 25 prompts take 27.9 us (62% of the copy
+// three CTAs per SM (80 registers, eight tokens of a head per warp): 10000 tokens of 25 prompts take 27.8 us (62% of the copy
 // bandwidth); 46 us with two CTAs of 128 registers whose warps had sixteen tokens, and the queries as well.  256 sequences
-// with a token each take 6.5 us (7.3), one token 3.4 us (4.9).
+// with a token each take 6.6 us (7.3), one token 3.4 us (4.9).
 //
 // Angles and keys are computed in 64 bits.  A key decides by comparison which code, and which scale, it gets; in 32 bits about one
 // value in a million falls on the wrong side of a border, and a position of 100000 has lost 7 bits of its angle before the

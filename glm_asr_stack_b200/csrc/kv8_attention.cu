@@ -5,7 +5,7 @@
 // queries are the narrow one:
 //   S^T [128 tokens, rows] = K Q^T,    O^T [128 dims, rows] += V^T P^T      (tcgen05, e4m3 x e4m3, sums in fp32)
 // so no code is ever converted and no thread touches a key or a value.  (Warp-level products of the same formulas on converted
-// codes took 450 instructions per 32 tokens and warp, and 29 us where this kernel takes 24.6 us for 256 sequences of 200 to 450 tokens.)
+// codes took 450 instructions per 32 tokens and warp, and 29 us where this kernel takes 24.7 us for 256 sequences of 200 to 450 tokens.)
 //   queries  A row is taken times a power of two that brings its largest element to 2^7 and split into two e4m3 numbers,
 //            q = hi + 2^-5 lo, side by side as columns: a bf16 number has 8 bits, each of them carries 4, so the split is exact for
 //            elements down to 2^-14 of the largest, and off by 2^-22 of the largest below.
@@ -881,10 +881,12 @@ size_t kv8_attention_workspace_bytes() {
 // Whole (sequence, kv head) pairs or pieces?  In cycles, from what the phases of the kernel take: a tile's chain 2200, the steps around a
 // context 2600, an SM's share of HBM 1400 a tile; pieces need 2000 for the table of units and 5000 for the join.  The longest
 // context stands for all, which flatters whole pairs where lengths are uneven, hence their limit of 8 tiles, or 16 if a window makes
-// them even.  Measured, us, whole : pieces (sequences of one new token, four heads a kv head, tokens):
-//   1 x 250        7.0 : 8.6    1 x 900       14 : 9.4    16 x 450      9.6 : 11.1   16 x 900      14 : 12.5    64 x 450      11 : 13
-//   64 x 900        17 : 18     64 x 2000     30 : 37     128 x 900     34 : 30      128 x 2000    61 : 51      256 x 450     29 : 35
-//   64 x 500..2000  25 : 20     128 x 225..900  23 : 21   128 x 500..2000  48 : 36   256 x 112..450  22 : 29    256 x 500..2000  67 : 62
+// them even.  Measured, us, whole : pieces (sequences of one new token, four kv heads with four heads each, tokens):
+//   1 x 250        7.0 : 8.1    1 x 900      13.9 : 9.1    16 x 450      9.5 : 11.7   16 x 900     14.2 : 13.1   64 x 450     11.3 : 13.8
+//   64 x 900      18.1 : 20.1   64 x 2000    28.9 : 30.7*  128 x 900    31.5 : 29.6*  128 x 2000   55.2 : 51.2   256 x 450    28.4 : 31.5
+//   64 x 500..2000  27.4 : 23.5   128 x 225..900  25.8 : 23.3*  128 x 500..2000  48.6 : 36.5  256 x 112..450  23.4 : 25.6  256 x 500..2000  67.3 : 61.8
+// On the lines with a star the rule takes the slower side, by 6 to 11%: it takes the same for even and uneven lengths, which it cannot tell
+// apart.  Other head layouts were not measured; the rule knows them by the number of contexts alone.
 static bool deal_whole(const Kv8Attend &a, int max_len, int slots) {
     const long long contexts = (long long)a.b.num_seqs * a.b.kv_heads;
     long long tokens = max_len < a.b.max_tokens ? max_len : a.b.max_tokens;
@@ -910,11 +912,12 @@ static int tile_rows(long long want) {
 // This kernel, or the one for many queries (128 rows of a (sequence, kv head) to a CTA, no splitting of long contexts)?  In cycles, two CTAs
 // per SM.  This one: 17000 around it all, 10000 for a tile of 128 tokens and up to 32 rows; lengths are taken to be uneven, half of the
 // longest on average, with a tile's worth for each context.  The other: 10000 for an item, and 2100 for 64 keys, 2700 when two
-// items share an SM.  Measured, us, this one : the other (sequences x new tokens of four heads a kv head, context):
-//   64 x 8, 200..2000    50 : 50     256 x 8, 200..450   62 : 64     19 x 8, 40..4450   36 : 80     4 x 8, 8000     33 : 139
-//   64 x 16, 200..2000   96 : 55     256 x 16, 200..450  121 : 68    19 x 12, 40..4450  43 : 80     2 x 16, 30000   57 : 498
-//   1 x 16, 200          20 : 10     1 x 32, 200         33 : 10     19 x 24, 40..4450  67 : 80     64 x 4, 200..2000  33 : 49
-// Up to 16 rows it is always this one.
+// items share an SM.  Measured, us, this one : the other (sequences x new tokens, four kv heads with four heads each, context):
+//   64 x 8, 200..2000    51 : 49     256 x 8, 200..450   61 : 55     19 x 8, 40..4450   34 : 83     4 x 8, 8000     31 : 143
+//   64 x 16, 200..2000   80 : 51     256 x 16, 200..450  119 : 59    19 x 12, 40..4450  45 : 82     2 x 16, 30000   56 : 519
+//   1 x 16, 200          18 : 10     1 x 32, 200         32 : 11     19 x 24, 40..4450  67 : 83*    64 x 4, 200..2000  35 : 49
+// Up to 16 rows it is always this one.  On the line with a star the rule takes the slower side; other head layouts were not measured.
+// The choice is one for the whole batch: a prompt's piece takes the decode steps beside it along to the other kernel.
 static bool few_rows(const Kv8Attend &a, long long want, int max_len) {
     if (a.b.num_seqs > MAX_SEQS) return false;
     // units are counted in 32 bits

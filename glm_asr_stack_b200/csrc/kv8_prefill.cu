@@ -15,7 +15,7 @@
 // Bound: the two products are 2 x 128 x 64 x 128 multiply-adds a step, 512 cycles at the tensor cores' nominal rate, and the exponentials 512
 // of the special-function units.  The softmax of a step is a chain of some 2000 cycles, so two CTAs share an SM, and a CTA's scores of
 // the next step are computed under its softmax: tensor memory has two of S and one of O.  (128 keys per step with one S: 382 us
-// where this takes 345, two sequences of 2000 new tokens behind 5000; 128 columns of S are all that O leaves of the half of
+// where this took 345, two sequences of 2000 new tokens behind 5000: 320 to 330 now; 128 columns of S are all that O leaves of the half of
 // tensor memory that a CTA has.  Two threads per row, eight warps of softmax: 386.)
 //   warp 8      producer: the work items, K and V tiles (a TMA box of 2 KB per group of 16 keys), scales of each step; places in the pool are
 //               looked up 8 steps ahead, which is worth 60 us there
@@ -23,7 +23,7 @@
 //   warps 4-7   V of a step as f16 (or bf16)
 //   warps 0-3   softmax: thread = row = lane of tensor memory; it also splits its row of queries and brings out its row of the output.  The
 //               queries of the next item are asked for under its last softmax and split before its output goes out, so that the
-//               products of the next item run meanwhile (25 prompts of 400 tokens: 61.5 us, 71 one after the other)
+//               products of the next item run meanwhile (25 prompts of 400 tokens: 61.5 us, 71 one after the other; 59 now)
 // (warps 10 and 11 only give their registers to the softmax.)  The loops are kept rolled up: fully unrolled, the kernel was 92 KB of code
 // and its softmax waited for instructions, 30 cycles a key instead of 21.
 // The grid has a CTA for every work item there could be; those that run take over the items of those that have not started.
