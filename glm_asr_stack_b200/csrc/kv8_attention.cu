@@ -11,8 +11,11 @@
 //            elements down to 2^-14 of the largest, and off by 2^-22 of the largest below.
 //   weights  2^(x_j - m) v_scale_j, x_j the score in log2, spans more than 8 bits have, so the accumulator has a reference of its own
 //            beside the running maximum m of the softmax: W, the running maximum of x_j + log2 v_scale_j.  The weight
-//            2^(x_j + log2 v_scale_j - W + 6), at most 2^8, is split as p = hi + 2^-4 lo: off by 6.6e-4 of its size (rms; bf16: 1.6e-3) or 2^-20
-//            of the largest, whichever is more.
+//            2^(x_j + log2 v_scale_j - W + 12), at most 2^14, is rounded to f16, whose upper byte is an e5m2 number: that byte, the upper byte of
+//            8 times what it leaves, and of 8 times what is left then, side by side as columns: p = hi + 2^-3 mid + 2^-6 lo.  That is off by 2^-9
+//            of the weight, or 2^-35 of the largest, whichever is more: a long tail of small weights beside one token that has
+//            nearly all of it, with little V, is what counts then.  (Two e4m3 numbers per weight end at 2^-20 of the largest: 5000
+//            weights of 2^-20.6 beside one came out 26% short.)
 //   lazily   m and W are touched when a term has grown past 2^8 m or 2^2 W: an ordinary tile needs one vote of the softmax's warps.
 //   split    Two ways to deal out the work, chosen on the host (see deal_whole()).  Whole: one CTA of the grid for each (sequence, kv
 //            head); those that run take over the work of those that have not started, and there is nothing to join.  Pieces: all
@@ -45,8 +48,10 @@ constexpr int TILE_GROUPS = SOFTMAX / kKv8Group;
 constexpr int GROUP_BYTES = kKv8Group * kKv8Dim;
 constexpr int TILE_BYTES = TILE_GROUPS * GROUP_BYTES;         // 16 KB of K, or V
 constexpr int MAX_SEQS = 4096;                                // the line's table lies in shared memory
-constexpr float kTop = 8.0f, kWeightTop = 2.0f, kWeightBase = 6.0f;
-constexpr float kQLo = 1.0f / 32.0f, kPLo = 1.0f / 16.0f;
+constexpr float kTop = 8.0f, kWeightTop = 2.0f, kWeightBase = 12.0f;
+constexpr float kQLo = 1.0f / 32.0f, kPMid = 1.0f / 8.0f, kPLo = 1.0f / 64.0f;
+constexpr int PARTS = 3;                                      // numbers per weight
+constexpr int weight_columns(int used) { return (PARTS * used + 15) / 16 * 16; }
 
 enum : int { B_KFULL = 0, B_KEMPTY = 2, B_VFULL = 4, B_PVDONE = 6, B_SFULL = 8, B_SCALES = 10, B_CFULL = 12, B_CEMPTY = 14, B_PFULL = 16, B_OFREE = 17, B_NEXT = 18, B_FIRST = 19, B_COUNT = 20 };
 
@@ -62,12 +67,12 @@ struct ContextInfo {
     int pos[R];
     __nv_bfloat16 *out[R];
 };
-// Shared memory; R = query rows of a context.
-template <int R>
+// Shared memory; R = query rows of a context as the scores have them, U those that the weights have.
+template <int R, int U>
 struct Smem {
     uint8_t k[2][TILE_BYTES], v[2][TILE_BYTES];
     uint8_t q[2][2 * R * kKv8Dim];        // B operand of S^T: rows hi, then lo
-    uint8_t p[2 * R * SOFTMAX];           // B operand of O^T: per 16 columns (rows hi, then lo) 16 bytes of each token
+    uint8_t p[weight_columns(U) * SOFTMAX];   // B operand of O^T: per 16 columns (rows hi, then mid, then lo) 16 bytes of each token
     ContextInfo<R> ctx[2];
     float4 row[R];                        // m + kTop, W + kWeightTop, -m, kWeightBase - W
     float red[4][R][2], factor[R][2];
@@ -93,11 +98,25 @@ __device__ __forceinline__ bool any_of_softmax(bool x) {
         : "=r"(r) : "r"(x ? 1u : 0u), "n"(COUNT) : "memory");
     return r != 0;
 }
+// Two weights (at least 0) as f16, in the upper byte of each half: an e5m2 number, the one of 8 times the rest, and the rounded one of 8 times
+// what is left of that.  All steps but the first and the last are exact.
+__device__ __forceinline__ void split_weights(float a, float b, uint32_t &hi, uint32_t &mid, uint32_t &lo) {
+    auto bits = [](__half2 h) { return *reinterpret_cast<const uint32_t *>(&h); };
+    auto upper = [&](uint32_t w) {
+        const uint32_t u = w & 0xFF00FF00u;
+        return *reinterpret_cast<const __half2 *>(&u);
+    };
+    const __half2 eight = __float2half2_rn(8.0f), w = __floats2half2_rn(a, b);
+    hi = bits(w);
+    const __half2 m = __hmul2(__hsub2(w, upper(hi)), eight);
+    mid = bits(m);
+    lo = bits(__hmul2(__hsub2(m, upper(mid)), eight)) + 0x00800080u;
+}
 // Query rows are split by QL lanes each (all rows of a small tile at a time, or eight): a lane has dims 8 QL i + 8 (lane % QL) .. + 7.
 constexpr int query_lanes(int rows) { return rows <= 4 ? 8 : 4; }
 // Row r of context cs, which is row `row` of its sequence.
-template <int QL, int R>
-__device__ __forceinline__ void split_row(const Kv8Attend &a, Smem<R> &sm, int cs, int r, bool exists, const uint4 (&q)[16 / QL], int row, int head, int first_token, int start) {
+template <int QL, int R, int U>
+__device__ __forceinline__ void split_row(const Kv8Attend &a, Smem<R, U> &sm, int cs, int r, bool exists, const uint4 (&q)[16 / QL], int row, int head, int first_token, int start) {
     const int part = (int)threadIdx.x % QL;
     uint32_t most = 0u;
 #pragma unroll
@@ -250,14 +269,15 @@ constexpr int max_ctas(int rows) { return rows <= 8 ? 3 : 2; }
 // of the narrowest product).
 template <int R, int U>
 __global__ void __launch_bounds__(threads(R), max_ctas(R)) kv8_attend_kernel(const __grid_constant__ Params p) {
-    constexpr int N = 2 * R;                                  // columns of both products
+    constexpr int N = 2 * R, NP = weight_columns(U);          // columns of the two products
     constexpr int SPLIT = split(R), THREADS = threads(R), WORKERS = SPLIT * SOFTMAX, COPIES = WORKERS / 32, PRODUCTS = COPIES + 1;       // the last two: warps
     // The softmax's warps split the queries of the first context, all rows at once (19 sequences with 4 new tokens behind 300, 16 rows:
     // 12.1 -> 11.4 us).  Up to 8 rows the copying warp is as quick, and nobody has to be told (6.3 us, 6.6 for one of 60 tokens).
     constexpr bool SHARED_FIRST = U > 8;
-    constexpr int TMEM_COLS = 3 * N <= 64 ? 64 : 3 * N <= 128 ? 128 : 256;     // two score buffers, the accumulator
+    constexpr int TMEM_COLS = 2 * N + NP <= 64 ? 64 : 2 * N + NP <= 128 ? 128 : 256;     // two score buffers, the accumulator
+    static_assert(2 * N + NP <= 256, "tensor memory of a CTA");
     extern __shared__ __align__(1024) uint8_t smem_raw[];
-    Smem<R> &sm = *reinterpret_cast<Smem<R> *>(smem_raw);
+    Smem<R, U> &sm = *reinterpret_cast<Smem<R, U> *>(smem_raw);
     const Kv8Attend &a = p.a;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t sbase = smem_u32(smem_raw);
@@ -531,7 +551,7 @@ __global__ void __launch_bounds__(threads(R), max_ctas(R)) kv8_attend_kernel(con
         // ================================ products ==============================
         const bool leader = elect_one();
         constexpr uint32_t idesc_s = idesc_e4m3(128, N);
-        constexpr uint32_t idesc_o = idesc_e4m3(128, N) | kIdescAMnMajor | kIdescBMnMajor;
+        constexpr uint32_t idesc_o = idesc_e4m3(128, NP) | kIdescBE5m2 | kIdescAMnMajor | kIdescBMnMajor;
         const uint32_t t_o = tmem + 2 * N;
         uint32_t t = 0, contexts = 0;
         bool ok = true;
@@ -673,7 +693,7 @@ __global__ void __launch_bounds__(threads(R), max_ctas(R)) kv8_attend_kernel(con
                         for (int r = 0; r < V; ++r) sum[r] *= sm.factor[base + r][0];
                         tc_fence_after();
 #pragma unroll 1
-                        for (int part = 0; part < N; part += R) {           // hi, lo
+                        for (int part = 0; part < PARTS * U; part += U) {
                             uint32_t o[V];
                             load_columns<V>(t_o + (uint32_t)(part + base), o);
                             tmem_ld_wait();
@@ -684,21 +704,25 @@ __global__ void __launch_bounds__(threads(R), max_ctas(R)) kv8_attend_kernel(con
                         tmem_st_wait();
                     }
                 }
-                uint32_t w_hi[V / 4] = {}, w_lo[V / 4] = {};  // the token's weights as codes
+                uint32_t codes[PARTS][V / 4];                 // the token's weights
 #pragma unroll
-                for (int r = 0; r < V; r += 2) {
-                    float w[2];
+                for (int r = 0; r < V; r += 4) {
+                    uint32_t part[PARTS][2];
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const float2 ref = *reinterpret_cast<const float2 *>(&sm.row[base + r + e].z);
-                        sum[r + e] += ex2(x[r + e] + ref.x);
-                        // a token that is not seen weighs 0 whatever its block's scale is
-                        w[e] = !all && x[r + e] == -INFINITY ? 0.0f : ex2(x[r + e] + (vs + ref.y));
+                    for (int two = 0; two < 2; ++two) {
+                        float w[2];
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const int i = r + 2 * two + e;
+                            const float2 ref = *reinterpret_cast<const float2 *>(&sm.row[base + i].z);
+                            sum[i] += ex2(x[i] + ref.x);
+                            // a token that is not seen weighs 0 whatever its block's scale is
+                            w[e] = !all && x[i] == -INFINITY ? 0.0f : ex2(x[i] + (vs + ref.y));
+                        }
+                        split_weights(w[0], w[1], part[0][two], part[1][two], part[2][two]);
                     }
-                    const uint32_t hi = e4m3_split(w[0], w[1]);
-                    const uint32_t lo = e4m3x2(w[0] / kPLo, w[1] / kPLo);
-                    w_hi[r / 4] |= hi << (8 * (r & 2));
-                    w_lo[r / 4] |= lo << (8 * (r & 2));
+#pragma unroll
+                    for (int i = 0; i < PARTS; ++i) codes[i][r / 4] = __byte_perm(part[i][0], part[i][1], 0x7531);
                 }
                 // the weights of the tile before have been read
                 ok = t == 0 || mbar_wait_short(bar(B_PVDONE + (s ^ 1)), ((t - 1) >> 1) & 1u, abort_word, ST_TIMEOUT_ATTENTION);
@@ -712,16 +736,19 @@ __global__ void __launch_bounds__(threads(R), max_ctas(R)) kv8_attend_kernel(con
                     }
                 }
                 if (!ok) *abort_word = ST_TIMEOUT_ATTENTION;  // said at the next vote
-                if constexpr (R == 8) {
-                    // all 16 columns; those of rows that do not exist are zero
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(smem_u32(sm.p) + me * 16), "r"(w_hi[0]), "r"(V == 8 ? w_hi[V / 8] : 0u), "r"(w_lo[0]),
-                                 "r"(V == 8 ? w_lo[V / 8] : 0u) : "memory");
+                const uint32_t to = smem_u32(sm.p) + me * 16;
+                if constexpr (V == 4) {                       // 16 columns, the last four of which nobody reads
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %3};" ::"r"(to), "r"(codes[0][0]), "r"(codes[1][0]), "r"(codes[2][0]) : "memory");
                 } else {
 #pragma unroll
-                    for (int i = 0; i < V / 4; ++i) {
-                        const int hi = base + 4 * i, lo = R + hi;
-                        *reinterpret_cast<uint32_t *>(sm.p + hi / 16 * (16 * SOFTMAX) + me * 16 + hi % 16) = w_hi[i];
-                        *reinterpret_cast<uint32_t *>(sm.p + lo / 16 * (16 * SOFTMAX) + me * 16 + lo % 16) = w_lo[i];
+                    for (int i = 0; i < PARTS; ++i) {
+#pragma unroll
+                        for (int r = 0; r < V; r += V % 8 == 0 ? 8 : 4) {
+                            const int at = i * U + base + r;
+                            const uint32_t dst = to + (uint32_t)(at / 16 * (16 * SOFTMAX) + at % 16);
+                            if constexpr (V % 8 == 0) asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(dst), "r"(codes[i][r / 4]), "r"(codes[i][r / 4 + 1]) : "memory");
+                            else asm volatile("st.shared.b32 [%0], %1;" ::"r"(dst), "r"(codes[i][r / 4]) : "memory");
+                        }
                     }
                 }
                 fence_proxy_async_smem();
@@ -763,9 +790,10 @@ __global__ void __launch_bounds__(threads(R), max_ctas(R)) kv8_attend_kernel(con
                 else p.part.stats[(size_t)c.slot * U + tid] = make_float4(-st.z, l, -st.w, 0.0f);
             }
             tc_fence_after();
-            uint32_t high[V], low[V];
+            uint32_t high[V], mid[V], low[V];
             load_columns<V>(t_o + (uint32_t)base, high);
-            load_columns<V>(t_o + (uint32_t)(R + base), low);
+            load_columns<V>(t_o + (uint32_t)(U + base), mid);
+            load_columns<V>(t_o + (uint32_t)(2 * U + base), low);
             tmem_ld_wait();
             tc_fence_before();
             mbar_arrive_warp(bar(B_OFREE));
@@ -774,7 +802,7 @@ __global__ void __launch_bounds__(threads(R), max_ctas(R)) kv8_attend_kernel(con
 #pragma unroll
             for (int r = 0; r < V; ++r) {
                 if (base + r >= c.rows) break;
-                const float o = fmaf(__uint_as_float(low[r]), kPLo, __uint_as_float(high[r]));
+                const float o = fmaf(__uint_as_float(low[r]), kPLo, fmaf(__uint_as_float(mid[r]), kPMid, __uint_as_float(high[r])));
                 if (c.slot < 0) c.out[base + r][me] = __float2bfloat16(o * sm.factor[base + r][0]);
                 else to[(base + r) * kKv8Dim] = o;
             }
@@ -843,12 +871,12 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) kv8_join_kernel(const __grid_
 
 constexpr int kSmemPerSm = 228 * 1024, kSmemReserved = 1024;       // of an SM; taken by the system from each CTA
 
-template <int R>
-size_t smem_bytes(int num_seqs) { return sizeof(Smem<R>) + (size_t)num_seqs * sizeof(int); }
+template <int R, int U>
+size_t smem_bytes(int num_seqs) { return sizeof(Smem<R, U>) + (size_t)num_seqs * sizeof(int); }
 // CTAs per SM that the launch bounds and the shared memory allow
-template <int R>
+template <int R, int U>
 int ctas_per_sm(int num_seqs) {
-    const int fit = (int)(kSmemPerSm / (smem_bytes<R>(num_seqs) + kSmemReserved));
+    const int fit = (int)(kSmemPerSm / (smem_bytes<R, U>(num_seqs) + kSmemReserved));
     return fit < 1 ? 1 : fit > max_ctas(R) ? max_ctas(R) : fit;
 }
 
@@ -856,15 +884,15 @@ template <int R, int U>
 bool launch_rows(Params &p, void *workspace, int num_seqs, cudaStream_t st, int &grid) {
     static PerDevice<bool> configured;
     const cudaError_t ready = once_per_device(configured, [] {
-        const cudaError_t e = cudaFuncSetAttribute(kv8_attend_kernel<R, U>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes<R>(MAX_SEQS));
+        const cudaError_t e = cudaFuncSetAttribute(kv8_attend_kernel<R, U>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes<R, U>(MAX_SEQS));
         if (e != cudaSuccess) return e;
         return cudaFuncSetAttribute(kv8_attend_kernel<R, U>, cudaFuncAttributePreferredSharedMemoryCarveout, (int)cudaSharedmemCarveoutMaxShared);
     });
     if (ready != cudaSuccess) return false;
-    grid = num_sms() * ctas_per_sm<R>(num_seqs);
+    grid = num_sms() * ctas_per_sm<R, U>(num_seqs);
     if (p.whole) grid = num_seqs * p.a.b.kv_heads;
     partial_bytes(grid, U, workspace, &p.part);
-    return launch_chained(kv8_attend_kernel<R, U>, dim3(grid), dim3(threads(R)), smem_bytes<R>(num_seqs), st, p) == cudaSuccess;
+    return launch_chained(kv8_attend_kernel<R, U>, dim3(grid), dim3(threads(R)), smem_bytes<R, U>(num_seqs), st, p) == cudaSuccess;
 }
 
 }  // namespace

@@ -5,9 +5,10 @@
 //                     element to 2^7 and split into two e4m3 numbers, q = hi + lo, both products into the same sums: exact for
 //                     elements down to 2^-9 of the largest, off by 2^-17 of the largest below.  Two products of 8-bit operands
 //                     cost what one of 16-bit operands does, and no key is converted.
-//   p = 2^(x - m)     x = s * (row scale) * (K scale of the block of 16 keys), in one pass over the scores: m moves when a weight would be
-//                     above 2^8, and only then is O touched.
-//   O += P V          f16 x f16: weights have 11 bits down to 2^-14 of the largest, and are off by 2^-25 of it below.  V's codes become
+//   p = 2^(x - m + 9) x = s * (row scale) * (K scale of the block of 16 keys), in one pass over the scores: m moves when a weight would be
+//                     above 2^15, and only then is O touched.
+//   O += P V          f16 x f16: weights have 11 bits down to 2^-23 of the largest, and are off by 2^-34 of it below, which a long tail of
+//                     small weights can do with.  (At most 2^8 and from 2^0 on they lost tails: 2^-26 each came out as 0.)  V's codes become
 //                     f16, times the scale of their block over the largest scale of the item so far (exact: a power of two),
 //                     which O is expressed against.  Once the scales of an item's blocks, in whatever order they come, are more than 2^5
 //                     apart (a block of zeros has the smallest one there is), small weights on large values may be what counts: from
@@ -45,7 +46,7 @@ constexpr int QT = 128, KT = 64, THREADS = 384;
 constexpr int REGS_SOFTMAX = 128, REGS_VALUES = 56, REGS_REST = 56;
 constexpr int GROUPS = KT / kKv8Group, GROUP_BYTES = kKv8Group * kKv8Dim;
 constexpr int TMEM_COLS = 256, COL_O = 128;
-constexpr float kLazy = 8.0f;                 // log2: the reference moves when a weight would be above 2^8
+constexpr float kBase = 9.0f, kLazy = 6.0f;   // log2: weights at the reference, and how far above it before that moves (f16 ends below 2^16)
 constexpr float kF16Range = 1.0f / 32.0f;     // smallest over largest V scale of an item's steps so far that f16 weights are taken for
 
 static_assert(GROUPS == 4, "a step's K scales are read as one float4");
@@ -557,7 +558,7 @@ __global__ void __launch_bounds__(THREADS, 2) kv8_prefill_kernel(const __grid_co
                     scale_columns(t_o, factor);
                 }
                 unsigned long long sum2[2] = {pack_f32x2(0.0f, 0.0f), pack_f32x2(0.0f, 0.0f)};
-                const unsigned long long neg_m2 = pack_f32x2(-m, -m);
+                const unsigned long long neg_m2 = pack_f32x2(kBase - m, kBase - m);
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     uint32_t w[16];

@@ -451,6 +451,7 @@ __host__ __device__ constexpr uint32_t idesc_bf16(int m, int n) {
 __host__ __device__ constexpr uint32_t idesc_e4m3(int m, int n) {
     return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
+constexpr uint32_t kIdescBE5m2 = 1u << 10;      // kind::f8f6f4: B is e5m2
 constexpr uint32_t kIdescAMnMajor = 1u << 15;   // A is MN-major
 constexpr uint32_t kIdescBMnMajor = 1u << 16;   // B is MN-major (both operands are K-major without it)
 // Instruction descriptor, kind::mxf4nvf4: e2m1 x e2m1, ue4m3 scales, K = 64, K-major.

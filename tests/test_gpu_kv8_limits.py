@@ -405,3 +405,53 @@ def test_pieces_captured_replayed_and_on_two_streams(new):
             assert torch.equal(out, want)
             assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(pool, eager))
     assert ops.status() == 0
+
+
+def beside_a_sink(tokens, new, score, page=64, seed=0):
+    """The first token has a score so far above the others' that it has nearly all the weight, and V codes of 0 in a block of ordinary ones:
+    the result is what the others, one small weight each, add up to."""
+    b = Batch([new], [tokens - new], 1, 4, page, seed=seed)
+    k, v, ks, vs = b.codes[0], b.codes[1], b.scales[0], b.scales[1]
+    k[...], ks[...], vs[...] = 0, 1.0, 1.0
+    v[...] = ref.e4m3(b.rng.uniform(2.0, 3.5, v.shape))
+    first = b.tables[0, 0]
+    k[first, 0, 0, 0], v[first, 0, 0] = ref.e4m3(np.array([float(score)]))[0], 0
+    assert ref.VALUE[k[first, 0, 0, 0]] == score
+    q = np.zeros((new, b.heads, ref.DIM))
+    q[:, :, 0] = STRETCH
+    return b, q
+
+
+def sink_bound(b, q, row, score):
+    """Weights off by 2^-8 of themselves; small ones by half the step that they are held in, 2^-34 of the largest (f16 steps of 2^-24 below a
+    reference of at least 2^9; e5m2 steps of 2^-16 over 2^6 below one of at least 2^12: 2^-35)."""
+    length = b.lens[0] - b.new[0] + row + 1
+    at = np.arange(length)
+    v = ref.VALUE[b.codes[1][b.tables[0, at // b.page], 0, at % b.page]]
+    w = np.full(length, 2.0 ** -(STRETCH * score))
+    w[0] = 1.0
+    w /= w.sum()
+    want = w @ v
+    return want, 2.0 ** -8 * np.abs(want) + (2.0 ** -8 + 2.0 ** -19) * 2 * (w @ np.abs(v)) + 2.0 ** -34 * np.abs(v).sum(0)
+
+
+@pytest.mark.parametrize("tokens,score", [(130, 14), (300, 18), (300, 22), (5000, 16), (5000, 20), (5000, 24), (30_000, 20), (30_000, 24), (30_000, 28)])
+@pytest.mark.parametrize("new", [1, 3, 40])
+def test_many_small_weights_beside_one_that_has_nearly_all(tokens, score, new):
+    b, q = beside_a_sink(tokens, new, score)
+    pool, tables, lens, cu = b.device()
+    for max_new in (1, 100_000):
+        out = ops.kv8_attention(dev(q), *pool, tables, lens, cu, max_new=max_new, scale=LN2).float().cpu().numpy()
+        for row in {0, new // 2, new - 1}:
+            want, tol = sink_bound(b, q, row, score)
+            assert np.all(np.abs(out[row] - want) <= tol), (max_new, row, (np.abs(out[row] - want) / tol).max(), (out[row] / want).mean())
+    assert ops.status() == 0
+
+
+@pytest.mark.parametrize("tokens,score", [(300, 22), (5000, 24)])
+def test_pieces_with_many_small_weights_beside_one(tokens, score):
+    b, q = beside_a_sink(tokens, 2, score)
+    out = in_pieces(b, q, 400, max_new=2, scale=LN2).float().cpu().numpy()
+    for row in range(2):
+        want, tol = sink_bound(b, q, row, score)
+        assert np.all(np.abs(out[row] - want) <= tol), (row, (np.abs(out[row] - want) / tol).max())
