@@ -889,10 +889,10 @@ bool launch_rows(Params &p, void *workspace, int num_seqs, cudaStream_t st, int 
         return cudaFuncSetAttribute(kv8_attend_kernel<R, U>, cudaFuncAttributePreferredSharedMemoryCarveout, (int)cudaSharedmemCarveoutMaxShared);
     });
     if (ready != cudaSuccess) return false;
-    grid = num_sms() * ctas_per_sm<R, U>(num_seqs);
-    if (p.whole) grid = num_seqs * p.a.b.kv_heads;
+    const int line = p.whole ? 0 : num_seqs;              // whole contexts need no table of the line
+    grid = p.whole ? num_seqs * p.a.b.kv_heads : num_sms() * ctas_per_sm<R, U>(line);
     partial_bytes(grid, U, workspace, &p.part);
-    return launch_chained(kv8_attend_kernel<R, U>, dim3(grid), dim3(threads(R)), smem_bytes<R, U>(num_seqs), st, p) == cudaSuccess;
+    return launch_chained(kv8_attend_kernel<R, U>, dim3(grid), dim3(threads(R)), smem_bytes<R, U>(line), st, p) == cudaSuccess;
 }
 
 }  // namespace
